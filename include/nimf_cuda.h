@@ -334,6 +334,130 @@ int nimf_embedding_lookup_dev(const float* table, int64_t vocab, int64_t dim,
 int nimf_greedy_sample_dev(const float* logits, int64_t rows, int64_t vocab, const int32_t* recent,
                            int64_t n_recent, float repeat_penalty, int32_t* out_ids, void* stream);
 
+/* Log-probabilities of given tokens with their rank, the entropy of each row
+ * and its n_top most likely tokens (no reference counterpart; beside the
+ * greedy choice above, on the same logits [rows][vocab]).  Per row, with
+ * p = softmax(logits):
+ *   logprob[row]  = log p(ids[row]); -inf for an id outside [0, vocab)
+ *   entropy[row]  = -sum p log p
+ *   rank[row]     = 1 + the number of logits above the given token's (0 for an
+ *                   id outside [0, vocab))
+ *   top_ids / top_logprobs [row][n_top]: the largest logits in falling order,
+ *                   equal ones by index; a NaN counts as -inf in that order
+ * logprob, entropy and rank are nullable (logprob and rank need ids, ids may
+ * be NULL without them); n_top 0 .. 32, at most vocab (0: no alternatives).
+ * A row with a NaN or +inf gives NaN log-probabilities and entropy; a row of
+ * -inf only gives log-probabilities -inf and entropy 0.  The logits are read
+ * once and not modified; vocab <= 262144.  No workspace, nothing allocated. */
+int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t vocab, const int32_t* ids,
+                      int64_t n_top, float* logprob, float* entropy, int32_t* rank,
+                      int32_t* top_ids, float* top_logprobs, void* stream);
+
+/* ------------------------------------------------------------ 4-bit paged KV cache */
+/* Attention of many requests over one pool of cache blocks whose keys and
+ * values are held in 4 bits (no reference counterpart: the reference's caches
+ * are fp32 and contiguous, nim_inference.nim:404-426).  A step is
+ *   reserve   block tables, slots and positions of the new tokens
+ *   append    RoPE of the new queries and keys; keys and values coded into
+ *             their slots
+ *   attention causal attention of the new tokens, prompts and single tokens
+ *             mixed in one call
+ * and release when requests finish.  All buffers are device buffers owned by
+ * the caller; the calls are asynchronous on `stream` (NULL: the library
+ * stream), allocate nothing and can be captured in a CUDA graph.
+ *
+ * The cache is n_blocks * n_kv_heads * block_size / 16 tiles of
+ *   16 * head_dim + 256 * (head_dim / group) bytes,
+ * a tile holding 16 tokens of one KV head.  Each group of `group` channels of
+ * a token is coded with its own scale and minimum (float32):
+ *   scale = (max - min) / 15, code = min(15, round((x - min) / scale)),
+ * every step rounded to float32, halves to even; a code stands for
+ * code * scale + min (a minimum of -0 is kept as 0).  A group holding a NaN, an infinity or a range above the
+ * largest float stands for NaN.  head_dim 64, 128 or 256; group 32, 64 or 128,
+ * at most head_dim; block_size a multiple of 16 up to 4096;
+ * n_blocks * block_size below 2^31.  Slot s is token s % block_size of block
+ * s / block_size. */
+typedef struct nimf_kv4_desc {
+  int64_t n_blocks, n_kv_heads, head_dim, block_size, group;
+} nimf_kv4_desc;
+
+/* Bytes of a cache (host only).  The buffer is 16-byte aligned and needs no
+ * initial contents. */
+int nimf_kv4_cache_bytes(const nimf_kv4_desc* desc, int64_t* bytes);
+
+/* Makes room for n_new[b] more tokens of each of n_seqs requests, in order.
+ * Request b holds lens[b] tokens in the blocks block_table[b][0 ..
+ * ceil(lens[b] / block_size)), rows of max_blocks entries; free_blocks
+ * [n_blocks] is a stack of n_free[0] block ids.  A request is granted when
+ * lens + n_new fits max_blocks blocks, its rows end at or before max_rows, and
+ * it needs no block or all that it and the requests before it need are free;
+ * a refused one changes nothing, and those after it may still be granted if
+ * they need no block.  Fresh blocks are taken from the top of the stack, which
+ * itself is not changed.  Writes
+ *   cu_rows [n_seqs + 1]   first row of each request's new tokens (prefix
+ *                          sums of n_new, granted or not)
+ *   lens_out [n_seqs]      lens + n_new where granted, else lens (may be lens)
+ *   n_free_out [1]         what is left on the stack (may be n_free)
+ *   slots [max_rows]       slot of each new row; -1 for refused requests and
+ *                          for the rows behind the last request
+ *   positions [max_rows]   its position in its request (0 where slot is -1)
+ *   granted [n_seqs]       1 or 0
+ * and the fresh entries of block_table.  Negative lens or n_new count as 0. */
+int nimf_kv4_reserve_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
+                         const int32_t* n_new, const int32_t* lens, int32_t* lens_out,
+                         int32_t* block_table, const int32_t* free_blocks, const int32_t* n_free,
+                         int32_t* n_free_out, int64_t max_rows, int32_t* cu_rows, int32_t* slots,
+                         int32_t* positions, int32_t* granted, void* stream);
+
+/* Puts the blocks of every request with finished[b] != 0 back on the stack (in
+ * the order of the requests and their tables) and sets its lens[b] to 0.  More
+ * blocks than n_blocks on the stack are dropped, which nimf_sync reports
+ * (NIMF_ERR_TIMEOUT-class device error 5). */
+int nimf_kv4_release_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
+                         const int32_t* finished, int32_t* lens, const int32_t* block_table,
+                         int32_t* free_blocks, int32_t* n_free, void* stream);
+
+/* Codes k, v [rows][n_kv_heads][head_dim] into slots[rows]; rows with a
+ * negative slot append nothing.  With cos_t / sin_t [max_seq][head_dim / 2]
+ * (nullable together) k is rotated at positions[row] first, and so is q
+ * [rows][n_heads][head_dim] into q_out (nullable together; q_out may be q); k
+ * and v are not modified.  Without tables q is copied.  The slots of one call
+ * must differ (equal ones leave a mixture of their rows).  A slot past the
+ * cache or a position outside [0, max_seq) appends nothing and makes nimf_sync
+ * report the NIMF_ERR_TIMEOUT-class device error 4.  Buffers 16-byte aligned. */
+int nimf_kv4_append_dev(const nimf_kv4_desc* desc, void* cache, const float* k, const float* v,
+                        int64_t rows, const int32_t* slots, const float* q, float* q_out,
+                        int64_t n_heads, const int32_t* positions, const float* cos_t,
+                        const float* sin_t, int64_t max_seq, void* stream);
+
+/* The values that slots[rows] stand for, k and v [rows][n_kv_heads][head_dim]
+ * (code * scale + min, rounded after the product and after the sum); zeros for
+ * a negative slot, and for one past the cache (reported as in append). */
+int nimf_kv4_read_dev(const nimf_kv4_desc* desc, const void* cache, const int32_t* slots,
+                      int64_t rows, float* k, float* v, void* stream);
+
+/* Bytes of attention's workspace for this cache (after nimf_init).  It needs
+ * no initial contents; two calls that may overlap need one each. */
+int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int64_t* bytes);
+
+/* out[t][h] = softmax(scale * q[t][h] . K) V over the cached tokens that row t
+ * sees, KV head h / (n_heads / n_kv_heads).  q and out are [rows][n_heads]
+ * [head_dim]; sequence b has the rows [cu_rows[b], cu_rows[b + 1]) (cu_rows
+ * NULL: row b alone), which are its last lens[b] tokens: row i of n sees the
+ * tokens 0 .. lens[b] - n + i, the cache holding them all (append first).  A
+ * row that sees nothing gives zeros; rows of no sequence are left as they
+ * were.  max_new is the largest number of rows of a sequence as the host knows
+ * it (a hint that chooses kernels, 1 for a decode step; results do not depend
+ * on its being right).  A block id outside the cache leaves its tokens out and
+ * makes nimf_sync report device error 4.  Scores, softmax and sums are float32;
+ * q and the probabilities enter the tensor cores as two fp16 terms each, the
+ * codes exactly.  Results do not depend on timing.  Buffers 16-byte aligned. */
+int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const float* q,
+                           int64_t rows, int64_t n_heads, int64_t n_seqs, const int32_t* cu_rows,
+                           const int32_t* lens, const int32_t* block_table, int64_t max_blocks,
+                           int64_t max_new, float scale, float* out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ whole decode step */
 /* One decode token of a Llama-style stack with int4 group-128 weights as ONE
  * persistent, cooperative launch: LlamaModelL.forwardStep(ids = [token],

@@ -1,0 +1,131 @@
+// kv4.cuh -- the 4-bit paged key/value cache shared by its kernels: where a
+// tile's parts lie, where a channel's code sits in its row, and the launch
+// helper of the entry points.
+//
+// The cache is [n_blocks][n_kv_heads][block_size / 16] tiles.  A tile holds 16
+// tokens of one KV head in one contiguous piece, so that a bulk copy brings
+// everything attention needs of them:
+//   K codes [16][D/2] | V codes [16][D/2] | K {scale, min} [D/G][16] | V {scale, min} [D/G][16]
+// A code c of a group with {scale, min} stands for c * scale + min.
+// The order of a row's channels is the one in which mma.m16n8k16 takes them:
+//   K: lane quad member c reads the words c*(D/32) .. of its row in one vector
+//      load; word j of them holds channels 32j + 8c .. + 7, so the 32 channels
+//      of one chunk j (never more than one group) feed the same two MMAs.
+//   V: lane group g reads the words g*(D/64) ..; word s of them holds channels
+//      64s + 4g .. + 3 in its low half and 64s + 32 + 4g .. + 3 in its high
+//      half, so an 8-wide output tile never spans two groups of 32 either.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+#include "device_util.cuh"
+#include "nimf_internal.h"
+
+namespace nimf {
+namespace kv4 {
+
+constexpr int kTile = 16;  // tokens of a tile
+
+// Sizes of a cache as the kernels take them.
+struct Shape {
+  int64_t n_blocks = 0;
+  int hkv = 0, d = 0, bs = 0, group = 0;
+};
+
+__host__ __device__ constexpr int tile_bytes(int d, int ng) { return kTile * d + 2 * kTile * 8 * ng; }
+__host__ __device__ constexpr int v_codes_at(int d) { return kTile * d / 2; }
+__host__ __device__ constexpr int k_params_at(int d) { return kTile * d; }
+__host__ __device__ constexpr int v_params_at(int d, int ng) { return kTile * d + kTile * 8 * ng; }
+
+// Byte and nibble (0: low) of channel ch in a K or V row of D channels.
+__host__ __device__ constexpr int k_byte(int ch, int d) {
+  return (((ch % 32) / 8) * (d / 32) + ch / 32) * 4 + (ch % 8) / 2;
+}
+__host__ __device__ constexpr int v_byte(int ch, int d) {
+  return (((ch % 32) / 4) * (d / 64) + ch / 64) * 4 + ((ch % 64) / 32) * 2 + (ch % 4) / 2;
+}
+
+// Checks a descriptor (NIMF_ERR_SHAPE / NIMF_ERR_ARG) and copies it.
+int check_desc(const nimf_kv4_desc* desc, const char* who, Shape* out);
+
+int stream_of(void* stream, cudaStream_t* st);
+
+// Lets a kernel use `bytes` of dynamic shared memory (asked of the driver once
+// per kernel and device binding).
+int allow_smem(const void* kern, int bytes);
+
+// Launch with programmatic dependent launch allowed; every kernel launched
+// this way waits (griddep_wait) before it touches memory.
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+           unsigned cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  NIMF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ((KArgs)args)...));
+  return NIMF_OK;
+}
+
+// Cluster barrier halves (every thread of every CTA of the cluster).
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// Inclusive sum over the block's threads (blockDim.x a multiple of 32, at most
+// 1024) of one value each; *total receives the block's sum.  sh: 33 words.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* sh, T* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    T w = lane < nw ? sh[lane] : (T)0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const T u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
+    }
+    sh[lane] = w;
+  }
+  __syncthreads();
+  if (warp > 0) v += sh[warp - 1];
+  *total = sh[nw - 1];
+  return v;
+}
+
+}  // namespace kv4
+}  // namespace nimf

@@ -1,0 +1,513 @@
+// kv4_pool.cu -- bookkeeping and contents of the 4-bit paged KV cache: block
+// tables, slot maps and positions from the requests' lengths, the return of
+// finished requests' blocks, the coding of new keys and values into their
+// slots, and reading rows back.
+#include <cfloat>
+
+#include "kv4.cuh"
+
+namespace nimf {
+namespace kv4 {
+
+int check_desc(const nimf_kv4_desc* desc, const char* who, Shape* out) {
+  if (!desc) return set_error(NIMF_ERR_ARG, "%s: NULL descriptor", who);
+  const int64_t d = desc->head_dim, g = desc->group, bs = desc->block_size;
+  if ((d != 64 && d != 128 && d != 256) || (g != 32 && g != 64 && g != 128) || g > d ||
+      bs < kTile || bs > 4096 || bs % kTile || desc->n_kv_heads < 1 || desc->n_kv_heads > 65535 ||
+      desc->n_blocks < 1 || desc->n_blocks > INT32_MAX / bs)
+    return set_error(NIMF_ERR_SHAPE,
+                     "%s: n_blocks %lld n_kv_heads %lld head_dim %lld (64, 128 or 256) block_size "
+                     "%lld (a multiple of 16, <= 4096) group %lld (32, 64 or 128, <= head_dim); "
+                     "n_blocks * block_size below 2^31",
+                     who, (long long)desc->n_blocks, (long long)desc->n_kv_heads, (long long)d,
+                     (long long)bs, (long long)g);
+  out->n_blocks = desc->n_blocks;
+  out->hkv = (int)desc->n_kv_heads;
+  out->d = (int)d;
+  out->bs = (int)bs;
+  out->group = (int)g;
+  return NIMF_OK;
+}
+
+int stream_of(void* stream, cudaStream_t* st) {
+  Context* c;
+  NIMF_TRY(require_ctx(&c));
+  *st = stream ? (cudaStream_t)stream : c->stream;
+  return NIMF_OK;
+}
+
+int allow_smem(const void* kern, int bytes) {
+  struct Done {
+    const void* kern;
+    int device, bytes;
+  };
+  static Done done[32];                      // zero: a free place
+  const int device = ctx()->device;
+  Done* d = done;
+  while (d < done + 31 && d->kern && d->kern != kern) ++d;
+  if (d->kern == kern && d->device == device && d->bytes >= bytes) return NIMF_OK;
+  NIMF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  *d = {kern, device, bytes};
+  return NIMF_OK;
+}
+
+namespace {
+
+constexpr int kPoolThreads = 1024;
+
+// Block tables and slot maps of one step.  Over the requests in order:
+//   rows(b) = [cu(b), cu(b) + new(b))              prefix sum of the new tokens
+//   need(b) = ceil((len + new) / bs) - ceil(len / bs)   where the request fits
+//   granted = fits and (need == 0 or its inclusive sum of needs <= n_free)
+// The sum never falls, so the granted needs are the first ones and the j-th
+// fresh block of request b is free[n_free - 1 - (sum before b) - j].  A new
+// row's block is either an old entry of the table or one of those, so no row
+// waits for a table entry to be written; the row that opens a block writes it.
+//
+// The cost is latency (a few dependent loads, two scans of 1,024 requests and
+// a search), not bytes.  Every CTA of the one cluster scans all requests and
+// they share the rows; lens may be its own output, so the CTAs meet between
+// reading a chunk of requests and CTA 0 writing it.
+__global__ void __launch_bounds__(kPoolThreads)
+    reserve_kernel(int64_t n_seqs, int64_t width, int bs, int64_t n_blocks,
+                   const int32_t* __restrict__ n_new, const int32_t* lens, int32_t* lens_out,
+                   int32_t* table, const int32_t* __restrict__ free_blocks, const int32_t* n_free_in,
+                   int32_t* n_free_out, int64_t max_rows, int32_t* __restrict__ cu_rows,
+                   int32_t* __restrict__ slots, int32_t* __restrict__ positions,
+                   int32_t* __restrict__ granted) {
+  __shared__ int64_t sh[33];
+  __shared__ int64_t s_cu[kPoolThreads];    // first row of each request of the chunk
+  __shared__ int64_t s_off[kPoolThreads];   // fresh blocks before it; -1: not granted
+  __shared__ int32_t s_len[kPoolThreads];
+  griddep_launch_dependents();
+  griddep_wait();
+  const unsigned rank = cluster_rank(), ctas = cluster_size();
+  const int tid = threadIdx.x;
+  const int64_t nf = min((int64_t)max(n_free_in[0], 0), n_blocks);
+  int64_t cu_base = 0, need_base = 0, taken = 0;
+  for (int64_t b0 = 0; b0 < n_seqs; b0 += kPoolThreads) {
+    const int64_t b = b0 + tid;
+    const bool live = b < n_seqs;
+    const int64_t len = live ? max(lens[b], 0) : 0;
+    const int64_t nw = live ? max(n_new[b], 0) : 0;
+    int64_t rows_total, need_total;
+    const int64_t cu_end = cu_base + block_scan<int64_t>(nw, sh, &rows_total);
+    const int64_t have = (len + bs - 1) / bs, total = (len + nw + bs - 1) / bs;
+    const bool fits = live && total <= width && cu_end <= max_rows;
+    const int64_t need = fits ? total - have : 0;
+    const int64_t upto = need_base + block_scan<int64_t>(need, sh, &need_total);
+    const bool ok = fits && (need == 0 || upto <= nf);
+    __syncthreads();
+    s_cu[tid] = cu_end - nw;
+    s_off[tid] = ok ? upto - need : -1;
+    s_len[tid] = (int32_t)len;
+    int64_t chunk_taken;
+    block_scan<int64_t>(ok ? need : 0, sh, &chunk_taken);
+    cluster_arrive();
+    cluster_wait();  // every CTA has read this chunk's lens
+    if (rank == 0 && live) {
+      lens_out[b] = (int32_t)(ok ? len + nw : len);
+      granted[b] = ok ? 1 : 0;
+      cu_rows[b] = (int32_t)min(cu_end - nw, (int64_t)INT32_MAX);
+      if (b == n_seqs - 1) cu_rows[n_seqs] = (int32_t)min(cu_end, (int64_t)INT32_MAX);
+    }
+    const int cnt = (int)min((int64_t)kPoolThreads, n_seqs - b0);
+    const int64_t row_end = min(cu_base + rows_total, max_rows);
+    for (int64_t t = cu_base + (int64_t)rank * kPoolThreads + tid; t < row_end;
+         t += (int64_t)ctas * kPoolThreads) {
+      int lo = 0, hi = cnt - 1;  // the last request whose first row is <= t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_cu[mid] <= t) lo = mid; else hi = mid - 1;
+      }
+      int32_t slot = -1, pos = 0;
+      if (s_off[lo] >= 0) {
+        const int64_t p = s_len[lo] + (t - s_cu[lo]);
+        const int64_t page = p / bs, old = (s_len[lo] + bs - 1) / bs;
+        int32_t* entry = table + (b0 + lo) * width + page;
+        int32_t blk;
+        if (page < old) {
+          blk = *entry;
+        } else {
+          blk = free_blocks[nf - 1 - s_off[lo] - (page - old)];
+          if (p % bs == 0) *entry = blk;
+        }
+        pos = (int32_t)p;
+        slot = blk >= 0 && blk < n_blocks ? (int32_t)(blk * (int64_t)bs + p % bs) : -1;
+      }
+      slots[t] = slot;
+      positions[t] = pos;
+    }
+    cu_base += rows_total;
+    need_base += need_total;
+    taken += chunk_taken;
+    __syncthreads();
+  }
+  for (int64_t t = cu_base + (int64_t)rank * kPoolThreads + tid; t < max_rows;
+       t += (int64_t)ctas * kPoolThreads) {
+    slots[t] = -1;
+    positions[t] = 0;
+  }
+  cluster_arrive();
+  cluster_wait();  // every CTA has read n_free
+  if (rank == 0 && tid == 0) {
+    n_free_out[0] = (int32_t)(nf - taken);
+    if (n_seqs == 0) cu_rows[0] = 0;
+  }
+}
+
+// Returns the blocks of the finished requests to the free list, in the order
+// of the requests and of their tables, and empties those requests.  One CTA:
+// a step finishes few requests.
+__global__ void __launch_bounds__(kPoolThreads)
+    release_kernel(int64_t n_seqs, int64_t width, int bs, int64_t n_blocks,
+                   const int32_t* __restrict__ finished, int32_t* __restrict__ lens,
+                   const int32_t* __restrict__ table, int32_t* __restrict__ free_blocks,
+                   int32_t* __restrict__ n_free, int* err) {
+  __shared__ int64_t sh[33];
+  __shared__ int64_t s_off[kPoolThreads];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x;
+  int64_t top = min((int64_t)max(n_free[0], 0), n_blocks);
+  for (int64_t b0 = 0; b0 < n_seqs; b0 += kPoolThreads) {
+    const int64_t b = b0 + tid;
+    const bool live = b < n_seqs && finished[b] != 0;
+    const int64_t pages = live ? min(((int64_t)max(lens[b], 0) + bs - 1) / bs, width) : 0;
+    int64_t total;
+    const int64_t upto = block_scan<int64_t>(pages, sh, &total);
+    s_off[tid] = upto - pages;
+    __syncthreads();
+    const int cnt = (int)min((int64_t)kPoolThreads, n_seqs - b0);
+    for (int64_t i = tid; i < total; i += kPoolThreads) {
+      int lo = 0, hi = cnt - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_off[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      if (top + i < n_blocks)
+        free_blocks[top + i] = table[(b0 + lo) * width + (i - s_off[lo])];
+      else if (err)
+        atomicExch(err, 5);  // more blocks returned than there are
+    }
+    if (live) lens[b] = 0;
+    top = min(top + total, n_blocks);
+    __syncthreads();
+  }
+  if (tid == 0) n_free[0] = (int32_t)top;
+}
+
+__device__ __forceinline__ float group_min(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float group_max(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// VPL consecutive floats of a row.
+template <int VPL>
+__device__ __forceinline__ void load_row(const float* p, float (&x)[VPL]) {
+  if constexpr (VPL == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x;
+    x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = v.x;
+      x[4 * i + 1] = v.y;
+      x[4 * i + 2] = v.z;
+      x[4 * i + 3] = v.w;
+    }
+  }
+}
+template <int VPL>
+__device__ __forceinline__ void store_row(float* p, const float (&x)[VPL]) {
+  if constexpr (VPL == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  }
+}
+
+// Rotate-half with the row's table entries, each product and sum rounded (as
+// nimf_rope_dev).  Lane l holds channels l*VPL ..; the other half of a pair is
+// in lane l ^ 16.
+template <int VPL>
+__device__ __forceinline__ void rotate(float (&x)[VPL], const float* cos_row, const float* sin_row,
+                                       int lane) {
+  const int at = (lane & 15) * VPL;
+  const bool upper = lane >= 16;
+  float c[VPL], s[VPL];
+  load_row<VPL>(cos_row + at, c);
+  load_row<VPL>(sin_row + at, s);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const float o = __shfl_xor_sync(0xffffffffu, x[i], 16);
+    x[i] = upper ? __fadd_rn(__fmul_rn(o, s[i]), __fmul_rn(x[i], c[i]))
+                 : __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o, s[i]));
+  }
+}
+
+// One warp per row and head: the query heads are rotated, the key heads
+// rotated and coded, the value heads coded.  A lane holds D/32 neighbouring
+// channels, a group lies within G / (D/32) lanes.
+//   scale = (max - min) / 15, code = min(15, round((x - min) / scale)),
+// rounded to float at each step, so the codes do not depend on the order of
+// anything.  A group with a NaN, an infinity or a range above the largest
+// float gets NaN as scale and minimum: all it stands for is NaN.
+template <int VPL>
+__global__ void __launch_bounds__(256)
+    append_kernel(const float* q, float* q_out, int h, const float* __restrict__ k,
+                  const float* __restrict__ v, int64_t rows, const int32_t* __restrict__ slots,
+                  const int32_t* __restrict__ positions, const float* __restrict__ cos_t,
+                  const float* __restrict__ sin_t, int64_t max_seq, uint8_t* __restrict__ cache,
+                  int hkv, int bs, int group, int64_t n_slots, int* err) {
+  constexpr int D = VPL * 32;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int ng = D / group, gl = group / VPL;
+  const int per = h + 2 * hkv;
+  const int64_t items = rows * per;
+  for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
+       it += (int64_t)gridDim.x * 8) {
+    const int64_t t = it / per;
+    const int hh = (int)(it - t * per);
+    const bool is_q = hh < h, is_k = !is_q && hh < h + hkv;
+    const int64_t slot = slots[t];
+    if (!is_q && (slot < 0 || slot >= n_slots)) {
+      if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
+      continue;
+    }
+    const int head = is_q ? hh : is_k ? hh - h : hh - h - hkv;
+    const float* src = is_q ? q + (t * h + head) * D
+                            : (is_k ? k : v) + (t * hkv + head) * D;
+    float x[VPL];
+    load_row<VPL>(src + lane * VPL, x);
+    if (cos_t) {
+      const int64_t pos = positions[t];
+      if (pos < 0 || pos >= max_seq) {  // neither the key nor the value is appended
+        if (lane == 0 && err) atomicExch(err, 4);
+        continue;
+      }
+      if (is_q || is_k) rotate<VPL>(x, cos_t + pos * (D / 2), sin_t + pos * (D / 2), lane);
+    }
+    if (is_q) {
+      store_row<VPL>(q_out + (t * h + head) * D + lane * VPL, x);
+      continue;
+    }
+    float mn = x[0], mx = x[0];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      mn = fminf(mn, x[i]);
+      mx = fmaxf(mx, x[i]);
+      bad |= !(fabsf(x[i]) <= FLT_MAX);
+    }
+    mn = __fadd_rn(group_min(mn, gl), 0.f);  // -0 and 0 are one minimum, kept as 0
+    mx = __fadd_rn(group_max(mx, gl), 0.f);
+    const unsigned in_group = (gl == 32 ? 0xffffffffu : ((1u << gl) - 1u)) << (lane / gl * gl);
+    bad = (__ballot_sync(0xffffffffu, bad) & in_group) != 0;
+    float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
+    bad |= !(scale <= FLT_MAX);
+    if (bad) scale = mn = __int_as_float(0x7fffffff);
+    uint32_t code = 0;
+    if (scale > 0.f) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const float c = rintf(__fdiv_rn(__fsub_rn(x[i], mn), scale));
+        code |= (uint32_t)fminf(c, 15.0f) << (4 * i);
+      }
+    }
+    const int64_t blk = slot / bs;
+    const int in_blk = (int)(slot - blk * bs), row = in_blk % kTile;
+    uint8_t* tile = cache + ((blk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
+    uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
+    const int ch = lane * VPL;
+    if constexpr (VPL == 2) {
+      codes[is_k ? k_byte(ch, D) : v_byte(ch, D)] = (uint8_t)code;
+    } else if constexpr (VPL == 4) {
+      *reinterpret_cast<uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D))) = (uint16_t)code;
+    } else if (is_k) {
+      *reinterpret_cast<uint32_t*>(codes + k_byte(ch, D)) = code;
+    } else {
+      *reinterpret_cast<uint16_t*>(codes + v_byte(ch, D)) = (uint16_t)code;
+      *reinterpret_cast<uint16_t*>(codes + v_byte(ch + 4, D)) = (uint16_t)(code >> 16);
+    }
+    if (lane % gl == 0)
+      *reinterpret_cast<float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
+                                 ((lane / gl) * kTile + row) * 8) = make_float2(scale, mn);
+  }
+}
+
+// Rows read back: code * scale + min, rounded after the product and after the
+// sum; a slot below zero gives zeros.  One warp per row and head of K and V.
+template <int VPL>
+__global__ void __launch_bounds__(256)
+    read_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__ slots, int64_t rows,
+                int hkv, int bs, int group, int64_t n_slots, float* __restrict__ k,
+                float* __restrict__ v, int* err) {
+  constexpr int D = VPL * 32;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int ng = D / group, gl = group / VPL;
+  const int64_t items = rows * hkv * 2;
+  for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
+       it += (int64_t)gridDim.x * 8) {
+    const int64_t t = it / (2 * hkv);
+    const int hh = (int)(it - t * 2 * hkv);
+    const bool is_k = hh < hkv;
+    const int head = is_k ? hh : hh - hkv;
+    const int64_t slot = slots[t];
+    float x[VPL];
+    if (slot < 0 || slot >= n_slots) {
+      if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) x[i] = 0.f;
+    } else {
+      const int64_t blk = slot / bs;
+      const int in_blk = (int)(slot - blk * bs), row = in_blk % kTile;
+      const uint8_t* tile = cache + ((blk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
+      const uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
+      const int ch = lane * VPL;
+      uint32_t code;
+      if constexpr (VPL == 2) {
+        code = codes[is_k ? k_byte(ch, D) : v_byte(ch, D)];
+      } else if constexpr (VPL == 4) {
+        code = *reinterpret_cast<const uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D)));
+      } else if (is_k) {
+        code = *reinterpret_cast<const uint32_t*>(codes + k_byte(ch, D));
+      } else {
+        code = *reinterpret_cast<const uint16_t*>(codes + v_byte(ch, D)) |
+               (uint32_t)*reinterpret_cast<const uint16_t*>(codes + v_byte(ch + 4, D)) << 16;
+      }
+      const float2 p = *reinterpret_cast<const float2*>(
+          tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) + ((lane / gl) * kTile + row) * 8);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        x[i] = __fadd_rn(__fmul_rn((float)((code >> (4 * i)) & 15u), p.x), p.y);
+    }
+    store_row<VPL>((is_k ? k : v) + (t * hkv + head) * D + lane * VPL, x);
+  }
+}
+
+unsigned warp_grid(int64_t items) {
+  Context* c = ctx();
+  const int64_t most = (int64_t)(c ? c->num_sms : 148) * 8;
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, (items + 7) / 8));
+}
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+}  // namespace
+}  // namespace kv4
+}  // namespace nimf
+
+using namespace nimf;
+
+extern "C" {
+
+int nimf_kv4_cache_bytes(const nimf_kv4_desc* desc, int64_t* bytes) {
+  kv4::Shape s;
+  NIMF_TRY(kv4::check_desc(desc, "kv4_cache_bytes", &s));
+  if (!bytes) return set_error(NIMF_ERR_ARG, "kv4_cache_bytes: NULL result");
+  *bytes = s.n_blocks * s.hkv * (s.bs / kv4::kTile) * kv4::tile_bytes(s.d, s.d / s.group);
+  return NIMF_OK;
+}
+
+int nimf_kv4_reserve_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
+                         const int32_t* n_new, const int32_t* lens, int32_t* lens_out,
+                         int32_t* block_table, const int32_t* free_blocks, const int32_t* n_free,
+                         int32_t* n_free_out, int64_t max_rows, int32_t* cu_rows, int32_t* slots,
+                         int32_t* positions, int32_t* granted, void* stream) {
+  cudaStream_t st;
+  kv4::Shape s;
+  NIMF_TRY(kv4::check_desc(desc, "kv4_reserve", &s));
+  if (n_seqs < 0 || n_seqs > INT32_MAX || max_blocks < 1 || max_blocks > INT32_MAX / s.bs ||
+      max_rows < 0 || max_rows > INT32_MAX)
+    return set_error(NIMF_ERR_SHAPE, "kv4_reserve: n_seqs %lld max_blocks %lld max_rows %lld",
+                     (long long)n_seqs, (long long)max_blocks, (long long)max_rows);
+  if (!free_blocks || !n_free || !n_free_out || !cu_rows ||
+      (n_seqs > 0 && (!n_new || !lens || !lens_out || !block_table || !granted)) ||
+      (max_rows > 0 && (!slots || !positions)))
+    return set_error(NIMF_ERR_ARG, "kv4_reserve: NULL buffer");
+  NIMF_TRY(kv4::stream_of(stream, &st));
+  // One CTA writes about 10,000 rows in the time that a cluster's two barriers
+  // and eight launches cost.
+  const unsigned ctas = max_rows > 8192 ? 8 : 1;
+  return kv4::launch(kv4::reserve_kernel, dim3(ctas), kv4::kPoolThreads, 0, st, ctas, n_seqs,
+                     max_blocks, s.bs, s.n_blocks, n_new, lens, lens_out, block_table, free_blocks,
+                     n_free, n_free_out, max_rows, cu_rows, slots, positions, granted);
+}
+
+int nimf_kv4_release_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
+                         const int32_t* finished, int32_t* lens, const int32_t* block_table,
+                         int32_t* free_blocks, int32_t* n_free, void* stream) {
+  cudaStream_t st;
+  kv4::Shape s;
+  NIMF_TRY(kv4::check_desc(desc, "kv4_release", &s));
+  if (n_seqs < 0 || n_seqs > INT32_MAX || max_blocks < 1 || max_blocks > INT32_MAX / s.bs)
+    return set_error(NIMF_ERR_SHAPE, "kv4_release: n_seqs %lld max_blocks %lld", (long long)n_seqs,
+                     (long long)max_blocks);
+  if (n_seqs == 0) return NIMF_OK;
+  if (!finished || !lens || !block_table || !free_blocks || !n_free)
+    return set_error(NIMF_ERR_ARG, "kv4_release: NULL buffer");
+  NIMF_TRY(kv4::stream_of(stream, &st));
+  return kv4::launch(kv4::release_kernel, dim3(1), kv4::kPoolThreads, 0, st, 1, n_seqs, max_blocks,
+                     s.bs, s.n_blocks, finished, lens, block_table, free_blocks, n_free,
+                     ctx()->dev_err);
+}
+
+int nimf_kv4_append_dev(const nimf_kv4_desc* desc, void* cache, const float* k, const float* v,
+                        int64_t rows, const int32_t* slots, const float* q, float* q_out,
+                        int64_t n_heads, const int32_t* positions, const float* cos_t,
+                        const float* sin_t, int64_t max_seq, void* stream) {
+  cudaStream_t st;
+  kv4::Shape s;
+  NIMF_TRY(kv4::check_desc(desc, "kv4_append", &s));
+  if (rows < 0 || rows > INT32_MAX || n_heads < 0 || n_heads > 65535)
+    return set_error(NIMF_ERR_SHAPE, "kv4_append: rows %lld n_heads %lld", (long long)rows,
+                     (long long)n_heads);
+  if (!cos_t != !sin_t || !q != !q_out || (q && n_heads < 1) || (cos_t && (!positions || max_seq < 1)))
+    return set_error(NIMF_ERR_ARG,
+                     "kv4_append: cos_t and sin_t come together, with positions and max_seq; q with "
+                     "q_out and n_heads");
+  if (rows == 0) return NIMF_OK;
+  if (!cache || !k || !v || !slots) return set_error(NIMF_ERR_ARG, "kv4_append: NULL buffer");
+  for (const void* p : {(const void*)cache, (const void*)k, (const void*)v, (const void*)q,
+                        (const void*)q_out, (const void*)cos_t, (const void*)sin_t})
+    if (!kv4::aligned(p, 16))
+      return set_error(NIMF_ERR_ARG, "kv4_append: buffers must be 16-byte aligned");
+  NIMF_TRY(kv4::stream_of(stream, &st));
+  const int h = q ? (int)n_heads : 0;
+  auto kern = s.d == 64 ? kv4::append_kernel<2> : s.d == 128 ? kv4::append_kernel<4> : kv4::append_kernel<8>;
+  return kv4::launch(kern, dim3(kv4::warp_grid(rows * (h + 2 * s.hkv))), 256, 0, st, 1, q, q_out, h, k, v,
+                     rows, slots, positions, cos_t, sin_t, max_seq, (uint8_t*)cache, s.hkv, s.bs,
+                     s.group, s.n_blocks * s.bs, ctx()->dev_err);
+}
+
+int nimf_kv4_read_dev(const nimf_kv4_desc* desc, const void* cache, const int32_t* slots,
+                      int64_t rows, float* k, float* v, void* stream) {
+  cudaStream_t st;
+  kv4::Shape s;
+  NIMF_TRY(kv4::check_desc(desc, "kv4_read", &s));
+  if (rows < 0 || rows > INT32_MAX)
+    return set_error(NIMF_ERR_SHAPE, "kv4_read: rows %lld", (long long)rows);
+  if (rows == 0) return NIMF_OK;
+  if (!cache || !slots || !k || !v) return set_error(NIMF_ERR_ARG, "kv4_read: NULL buffer");
+  if (!kv4::aligned(cache, 16) || !kv4::aligned(k, 16) || !kv4::aligned(v, 16))
+    return set_error(NIMF_ERR_ARG, "kv4_read: buffers must be 16-byte aligned");
+  NIMF_TRY(kv4::stream_of(stream, &st));
+  auto kern = s.d == 64 ? kv4::read_kernel<2> : s.d == 128 ? kv4::read_kernel<4> : kv4::read_kernel<8>;
+  return kv4::launch(kern, dim3(kv4::warp_grid(rows * 2 * s.hkv)), 256, 0, st, 1, (const uint8_t*)cache,
+                     slots, rows, s.hkv, s.bs, s.group, s.n_blocks * s.bs, k, v, ctx()->dev_err);
+}
+
+}  // extern "C"

@@ -59,6 +59,9 @@ EXPORTS = [
     "nimf_gather_create", "nimf_matmul_w_group_gather_dev", "nimf_gather_set_timeout_ms",
     "nimf_gather_destroy", "nimf_attention_prefill_dev", "nimf_attention_decode_batch_dev",
     "nimf_q4_prefill_mode", "nimf_decode_timeline",
+    "nimf_logprobs_dev", "nimf_kv4_cache_bytes", "nimf_kv4_reserve_dev", "nimf_kv4_release_dev",
+    "nimf_kv4_append_dev", "nimf_kv4_read_dev", "nimf_kv4_attention_workspace",
+    "nimf_kv4_attention_dev",
 ]
 
 
@@ -157,6 +160,15 @@ def lib():
         "nimf_attention_decode_batch_dev": [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp,
                                             vp, ctypes.c_float, i32, vp, vp],
         "nimf_greedy_sample_dev": [vp, i64, i64, vp, i64, ctypes.c_float, vp, vp],
+        "nimf_logprobs_dev": [vp, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp],
+        "nimf_kv4_cache_bytes": [vp, ctypes.POINTER(i64)],
+        "nimf_kv4_reserve_dev": [vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp],
+        "nimf_kv4_release_dev": [vp, i64, i64, vp, vp, vp, vp, vp, vp],
+        "nimf_kv4_append_dev": [vp, vp, vp, vp, i64, vp, vp, vp, i64, vp, vp, vp, i64, vp],
+        "nimf_kv4_read_dev": [vp, vp, vp, i64, vp, vp, vp],
+        "nimf_kv4_attention_workspace": [vp, i64, ctypes.POINTER(i64)],
+        "nimf_kv4_attention_dev": [vp, vp, vp, i64, i64, i64, vp, vp, vp, i64, i64, ctypes.c_float,
+                                   vp, vp, i64, vp],
         "nimf_add_dev": [vp, vp, i64, vp, vp],
         "nimf_add_rmsnorm_dev": [vp, vp, vp, i64, i64, ctypes.c_float, vp, vp, vp],
         "nimf_swiglu_dev": [vp, vp, i64, vp, vp],
@@ -242,6 +254,74 @@ class DecodePlan:
         if self.plan:
             check(lib().nimf_decode_destroy(self.plan))
             self.plan = 0
+
+
+class KV4Desc(ctypes.Structure):
+    """nimf_kv4_desc: sizes of a 4-bit paged KV cache."""
+    _fields_ = [("n_blocks", ctypes.c_int64), ("n_kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("block_size", ctypes.c_int64),
+                ("group", ctypes.c_int64)]
+
+
+class KV4Cache:
+    """A paged KV cache with keys and values in 4 bits, shared by many requests
+    (the nimf_kv4_* entry points; no reference counterpart).  It holds the sizes
+    only: the cache (`nbytes` bytes, 16-byte aligned), the block tables and all
+    other buffers belong to the caller and are passed as device pointers (ints,
+    0 or None for NULL).  Every call is asynchronous on `stream` (an int handle;
+    None or 0: the library stream; 1: CUDA's legacy default stream)."""
+
+    def __init__(self, *, n_blocks, n_kv_heads, head_dim, block_size=16, group=64):
+        self.desc = KV4Desc(n_blocks, n_kv_heads, head_dim, block_size, group)
+        self._d = ctypes.addressof(self.desc)
+        n = ctypes.c_int64()
+        check(lib().nimf_kv4_cache_bytes(self._d, ctypes.byref(n)))
+        self.nbytes = n.value
+
+    def reserve(self, n_seqs, max_blocks, n_new, lens, lens_out, block_table, free_blocks, n_free,
+                n_free_out, max_rows, cu_rows, slots, positions, granted, stream=None):
+        """Block tables, slots and positions of n_new more tokens per request."""
+        check(lib().nimf_kv4_reserve_dev(self._d, n_seqs, max_blocks, n_new, lens, lens_out,
+                                         block_table, free_blocks, n_free, n_free_out, max_rows,
+                                         cu_rows, slots, positions, granted, stream))
+
+    def release(self, n_seqs, max_blocks, finished, lens, block_table, free_blocks, n_free,
+                stream=None):
+        """Finished requests' blocks back to the free stack."""
+        check(lib().nimf_kv4_release_dev(self._d, n_seqs, max_blocks, finished, lens, block_table,
+                                         free_blocks, n_free, stream))
+
+    def append(self, cache, k, v, rows, slots, q=None, q_out=None, n_heads=0, positions=None,
+               cos=None, sin=None, max_seq=0, stream=None):
+        """k, v [rows][n_kv_heads][head_dim] into their slots, rotated with q if
+        tables are given."""
+        check(lib().nimf_kv4_append_dev(self._d, cache, k, v, rows, slots, q, q_out, n_heads,
+                                        positions, cos, sin, max_seq, stream))
+
+    def read(self, cache, slots, rows, k_out, v_out, stream=None):
+        """The values that the slots stand for."""
+        check(lib().nimf_kv4_read_dev(self._d, cache, slots, rows, k_out, v_out, stream))
+
+    def attention_workspace(self, n_heads):
+        """Bytes of attention's workspace (no initial contents needed)."""
+        n = ctypes.c_int64()
+        check(lib().nimf_kv4_attention_workspace(self._d, n_heads, ctypes.byref(n)))
+        return n.value
+
+    def attention(self, cache, q, rows, n_heads, n_seqs, cu_rows, lens, block_table, max_blocks,
+                  scale, out, workspace, workspace_bytes, max_new=1, stream=None):
+        """Causal attention of q [rows][n_heads][head_dim] over the cache."""
+        check(lib().nimf_kv4_attention_dev(self._d, cache, q, rows, n_heads, n_seqs, cu_rows, lens,
+                                           block_table, max_blocks, max_new, scale, out, workspace,
+                                           workspace_bytes, stream))
+
+
+def logprobs_dev(logits, rows, vocab, ids, n_top, logprob, entropy, rank, top_ids, top_logprobs,
+                 stream=None):
+    """nimf_logprobs_dev on device pointers (ints): log-probabilities of given
+    tokens, entropies, ranks and the n_top most likely tokens of each row."""
+    check(lib().nimf_logprobs_dev(logits, rows, vocab, ids, n_top, logprob, entropy, rank, top_ids,
+                                  top_logprobs, stream))
 
 
 class NimqTensor(ctypes.Structure):

@@ -1,0 +1,517 @@
+"""The 4-bit paged KV cache on the GPU against plain numpy forms: block tables
+and slot maps exactly, coded rows bit for bit, attention within a bound derived
+from its roundings (kv4_reference.attention)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv4_reference as R
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+@pytest.fixture(scope="module")
+def torch_dev(nimf_gpu):
+    import torch
+    return torch
+
+
+def up(torch, a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def sync(torch, nimf):
+    torch.cuda.synchronize()
+    nimf.check(nimf.lib().nimf_sync())
+
+
+# ------------------------------------------------------------------ reserve / release
+def make_requests(rng, n, bs, width, n_blocks, max_new):
+    lens = rng.integers(0, max(1, width * bs - max_new + 2), n).astype(np.int32)
+    new = rng.integers(0, max_new + 1, n).astype(np.int32)
+    table = np.full((n, width), -7, np.int32)
+    order = rng.permutation(n_blocks).astype(np.int32)
+    at = 0
+    for b in range(n):
+        pages = -(-int(lens[b]) // bs)
+        if at + pages > n_blocks:
+            lens[b], pages = 0, 0
+        table[b, :pages] = order[at:at + pages]
+        at += pages
+    return lens, new, table, np.concatenate((order[at:], order[:at])), n_blocks - at
+
+
+def run_reserve(torch, nimf, kv4, n, width, new, lens, table, free, n_free, max_rows, in_place):
+    d = dict(new=up(torch, new), lens=up(torch, lens), table=up(torch, table), free=up(torch, free),
+             n_free=up(torch, np.array([n_free], np.int32)))
+    lens_out = d["lens"] if in_place else torch.full_like(d["lens"], -5)
+    n_free_out = d["n_free"] if in_place else torch.full_like(d["n_free"], -5)
+    cu = torch.full((n + 1,), -5, dtype=torch.int32, device="cuda")
+    slots, pos = (torch.full((max_rows,), -5, dtype=torch.int32, device="cuda") for _ in range(2))
+    granted = torch.full((n,), -5, dtype=torch.int32, device="cuda")
+    kv4.reserve(n, width, d["new"].data_ptr(), d["lens"].data_ptr(), lens_out.data_ptr(), d["table"].data_ptr(),
+                d["free"].data_ptr(), d["n_free"].data_ptr(), n_free_out.data_ptr(), max_rows, cu.data_ptr(),
+                slots.data_ptr(), pos.data_ptr(), granted.data_ptr(), stream=1)
+    sync(torch, nimf)
+    return dict(lens=lens_out, table=d["table"], n_free=n_free_out, cu_rows=cu, slots=slots, positions=pos, granted=granted)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,bs,width,spare,max_new,short", [
+    (1, 16, 3, 10, 1, 0), (5, 16, 9, 4, 40, 0), (64, 16, 20, 7, 1, 3), (1024, 32, 6, 400, 5, 0),
+    (1025, 16, 5, 200, 9, 100), (2500, 64, 3, 1000, 30, 0), (37, 128, 12, -1, 900, 50), (300, 16, 40, 2000, 300, 0)])
+def test_reserve(nimf_gpu, torch_dev, n, bs, width, spare, max_new, short, in_place):
+    """Granted and refused requests, a pool that runs dry, rows cut off by
+    max_rows, padded rows, more requests than one scan holds, both grids."""
+    rng = np.random.default_rng(n + bs)
+    blocks = n * width
+    lens, new, table, free, n_free = make_requests(rng, n, bs, width, blocks, max_new)
+    n_free = min(n_free, max(0, spare))
+    max_rows = max(1, int(new.sum()) + (-short if short else 9))
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=1, head_dim=64, block_size=bs, group=32)
+    got = run_reserve(torch_dev, nimf_gpu, kv4, n, width, new, lens, table, free, n_free, max_rows, in_place)
+    want = R.reserve(bs, blocks, width, new, lens, table, free, n_free, max_rows)
+    for k in want:
+        assert np.array_equal(got[k].cpu().numpy(), np.reshape(want[k], got[k].shape)), k
+
+
+def test_reserve_odd_inputs(nimf_gpu, torch_dev):
+    """No requests, negative lengths, a free count above the pool."""
+    kv4 = nimf_gpu.KV4Cache(n_blocks=8, n_kv_heads=1, head_dim=64, block_size=16, group=32)
+    z = np.zeros(0, np.int32)
+    got = run_reserve(torch_dev, nimf_gpu, kv4, 0, 2, z, z, np.zeros((0, 2), np.int32), np.arange(8, dtype=np.int32), 5, 3, False)
+    assert got["cu_rows"].tolist() == [0] and got["n_free"].item() == 5 and got["slots"].tolist() == [-1] * 3
+    new, lens = np.array([-3, 20, 1], np.int32), np.array([5, -9, 31], np.int32)
+    table = np.array([[3, -1], [-1, -1], [1, 2]], np.int32)
+    free = np.array([7, 6, 5, 4, 0, 9, 9, 9], np.int32)
+    got = run_reserve(torch_dev, nimf_gpu, kv4, 3, 2, new, lens, table, free, 5, 30, True)
+    want = R.reserve(16, 8, 2, new, lens, table, free, 5, 30)
+    for k in want:
+        assert np.array_equal(got[k].cpu().numpy(), np.reshape(want[k], got[k].shape)), k
+
+
+def test_release_returns_blocks_in_order(nimf_gpu, torch_dev):
+    torch = torch_dev
+    rng = np.random.default_rng(8)
+    for n, bs, width in ((3, 16, 4), (1500, 16, 7), (2, 16, 3000)):
+        blocks = n * width
+        lens, _, table, free, n_free = make_requests(rng, n, bs, width, blocks, 1)
+        done = rng.integers(0, 2, n).astype(np.int32)
+        want, top = free.copy(), n_free
+        for b in range(n):
+            if done[b]:
+                pages = -(-int(lens[b]) // bs)
+                want[top:top + pages] = table[b, :pages]
+                top += pages
+        d = [up(torch, v) for v in (done, lens, table, free, np.array([n_free], np.int32))]
+        kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=1, head_dim=64, block_size=bs, group=32)
+        for _ in range(2):      # the second time there is nothing left to return
+            kv4.release(n, width, *[t.data_ptr() for t in d], stream=1)
+            sync(torch, nimf_gpu)
+            assert d[4].item() == top
+            assert np.array_equal(d[3].cpu().numpy()[:top], want[:top])
+            assert np.array_equal(d[1].cpu().numpy(), np.where(done, 0, lens))
+
+
+def test_release_of_too_many_blocks_is_reported(nimf_gpu, torch_dev):
+    torch = torch_dev
+    kv4 = nimf_gpu.KV4Cache(n_blocks=4, n_kv_heads=1, head_dim=64, block_size=16, group=32)
+    d = [up(torch, np.array(v, np.int32)) for v in ([1], [48], [[0, 1, 2]], [3, 9, 9, 9], [2])]
+    guard = torch.full((4,), 77, dtype=torch.int32, device="cuda")
+    kv4.release(1, 3, *[t.data_ptr() for t in d], stream=1)
+    torch.cuda.synchronize()
+    assert nimf_gpu.lib().nimf_sync() == -5
+    assert d[3].tolist() == [3, 9, 0, 1] and d[4].item() == 4 and guard.tolist() == [77] * 4
+
+
+# ------------------------------------------------------------------ append / read
+def tables(dim, max_seq):
+    inv = 1.0 / 10000.0 ** (np.arange(dim // 2) / (dim // 2))
+    ang = np.arange(max_seq)[:, None] * inv
+    return np.cos(ang).astype(F), np.sin(ang).astype(F)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)])
+@pytest.mark.parametrize("rows,hkv,r,bs", [(1, 1, 1, 16), (37, 3, 2, 48), (70, 2, 7, 16)])
+def test_append_and_read_bit_exact(nimf_gpu, torch_dev, dim, group, rows, hkv, r, bs):
+    """Codes, scales and minima byte for byte, nothing else in the cache
+    touched; constant groups, huge and tiny ranges, NaN and infinities; rows
+    without a slot; queries rotated."""
+    torch = torch_dev
+    rng = np.random.default_rng(dim + group + rows)
+    blocks = -(-rows // bs) + 2
+    h = hkv * r
+    k, v = (rng.standard_normal((rows, hkv, dim)).astype(F) for _ in range(2))
+    q = rng.standard_normal((rows, h, dim)).astype(F)
+    v[0, 0, :group] = 3.25
+    if rows > 5:
+        v[1] *= F(1e30)
+        v[2] *= F(1e-41)
+        v[3, 0, 5] = np.nan
+        v[4, 0, 7] = -np.inf
+        v[5, 0, :2] = [3e38, -3e38]
+        k[4, 0, 1] = np.inf
+        v[6, 0] = np.where(rng.random(dim) < 0.5, F(-0.0), F(0.0))
+    slots = rng.permutation(blocks * bs)[:rows].astype(np.int32)
+    if rows > 9:
+        slots[[8, 9]] = -1
+    pos = rng.integers(0, 300, rows).astype(np.int32)
+    ct, st = tables(dim, 300)
+    pool = R.Pool(blocks, hkv, dim, bs, group, rng)
+    before = pool.buf.copy()
+    with np.errstate(all="ignore"):
+        qr, kr = R.rope(q, pos, ct, st), R.rope(k, pos, ct, st)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=hkv, head_dim=dim, block_size=bs, group=group)
+    assert kv4.nbytes == before.size
+    dk, dv, dq, ds, dp, dc, dn = (up(torch, a) for a in (k, v, q, slots, pos, ct, st))
+    for with_rope in (True, False):
+        pool.buf[:] = before
+        for t in range(rows):
+            if slots[t] >= 0:
+                pool.write(slots[t], True, (kr if with_rope else k)[t])
+                pool.write(slots[t], False, v[t])
+        cache = up(torch, before)
+        qo = dq.clone()
+        rope = dict(positions=dp.data_ptr(), cos=dc.data_ptr(), sin=dn.data_ptr(), max_seq=300) if with_rope else {}
+        kv4.append(cache.data_ptr(), dk.data_ptr(), dv.data_ptr(), rows, ds.data_ptr(), q=qo.data_ptr(), q_out=qo.data_ptr(),
+                   n_heads=h, stream=1, **rope)
+        ko, vo = (torch.full((rows, hkv, dim), 7.0, device="cuda") for _ in range(2))
+        kv4.read(cache.data_ptr(), ds.data_ptr(), rows, ko.data_ptr(), vo.data_ptr(), stream=1)
+        sync(torch, nimf_gpu)
+        got = cache.cpu().numpy()
+        # a NaN's bits are not fixed: compare such parameters as floats
+        nan_ok = np.ascontiguousarray(pool.buf).view(F)
+        same = (got == pool.buf) | (np.isnan(nan_ok) & np.isnan(np.ascontiguousarray(got).view(F))).repeat(4, -1)
+        assert same.all()
+        assert np.array_equal(qo.cpu().numpy(), qr if with_rope else q)
+        assert np.array_equal(dk.cpu().numpy(), k, equal_nan=True)
+        for out, x in ((ko, kr if with_rope else k), (vo, v)):
+            with np.errstate(all="ignore"):
+                want = R.decode(*R.encode(x, group))
+            want[slots < 0] = 0
+            assert np.array_equal(out.cpu().numpy(), want, equal_nan=True)
+
+
+def test_append_keeps_out_of_range_rows_out(nimf_gpu, torch_dev):
+    """A slot past the cache or a position past the tables appends nothing, is
+    reported once, and leaves the other rows' work done."""
+    torch = torch_dev
+    rng = np.random.default_rng(3)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=2, n_kv_heads=2, head_dim=64, block_size=16, group=32)
+    k, v = (up(torch, rng.standard_normal((4, 2, 64)).astype(F)) for _ in range(2))
+    ct, st = (up(torch, t) for t in tables(64, 10))
+    cache = torch.zeros(kv4.nbytes, dtype=torch.uint8, device="cuda")
+    for slots, pos in (([0, 32, 5, 2 ** 31 - 1], [0, 1, 2, 3]), ([0, -1, 5, 7], [0, 3, 2, 10]), ([0, -1, 5, 7], [0, 3, 2, -1])):
+        cache.zero_()
+        ds, dp = up(torch, np.array(slots, np.int32)), up(torch, np.array(pos, np.int32))
+        kv4.append(cache.data_ptr(), k.data_ptr(), v.data_ptr(), 4, ds.data_ptr(), positions=dp.data_ptr(),
+                   cos=ct.data_ptr(), sin=st.data_ptr(), max_seq=10, stream=1)
+        torch.cuda.synchronize()
+        assert nimf_gpu.lib().nimf_sync() == -5
+        nimf_gpu.check(nimf_gpu.lib().nimf_sync())
+        ko, vo = (torch.empty(4, 2, 64, device="cuda") for _ in range(2))
+        kv4.read(cache.data_ptr(), up(torch, np.array([0, 5, 7, 31], np.int32)).data_ptr(), 4, ko.data_ptr(), vo.data_ptr(), stream=1)
+        sync(torch, nimf_gpu)
+        assert (vo[:2].abs().sum((1, 2)) > 0).all() and not vo[2:].any() and not ko[2:].any()
+
+
+# ------------------------------------------------------------------ attention
+def fill(pool, rng, wide=True):
+    """Random codes and parameters for every row, as projections give them."""
+    for key in (True, False):
+        codes, params = pool.parts(key)
+        half, ng = 8 * pool.dim, pool.dim // pool.group
+        pool.buf[..., codes:codes + half] = rng.integers(0, 256, pool.buf[..., :half].shape)
+        shape = (*pool.buf.shape[:-1], 16 * ng)
+        p = np.empty((*shape, 2), F)
+        p[..., 0] = rng.uniform(0.1, 0.4, shape) * (np.exp2(rng.integers(-6, 5, shape)) if wide and not key else 1.0)
+        p[..., 1] = -7.5 * p[..., 0] + rng.standard_normal(shape) * 0.3
+        pool.buf[..., params:params + 128 * ng] = np.ascontiguousarray(p).view(np.uint8).reshape(*pool.buf.shape[:-1], -1)
+
+
+def poison(pool, table, length):
+    """NaN parameters in every row of the sequence's last block behind its end."""
+    for t in range(length, -(-length // pool.bs) * pool.bs):
+        for key in (True, False):
+            _, params = pool.parts(key)
+            for n in range(pool.dim // pool.group):
+                at = params + (n * 16 + t % 16) * 8
+                pool.buf[table[t // pool.bs], :, t % pool.bs // 16, at:at + 8] = np.array([np.nan, np.nan], F).view(np.uint8)
+
+
+def attend(torch, nimf, pool, tab, lens, new, q, scale, rows=None, cu=True, max_new=None, out=None, work=None, stream=1):
+    h = q.shape[1]
+    kv4 = nimf.KV4Cache(n_blocks=pool.blocks, n_kv_heads=pool.hkv, head_dim=pool.dim, block_size=pool.bs, group=pool.group)
+    d = dict(cache=up(torch, pool.buf), q=up(torch, q), lens=up(torch, np.array(lens, np.int32)), tab=up(torch, np.array(tab, np.int32)),
+             cu=up(torch, np.concatenate(([0], np.cumsum(new))).astype(np.int32)))
+    out = torch.full(q.shape, 5.0, device="cuda") if out is None else out
+    n = kv4.attention_workspace(h)
+    work = torch.full((n,), 255, dtype=torch.uint8, device="cuda") if work is None else work
+    kv4.attention(d["cache"].data_ptr(), d["q"].data_ptr(), q.shape[0] if rows is None else rows, h, len(lens),
+                  d["cu"].data_ptr() if cu else None, d["lens"].data_ptr(), d["tab"].data_ptr(), d["tab"].shape[1], scale,
+                  out.data_ptr(), work.data_ptr(), n, max_new=max(new) if max_new is None else max_new, stream=stream)
+    sync(torch, nimf)
+    return out.cpu().numpy()
+
+
+def check(got, pool, tab, lens, new, q, scale):
+    row = 0
+    for b, (n, m) in enumerate(zip(lens, new)):
+        want, tol = R.attention(pool, tab[b], n, q[row:row + m], scale)
+        err = np.abs(got[row:row + m] - want)
+        assert np.isfinite(got[row:row + m]).all()
+        assert (err <= tol).all(), (b, n, m, float((err / tol).max()))
+        row += m
+    return row
+
+
+def layout(rng, lens, bs, extra=2):
+    pages = [-(-n // bs) for n in lens]
+    blocks = sum(pages) + extra
+    order = rng.permutation(blocks).astype(np.int32)
+    tab = np.full((len(lens), max(1, max(pages)) + 1), -1, np.int32)
+    at = 0
+    for b, p in enumerate(pages):
+        tab[b, :p] = order[at:at + p]
+        at += p
+    return blocks, tab
+
+
+SHAPES = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)]
+
+
+@pytest.mark.parametrize("dim,group", SHAPES)
+@pytest.mark.parametrize("hkv,r,bs", [(2, 1, 16), (1, 4, 32), (3, 7, 48), (1, 12, 64)])
+def test_attention_single_tokens(nimf_gpu, torch_dev, dim, group, hkv, r, bs):
+    """One row per sequence at lengths around every tile, unit and block edge,
+    an empty sequence, NaN behind the ends, more heads than a row tile."""
+    rng = np.random.default_rng(dim * 3 + group + r)
+    lens = [1, 0, 15, 16, 17, 31, 32, 33, 63, 64, 65, 200, 513]
+    blocks, tab = layout(rng, lens, bs)
+    pool = R.Pool(blocks, hkv, dim, bs, group, rng)
+    fill(pool, rng)
+    for b, n in enumerate(lens):
+        poison(pool, tab[b], n)
+    new = [1] * len(lens)
+    q = (rng.standard_normal((len(lens), hkv * r, dim)) * 2).astype(F)
+    scale = 1 / np.sqrt(dim)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale)
+    check(got, pool, tab, lens, new, q, scale)
+    again = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale, cu=False)
+    assert np.array_equal(got, again)
+
+
+@pytest.mark.parametrize("dim,group", SHAPES)
+@pytest.mark.parametrize("hkv,r,bs", [(2, 1, 16), (2, 3, 32)])
+def test_attention_prompts_and_tokens_mixed(nimf_gpu, torch_dev, dim, group, hkv, r, bs):
+    """Prompts, later chunks, single tokens, a sequence without new rows and one
+    with more rows than tokens in one call; rows behind the last are left."""
+    rng = np.random.default_rng(dim + group * 5 + r)
+    lens = [70, 1, 300, 40, 5, 129, 257]
+    new = [70, 1, 37, 0, 8, 1, 200]
+    blocks, tab = layout(rng, lens, bs)
+    pool = R.Pool(blocks, hkv, dim, bs, group, rng)
+    fill(pool, rng)
+    for b, n in enumerate(lens):
+        poison(pool, tab[b], n)
+    q = rng.standard_normal((sum(new) + 6, hkv * r, dim)).astype(F)
+    scale = 1 / np.sqrt(dim)
+    for hint in (1, 200):
+        got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale, max_new=hint)
+        end = check(got, pool, tab, lens, new, q, scale)
+        assert (got[end:] == 5.0).all()
+
+
+@pytest.mark.parametrize("dim,group,hkv,r", [(128, 128, 1, 1), (128, 64, 2, 4), (64, 64, 1, 8), (256, 128, 1, 2)])
+def test_attention_long_sequence_is_split_and_repeatable(nimf_gpu, torch_dev, dim, group, hkv, r):
+    """A context long enough for every CTA to hold a piece of it, beside short
+    ones; the same bits every time."""
+    rng = np.random.default_rng(dim + r)
+    lens, new = [3, 20011, 40], [1, 1, 2]
+    blocks, tab = layout(rng, lens, 32)
+    pool = R.Pool(blocks, hkv, dim, 32, group, rng)
+    fill(pool, rng)
+    q = rng.standard_normal((4, hkv * r, dim)).astype(F)
+    scale = 1 / np.sqrt(dim)
+    first = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale)
+    check(first, pool, tab, lens, new, q, scale)
+    for _ in range(3):
+        assert np.array_equal(first, attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale))
+
+
+def test_attention_many_sequences(nimf_gpu, torch_dev):
+    """More sequences than one scan of the units holds."""
+    rng = np.random.default_rng(12)
+    lens = [int(n) for n in rng.integers(0, 60, 700)]
+    lens[650] = 900
+    new = [int(n) for n in rng.integers(0, 3, 700)]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, 2, 64, 16, 32, rng)
+    fill(pool, rng)
+    q = rng.standard_normal((sum(new), 4, 64)).astype(F)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.125)
+    check(got, pool, tab, lens, new, q, 0.125)
+
+
+def test_attention_scales_of_every_size(nimf_gpu, torch_dev):
+    """Large and tiny queries and value scales keep their relative accuracy, a
+    softmax scale of zero averages, a negative one is taken as it is."""
+    rng = np.random.default_rng(5)
+    lens, new = [77, 150], [1, 3]
+    blocks, tab = layout(rng, lens, 16)
+    for q_size, v_size, scale in ((1e-20, 1e-30, 1.0), (1e3, 1e30, 1e-3), (1.0, 1.0, 0.0), (1.0, 1.0, -0.2), (0.0, 1.0, 1.0)):
+        pool = R.Pool(blocks, 1, 128, 16, 64, rng)
+        fill(pool, rng)
+        codes, params = pool.parts(False)
+        at = pool.buf[..., params:params + 256]
+        p = np.ascontiguousarray(at).view(F) * F(v_size)
+        pool.buf[..., params:params + 256] = np.ascontiguousarray(p).view(np.uint8)
+        q = (rng.standard_normal((4, 2, 128)) * q_size).astype(F)
+        got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale)
+        check(got, pool, tab, lens, new, q, scale)
+
+
+def test_attention_nan_reaches_only_who_sees_it(nimf_gpu, torch_dev):
+    """A group coded from a NaN gives NaN to the rows that see its token (its
+    key to the whole row, its value to that group's channels), to none before."""
+    rng = np.random.default_rng(6)
+    lens, new = [50, 40], [50, 1]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, 1, 64, 16, 32, rng)
+    fill(pool, rng)
+    x = rng.standard_normal((1, 64)).astype(F)
+    x[0, 40] = np.nan
+    pool.write(tab[0][1] * 16 + 4, False, x)      # token 20's values, channels 32..63
+    q = rng.standard_normal((51, 2, 64)).astype(F)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.125)
+    assert np.isnan(got[20:50, :, 32:]).all() and np.isfinite(got[:50, :, :32]).all()
+    assert np.isfinite(got[:20]).all() and np.isfinite(got[50]).all()
+    want, tol = R.attention(pool, tab[0], 20, q[:20], 0.125)
+    assert (np.abs(got[:20] - want) <= tol).all()
+    pool.write(tab[0][1] * 16 + 4, True, x)       # and its key
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.125)
+    assert np.isnan(got[20:50]).all() and np.isfinite(got[:20]).all() and np.isfinite(got[50]).all()
+
+
+def test_attention_leaves_out_blocks_that_are_not_there(nimf_gpu, torch_dev):
+    """A table entry outside the cache: its tokens take no part, nimf_sync
+    reports it, and lens past the table are cut to it."""
+    torch = torch_dev
+    rng = np.random.default_rng(7)
+    pool = R.Pool(6, 1, 64, 16, 64, rng)
+    fill(pool, rng)
+    q = rng.standard_normal((2, 1, 64)).astype(F)
+    tab = np.array([[0, -3, 2], [4, 5, 6]], np.int32)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=6, n_kv_heads=1, head_dim=64, block_size=16, group=64)
+    d = [up(torch, a) for a in (pool.buf, q, np.array([48, 1000], np.int32), tab)]
+    out = torch.empty(2, 1, 64, device="cuda")
+    n = kv4.attention_workspace(1)
+    work = torch.empty(n, dtype=torch.uint8, device="cuda")
+    kv4.attention(d[0].data_ptr(), d[1].data_ptr(), 2, 1, 2, None, d[2].data_ptr(), d[3].data_ptr(), 3, 0.125, out.data_ptr(),
+                  work.data_ptr(), n, stream=1)
+    torch.cuda.synchronize()
+    assert nimf_gpu.lib().nimf_sync() == -5
+    nimf_gpu.check(nimf_gpu.lib().nimf_sync())
+    for b, blocks in ((0, [0, 2]), (1, [4, 5])):
+        want, tol = R.attention(pool, blocks, 32, q[b:b + 1], 0.125)
+        assert (np.abs(out[b].cpu().numpy() - want[0]) <= tol[0]).all()
+
+
+def test_attention_in_graphs_on_two_streams(nimf_gpu, torch_dev):
+    """Captured calls replayed at the same time on two streams, a workspace
+    each, with new contents in the captured buffers."""
+    torch = torch_dev
+    rng = np.random.default_rng(9)
+    lens, new = [900, 33, 2000], [1, 1, 1]
+    blocks, tab = layout(rng, lens, 16)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=2, head_dim=128, block_size=16, group=128)
+    jobs = []
+    for i in range(2):
+        pool = R.Pool(blocks, 2, 128, 16, 128, rng)
+        fill(pool, rng)
+        d = dict(cache=up(torch, pool.buf), q=torch.zeros(3, 4, 128, device="cuda"), lens=up(torch, np.array(lens, np.int32)),
+                 tab=up(torch, tab), out=torch.empty(3, 4, 128, device="cuda"),
+                 work=torch.empty(kv4.attention_workspace(4), dtype=torch.uint8, device="cuda"))
+        torch.cuda.synchronize()
+        st = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            kv4.attention(d["cache"].data_ptr(), d["q"].data_ptr(), 3, 4, 3, None, d["lens"].data_ptr(), d["tab"].data_ptr(), tab.shape[1],
+                          0.1, d["out"].data_ptr(), d["work"].data_ptr(), d["work"].numel(), stream=st.cuda_stream)
+        jobs.append((pool, d, st, graph))
+    for _ in range(3):
+        qs = [rng.standard_normal((3, 4, 128)).astype(F) for _ in jobs]
+        for (_, d, _, _), q in zip(jobs, qs):
+            d["q"].copy_(up(torch, q))
+        torch.cuda.synchronize()
+        for _, _, st, graph in jobs:
+            with torch.cuda.stream(st):
+                for _ in range(4):
+                    graph.replay()
+        sync(torch, nimf_gpu)
+        for (pool, d, _, _), q in zip(jobs, qs):
+            check(d["out"].cpu().numpy(), pool, tab, lens, new, q, 0.1)
+
+
+# ------------------------------------------------------------------ together
+def test_serving_steps(nimf_gpu, torch_dev):
+    """Prompts admitted, tokens decoded, a request finished and its blocks used
+    again: reserve, append, attention and log-probabilities step by step, the
+    cache's contents and every output against the plain forms."""
+    torch = torch_dev
+    rng = np.random.default_rng(21)
+    bs, hkv, r, dim, group, width, blocks, n, vocab = 16, 2, 2, 64, 32, 8, 14, 3, 501
+    h, max_rows, max_seq = hkv * r, 64, 128
+    ct, st = tables(dim, max_seq)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=hkv, head_dim=dim, block_size=bs, group=group)
+    pool = R.Pool(blocks, hkv, dim, bs, group)
+    proj = rng.standard_normal((h * dim, vocab)).astype(F)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = torch.zeros(kv4.nbytes, dtype=torch.uint8, device="cuda")
+    free = rng.permutation(blocks).astype(np.int32)
+    d_free, d_nf, d_lens, d_tab = up(torch, free), i32(1) + blocks, i32(n), i32(n, width) - 1
+    cu, slots, pos, granted = i32(n + 1), i32(max_rows), i32(max_rows), i32(n)
+    d_ct, d_st = up(torch, ct), up(torch, st)
+    work = torch.empty(kv4.attention_workspace(h), dtype=torch.uint8, device="cuda")
+    lens, tab, n_free = np.zeros(n, np.int32), np.full((n, width), -1, np.int32), blocks
+    for step, new in enumerate(([33, 20, 0], [1, 1, 30], [1, 0, 1], [4, 1, 1], "release 0", [20, 1, 16], [1, 1, 1])):
+        if isinstance(new, str):
+            done = np.array([1, 0, 0], np.int32)
+            pages = -(-int(lens[0]) // bs)
+            free[n_free:n_free + pages] = tab[0, :pages]
+            n_free, lens[0] = n_free + pages, 0
+            kv4.release(n, width, up(torch, done).data_ptr(), d_lens.data_ptr(), d_tab.data_ptr(), d_free.data_ptr(), d_nf.data_ptr(), stream=1)
+            continue
+        want = R.reserve(bs, blocks, width, new, lens, tab, free, n_free, max_rows)
+        assert want["granted"].all()
+        total = int(want["cu_rows"][-1])
+        q, k, v = (rng.standard_normal((max_rows, x, dim)).astype(F) for x in (h, hkv, hkv))
+        ids = rng.integers(0, vocab, max_rows).astype(np.int32)
+        dn, dq, dk, dv, di = (up(torch, a) for a in (np.array(new, np.int32), q, k, v, ids))
+        out = torch.zeros(max_rows, h, dim, device="cuda")
+        kv4.reserve(n, width, dn.data_ptr(), d_lens.data_ptr(), d_lens.data_ptr(), d_tab.data_ptr(), d_free.data_ptr(), d_nf.data_ptr(),
+                    d_nf.data_ptr(), max_rows, cu.data_ptr(), slots.data_ptr(), pos.data_ptr(), granted.data_ptr(), stream=1)
+        kv4.append(cache.data_ptr(), dk.data_ptr(), dv.data_ptr(), max_rows, slots.data_ptr(), q=dq.data_ptr(), q_out=dq.data_ptr(), n_heads=h,
+                   positions=pos.data_ptr(), cos=d_ct.data_ptr(), sin=d_st.data_ptr(), max_seq=max_seq, stream=1)
+        kv4.attention(cache.data_ptr(), dq.data_ptr(), max_rows, h, n, cu.data_ptr(), d_lens.data_ptr(), d_tab.data_ptr(), width, 0.125,
+                      out.data_ptr(), work.data_ptr(), work.numel(), max_new=max(new), stream=1)
+        logits = (out.reshape(max_rows, -1) @ up(torch, proj)).contiguous()
+        lp, ent = torch.empty(max_rows, device="cuda"), torch.empty(max_rows, device="cuda")
+        rank, top_i, top_p = i32(max_rows), i32(max_rows, 4), torch.empty(max_rows, 4, device="cuda")
+        nimf_gpu.logprobs_dev(logits.data_ptr(), max_rows, vocab, di.data_ptr(), 4, lp.data_ptr(), ent.data_ptr(), rank.data_ptr(),
+                              top_i.data_ptr(), top_p.data_ptr(), stream=1)
+        sync(torch, nimf_gpu)
+        lens, tab, n_free = want["lens"], want["table"], want["n_free"]
+        for name, got in (("lens", d_lens), ("table", d_tab), ("n_free", d_nf), ("cu_rows", cu), ("slots", slots), ("positions", pos)):
+            assert np.array_equal(got.cpu().numpy(), np.reshape(want[name], got.shape)), (step, name)
+        qr, kr = R.rope(q, want["positions"], ct, st), R.rope(k, want["positions"], ct, st)
+        for t in range(total):
+            pool.write(want["slots"][t], True, kr[t])
+            pool.write(want["slots"][t], False, v[t])
+        assert np.array_equal(cache.cpu().numpy(), pool.buf.ravel())
+        assert check(out.cpu().numpy(), pool, tab, lens, new, qr, 0.125) == total
+        ref = R.logprobs(logits.cpu().numpy(), ids, 4)
+        assert np.array_equal(rank.cpu().numpy(), ref["rank"]) and np.array_equal(top_i.cpu().numpy(), ref["top_ids"])
+        assert np.allclose(lp.cpu().numpy(), ref["logprob"], rtol=2e-6, atol=2e-6)
