@@ -4,16 +4,22 @@
 //   k^_j = c_j s_j + m_j per group of channels (v^ likewise),
 // over the cached tokens j that row t may see (causal).
 //
-// The products run on the tensor cores with the codes as they are: a nibble
-// masked in place in a 16-bit lane IS the fp16 number c * 2^-24 (a subnormal,
-// or 16 c * 2^-24 for the nibble above it), so eight codes cost five logic
-// operations and nothing is converted.  Scale and minimum enter outside:
-//   q . k^_j = sum_groups s_j (q . c_j) + m_j sum(q)
-//   sum_j p_j v^_j = sum_j (p_j s_j) c_j + sum_j p_j m_j
-// q and p s are given as two fp16 terms each (22 bits), high terms in rows
-// 0..7 of the MMA's A operand and low terms in rows 8..15, so one 16-row tile
-// carries 8 query rows at close to float32 accuracy; both halves of an
-// accumulator are added in registers.
+// The products run on the tensor cores with codes centred at 8: a nibble masked
+// into the fp16 number 1024 + c (or 1024 + 16 c for the nibble above it) less
+// 1032 (1152) is c - 8 (16 times that) exactly, so eight codes cost nine
+// operations.  Scale and minimum enter outside:
+//   q . k^_j = sum_groups s_j (q . (c_j - 8)) + (m_j + 8 s_j) sum(q)
+//   sum_j p_j v^_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)
+// Centred, both sums of the second line are as small as the result; the codes
+// taken from 0 make them grow with the context while the result shrinks, and
+// the difference lost 2^-11 of it at 131,000 tokens.
+// q and p s are given as two fp16 terms each, high terms in rows 0..7 of the
+// MMA's A operand and low terms in rows 8..15, so one 16-row tile carries 8
+// query rows at float32's accuracy; both halves of an accumulator are added in
+// registers.  The tensor core cuts what an addition shifts out.  So q's high
+// terms are integers of 11 bits: their products with the codes and all sums of
+// them are exact.  p s, whose values differ by many powers of two, has 22 bits
+// of each value, and sums of 32 tokens at most run in the tensor core.
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -106,6 +112,20 @@ __device__ __forceinline__ void split_f16x2(float x0, float x1, uint32_t& hi, ui
   const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// Two floats up to 2^11 as integers and fp16 rests, both times f.
+__device__ __forceinline__ void split_int(float x0, float x1, float f, uint32_t& hi, uint32_t& lo) {
+  const float r0 = rintf(x0), r1 = rintf(x1);
+  const __half2 h = __floats2half2_rn(r0 * f, r1 * f), l = __floats2half2_rn((x0 - r0) * f, (x1 - r1) * f);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// The codes of the even (odd: 16 times them) nibbles of the low and the third
+// byte's half words, less 8, as two fp16 numbers.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, bool odd) {
+  uint32_t v = lop3_and_or(w, odd ? 0x00F000F0u : 0x000F000Fu, 0x64006400u), r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(odd ? 0xE480E480u : 0xE408E408u));
+  return r;
 }
 // 2^(e - 127) for an exponent field e clamped to the normal range.
 __device__ __forceinline__ float pow2_field(int e) {
@@ -320,25 +340,24 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // The largest magnitude goes to [2^14, 2^15): fp16 keeps 22 bits of it
-      // in two terms, and the smallest subnormal lies 2^38 below.
+      // the largest magnitude goes to [2^10, 2^11): integers and their rests
       const int e = max(14, min(244, exp_field(amax)));
-      const float up = pow2_field(268 - e);
-      row_f = pow2_field(e + 10);           // 2^24 / up: the codes are c * 2^-24
+      const float up = pow2_field(264 - e);
+      row_f = pow2_field(e - 10);           // 1 / up
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {       // even nibbles, then odd ones (16 c)
-          const float f = p ? up * 0.0625f : up;
-          split_f16x2(x[j][p] * f, x[j][p + 4] * f, qf[j][p][0], qf[j][p][1]);
-          split_f16x2(x[j][p + 2] * f, x[j][p + 6] * f, qf[j][p][2], qf[j][p][3]);
+          const float f = p ? 0.0625f : 1.f;
+          split_int(x[j][p] * up, x[j][p + 4] * up, f, qf[j][p][0], qf[j][p][1]);
+          split_int(x[j][p + 2] * up, x[j][p + 6] * up, f, qf[j][p][2], qf[j][p][3]);
         }
     }
 
     // ---- online softmax over the units
     float m = -INFINITY, l = 0.f, mins[NG];
     float o[NS][2][4][2];                   // [span][half][nibble][column]
-    int e_run = 14;                         // exponent field of the largest value scale so far
+    int e_run = 20;                         // exponent field of the largest value scale so far
 #pragma unroll
     for (int n = 0; n < NG; ++n) mins[n] = 0.f;
 #pragma unroll
@@ -377,9 +396,9 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
           for (int j = 0; j < NC; ++j) {
             const uint32_t w8 = w[j] >> 8;
             mma_f16_16816(acc[j * 32 / G], qf[j][0][0], qf[j][0][1], qf[j][0][2], qf[j][0][3],
-                          w[j] & 0x000F000Fu, w8 & 0x000F000Fu);
+                          codes_f16(w[j], false), codes_f16(w8, false));
             mma_f16_16816(acc[j * 32 / G], qf[j][1][0], qf[j][1][1], qf[j][1][2], qf[j][1][3],
-                          w[j] & 0x00F000F0u, w8 & 0x00F000F0u);
+                          codes_f16(w[j], true), codes_f16(w8, true));
           }
           float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -387,8 +406,9 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
             const float4 p = *reinterpret_cast<const float4*>(
                 buf + t * TB + k_params_at(D) + (n * kTile + hf * 8 + 2 * c) * 8);
             const float a0 = (acc[n][0] + acc[n][2]) * row_f, a1 = (acc[n][1] + acc[n][3]) * row_f;
-            s0 = fmaf(a0, c & 1 ? p.z : p.x, fmaf(qsum[n], c & 1 ? p.w : p.y, s0));
-            s1 = fmaf(a1, c & 1 ? p.x : p.z, fmaf(qsum[n], c & 1 ? p.y : p.w, s1));
+            const float k0 = c & 1 ? p.z : p.x, k1 = c & 1 ? p.x : p.z;
+            s0 = fmaf(a0, k0, fmaf(qsum[n], fmaf(8.f, k0, c & 1 ? p.w : p.y), s0));
+            s1 = fmaf(a1, k1, fmaf(qsum[n], fmaf(8.f, k1, c & 1 ? p.y : p.w), s1));
           }
           const int t0 = u * kUnit + t * kTile + hf * 8 + 2 * c;
           const bool in = (has >> t) & 1u;
@@ -473,8 +493,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
                 const float p0 = sc[t][hf][0], p1 = sc[t][hf][1];
                 const float w0 = p0 < 0.f ? 0.f : p0 * (p.x * up);
                 const float w1 = p1 < 0.f ? 0.f : p1 * (p.z * up);
-                if (!(p0 < 0.f)) mins[n] = fmaf(p0, p.y, mins[n]);
-                if (!(p1 < 0.f)) mins[n] = fmaf(p1, p.w, mins[n]);
+                if (!(p0 < 0.f)) mins[n] = fmaf(p0, fmaf(8.f, p.x, p.y), mins[n]);
+                if (!(p1 < 0.f)) mins[n] = fmaf(p1, fmaf(8.f, p.z, p.w), mins[n]);
                 split_f16x2(w0, w1, pa[t][2 * hf], pa[t][2 * hf + 1]);
               }
           }
@@ -486,10 +506,10 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
             const uint32_t x0 = prmt(vw[t][0][sp], vw[t][1][sp], hv ? 0x7632 : 0x5410);
             const uint32_t x1 = prmt(vw[t][2][sp], vw[t][3][sp], hv ? 0x7632 : 0x5410);
             const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-            mma_f16_16816(acc[0], pa[t][0], pa[t][1], pa[t][2], pa[t][3], x0 & 0x000F000Fu, x1 & 0x000F000Fu);
-            mma_f16_16816(acc[1], pa[t][0], pa[t][1], pa[t][2], pa[t][3], x0 & 0x00F000F0u, x1 & 0x00F000F0u);
-            mma_f16_16816(acc[2], pa[t][0], pa[t][1], pa[t][2], pa[t][3], y0 & 0x000F000Fu, y1 & 0x000F000Fu);
-            mma_f16_16816(acc[3], pa[t][0], pa[t][1], pa[t][2], pa[t][3], y0 & 0x00F000F0u, y1 & 0x00F000F0u);
+            mma_f16_16816(acc[0], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(x0, false), codes_f16(x1, false));
+            mma_f16_16816(acc[1], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(x0, true), codes_f16(x1, true));
+            mma_f16_16816(acc[2], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(y0, false), codes_f16(y1, false));
+            mma_f16_16816(acc[3], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(y0, true), codes_f16(y1, true));
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -514,7 +534,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
       mins[n] += __shfl_xor_sync(0xffffffffu, mins[n], 1);
       mins[n] += __shfl_xor_sync(0xffffffffu, mins[n], 2);
     }
-    const float f_e = pow2_field(e_run);    // a code counts 2^-24, p * scale 2^(14 + 127 - e)
+    const float f_even = pow2_field(e_run - 14), f_odd = pow2_field(e_run - 18);
     const bool whole = u_count == nu;
     const int64_t u0 = at - u_first;
     const int k = u0 <= w_a ? 0 : 1;
@@ -533,7 +553,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              r8[4 * e + i] = fmaf(o[sp][hv][i][e] * (i & 1 ? 64.f : 1024.f), f_e, mn) * inv;
+              r8[4 * e + i] = fmaf(o[sp][hv][i][e], i & 1 ? f_odd : f_even, mn) * inv;
           float4* p4 = reinterpret_cast<float4*>(dst + 64 * sp + 32 * hv + 8 * c);
           p4[0] = make_float4(r8[0], r8[1], r8[2], r8[3]);
           p4[1] = make_float4(r8[4], r8[5], r8[6], r8[7]);

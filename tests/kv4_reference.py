@@ -135,10 +135,10 @@ def attention(pool, table, length, q, scale):
     off, by element.
 
     With u = 2^-24 (half a float32 step): a score is sum over channels of
-    (q scale) (c s + m).  q's two fp16 terms are off by 2^-22 of it; the tensor
+    (q scale) ((c - 8) s + (m + 8 s)).  q's two fp16 terms are off by 2^-22 of it; the tensor
     core cuts each of its D / 8 partial sums (two terms, 16 channels a step) by
     at most 2u of it; scale, row factor, log2(e), the sums of q and the FMAs add
-    at most 16u more.  So with A = sum |q scale| (c s + |m|) log2(e) a base-2
+    at most 16u more.  So with A = sum |q scale| (|c - 8| s + |m + 8 s|) log2(e) a base-2
     score is off by E = A (2^-22 + 2u D / 8 + 16u).  A probability is off by
     E ln 2 for its own score and the same for the maximum's, by the exponent's
     rounding |s - max| 2u and by ex2's own 2^-22, so relatively by
@@ -146,7 +146,7 @@ def attention(pool, table, length, q, scale):
     rounded twice and held in two fp16 terms (2^-22 + 2u).  The weighted sums
     run over 32 tokens in the tensor core (4 steps, 2u each) and over at most
     n / 32 + 3 warps' and CTAs' pieces in float32, each with a rescaling (4u);
-    the denominator the same.  Out of that, with V = sum p (c s + |m|):
+    the denominator the same.  Out of that, with V = sum p (|c - 8| s + |m + 8 s|):
     |error| <= V (2 max e + 2^-22 + 2u + 8u + 2 * 4u (n / 32 + 8))."""
     n, heads, dim = q.shape
     hkv, u = pool.hkv, 2.0 ** -24
@@ -158,7 +158,7 @@ def attention(pool, table, length, q, scale):
     for key in (True, False):
         code, sc, low = pool.tokens(table, length, key)
         sc, low = (v.astype(np.float64).repeat(pool.group, -1) for v in (sc, low))
-        full.append((code * sc + low, code * sc + np.abs(low)))
+        full.append((code * sc + low, np.abs(code - 8.0) * sc + np.abs(low + 8 * sc)))
     (k, ka), (v, va) = full
     seen = np.arange(length)[None, :] <= (length - n + np.arange(n))[:, None]
     with np.errstate(all="ignore"):
