@@ -4,22 +4,23 @@
 //   k^_j = c_j s_j + m_j per group of channels (v^ likewise),
 // over the cached tokens j that row t may see (causal).
 //
-// The products run on the tensor cores with codes centred at 8: a nibble masked
-// into the fp16 number 1024 + c (or 1024 + 16 c for the nibble above it) less
-// 1032 (1152) is c - 8 (16 times that) exactly, so eight codes cost nine
-// operations.  Scale and minimum enter outside:
+// The products run on the tensor cores with the codes as they are: a nibble
+// masked in place in a 16-bit lane IS the fp16 number c * 2^-24 (a subnormal,
+// or 16 c * 2^-24 for the nibble above it), so eight codes cost five logic
+// operations and nothing is converted.  Scale and minimum enter outside:
 //   q . k^_j = sum_groups s_j (q . (c_j - 8)) + (m_j + 8 s_j) sum(q)
-//   sum_j p_j v^_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)
-// Centred, both sums of the second line are as small as the result; the codes
-// taken from 0 make them grow with the context while the result shrinks, and
-// the difference lost 2^-11 of it at 131,000 tokens.
-// q and p s are given as two fp16 terms each, high terms in rows 0..7 of the
-// MMA's A operand and low terms in rows 8..15, so one 16-row tile carries 8
-// query rows at float32's accuracy; both halves of an accumulator are added in
-// registers.  The tensor core cuts what an addition shifts out.  So q's high
-// terms are integers of 11 bits: their products with the codes and all sums of
-// them are exact.  p s, whose values differ by many powers of two, has 22 bits
-// of each value, and sums of 32 tokens at most run in the tensor core.
+//   sum_j p_j v^_j = sum_j w_j (c_j - 8) + sum_j p_j (m_j + 8 s_j),  w_j = p_j s_j
+// The codes count from 8, so that the sums are as small as the result: counted
+// from 0 they grow with the context while the result shrinks, and their
+// difference lost 2^-11 of it at 131,000 tokens.  The 8 is taken off in the
+// accumulators' first value: -8 sum(q), and -8 sum(w) out of one MMA.
+//
+// The codes are the A operand (16 tokens, or 16 channels of the values), q and
+// w the B operand: 4 query rows a tile, each as two columns, an integer of 11
+// bits and the fp16 rest of it.  The tensor core cuts what an addition shifts
+// out; sums of the integer columns stay below 2^24 and are exact, the rests
+// are small, and so products and sums have float32's accuracy.  w's integers
+// count from the largest w of the 32 tokens of a unit.
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -31,7 +32,6 @@ namespace {
 
 constexpr int kUnit = 32;        // tokens a warp takes at a time (two tiles)
 constexpr int kStages = 2;       // units in flight per warp
-constexpr int kRows = 8;         // query rows of a row tile
 // Warps of a CTA: with the ring of a 256-channel tile, six fill the shared memory.
 __host__ __device__ constexpr int warps_of(int d) { return d <= 128 ? 8 : 6; }
 
@@ -45,15 +45,18 @@ struct WsHead {
 };
 constexpr int kWsHeadBytes = 64;
 
-__host__ __device__ constexpr int part_floats(int d) { return kRows * (d + 2); }
+// A segment's query rows: 4 per column tile of the MMA's B operand.
+__host__ __device__ constexpr int rows_of(int nb) { return 4 * nb; }
+constexpr int kMaxNB = 2;
+__host__ __device__ constexpr int part_floats(int d, int nb) { return rows_of(nb) * (d + 2); }
 
 // Rings, then one kept piece per warp.
-constexpr int attn_smem(int d, int ng) {
-  return warps_of(d) * (kStages * 2 * tile_bytes(d, ng) + part_floats(d) * 4);
+constexpr int attn_smem(int d, int ng, int nb) {
+  return warps_of(d) * (kStages * 2 * tile_bytes(d, ng) + part_floats(d, nb) * 4);
 }
 
 size_t ws_bytes(int ctas, int d) {
-  return kWsHeadBytes + (size_t)ctas * sizeof(SegInfo) + (size_t)ctas * 2 * part_floats(d) * 4;
+  return kWsHeadBytes + (size_t)ctas * sizeof(SegInfo) + (size_t)ctas * 2 * part_floats(d, kMaxNB) * 4;
 }
 
 struct Args {
@@ -91,8 +94,9 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int64_t b) {
   return s;
 }
 __device__ __forceinline__ int seq_units(int len) { return max(1, (len + kUnit - 1) / kUnit); }
+template <int ROWS>
 __device__ __forceinline__ int seq_tiles(int n, int r) {
-  return (int)(((int64_t)n * r + kRows - 1) / kRows);
+  return (int)(((int64_t)n * r + ROWS - 1) / ROWS);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -105,27 +109,27 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
   return d;
 }
-// Two floats as fp16 high terms and the fp16 rests.
-__device__ __forceinline__ void split_f16x2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+// An integer up to 2^11 (nearest, halves to even) and the rest of x.
+__device__ __forceinline__ float int_part(float x) { return __fadd_rn(__fadd_rn(x, 12582912.f), -12582912.f); }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Two floats up to 2^11 as integers and fp16 rests, both times f.
-__device__ __forceinline__ void split_int(float x0, float x1, float f, uint32_t& hi, uint32_t& lo) {
-  const float r0 = rintf(x0), r1 = rintf(x1);
-  const __half2 h = __floats2half2_rn(r0 * f, r1 * f), l = __floats2half2_rn((x0 - r0) * f, (x1 - r1) * f);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+// 8 x 8 16-bit matrix, a row of two elements a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
-// The codes of the even (odd: 16 times them) nibbles of the low and the third
-// byte's half words, less 8, as two fp16 numbers.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w, bool odd) {
-  uint32_t v = lop3_and_or(w, odd ? 0x00F000F0u : 0x000F000Fu, 0x64006400u), r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(odd ? 0xE480E480u : 0xE408E408u));
-  return r;
+// D = A(16x16 f16, row) . B(16x8 f16, col) + C.
+__device__ __forceinline__ void mma_f16_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1,
+                                          float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 // 2^(e - 127) for an exponent field e clamped to the normal range.
 __device__ __forceinline__ float pow2_field(int e) {
@@ -154,9 +158,7 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// Attention of few rows per sequence (decode and short chunks).
-//
-// Work: a segment is 8 query rows (tokens x heads of one KV head) of one
+// Work: a segment is 4 NB query rows (tokens x heads of one KV head) of one
 // sequence over all its tokens; its units are 32 tokens.  All units of all
 // segments lie on one line that is cut evenly among the warps of a grid that
 // fits the GPU at once, whatever the lengths are.  A warp's pieces of
@@ -164,10 +166,11 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
 // that other CTAs continue go to the workspace for join_kernel.
 //
 // Each warp streams its tiles with bulk copies into its own two-stage ring.
-template <int D, int NG>
+template <int D, int NG, int NB>
 __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kernel(const Args a) {
   constexpr int NC = D / 32, NS = D / 64, G = D / NG, W = warps_of(D);
-  constexpr int TB = tile_bytes(D, NG), PF = part_floats(D);
+  constexpr int TB = tile_bytes(D, NG), PF = part_floats(D, NB), ROWS = rows_of(NB);
+  constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // codes, and 16 times them
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[W][kStages];
   __shared__ int64_t sh[33];
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
   auto line_units = [&](int64_t b) -> int64_t {
     if (b >= a.n_seqs) return 0;
     const Seq s = seq_of(a, b);
-    return (int64_t)seq_units(s.len) * seq_tiles(s.n, a.r) * a.hkv;
+    return (int64_t)seq_units(s.len) * seq_tiles<ROWS>(s.n, a.r) * a.hkv;
   };
   int64_t total = 0;
   for (int64_t b0 = 0; b0 < a.n_seqs; b0 += W * 32) {
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
   if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if it is the first cut
     const int64_t b = s_b[0], off = s_off[0];
     const Seq s = seq_of(a, b);
-    const int tiles = seq_tiles(s.n, a.r), nu = seq_units(s.len);
+    const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
     const int64_t seg = off / nu;
     SegInfo si;
     si.u0 = cta_a - (off - seg * nu);
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
   }
   for (int64_t at = w_a; at < w_b;) {
     const Seq s = seq_of(a, b);
-    const int tiles = seq_tiles(s.n, a.r), nu = seq_units(s.len);
+    const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
     if (off >= (int64_t)nu * tiles * a.hkv) {  // the next sequence
       off = 0;
       ++b;
@@ -262,59 +265,62 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     const int u_count = (int)min((int64_t)(nu - u_first), w_b - at);
     const int kvh = (int)(seg / tiles), tile = (int)(seg - (int64_t)kvh * tiles);
 
-    // this lane's query row (row g of the tile) and how far it sees
-    const int rr = tile * kRows + g;
-    const bool row_ok = rr < s.n * a.r;
-    const int tok = rr / a.r, hq = kvh * a.r + rr - tok * a.r;
-    const int limit = row_ok ? max(0, min(s.len, s.len - s.n + tok + 1)) : 0;
-    const int last_tok = min(s.n - 1, (tile * kRows + kRows - 1) / a.r);
+    // Rows of the tile: lane column g of B is row g / 2 (integer part, then
+    // rest); scores, softmax and outputs of row c are with the lanes c.
+    auto row_at = [&](int i, int& tok, int& hq) -> bool {
+      const int rr = tile * ROWS + i;
+      tok = rr / a.r;
+      hq = kvh * a.r + rr - tok * a.r;
+      return rr < s.n * a.r;
+    };
+    const int last_tok = min(s.n - 1, (tile * ROWS + ROWS - 1) / a.r);
     const int seg_len = max(0, min(s.len, s.len - s.n + last_tok + 1));  // no row sees further
+    const int all_see = s.len - s.n + tile * ROWS / a.r + 1;             // every row sees these
     const int u_live = min(u_first + u_count, (seg_len + kUnit - 1) / kUnit);
 
-    int32_t blk = 0;                        // the block of tile 2 * ids_at + lane
+    // Tiles are fetched by the lanes that know where they are: lane i has the
+    // place of tile 2 ids_at + i.
+    const uint8_t* src = nullptr;
+    uint32_t known = 0;                     // which of those are there
     int ids_at = -1024;
-    auto issue = [&](int u, int stage) -> int {
+    auto issue = [&](int u, int stage) -> uint32_t {
       if (u - ids_at >= 16) {
         ids_at = u;
-        const int64_t t0 = (int64_t)(2 * u + lane) * kTile;
-        blk = t0 < seg_len ? a.table[b * a.width + t0 / a.bs] : -1;
-        if (blk < 0 || blk >= a.n_blocks) {  // never read: its tokens are left out
-          if (t0 < seg_len && a.err) atomicExch(a.err, 4);
-          blk = -1;
-        }
-      }
-      const int p0 = __shfl_sync(0xffffffffu, blk, 2 * (u - ids_at));
-      const int p1 = __shfl_sync(0xffffffffu, blk, 2 * (u - ids_at) + 1);
-      if (lane == 0) {
+        const int64_t tt = 2 * (int64_t)u + lane;
+        const bool in = tt * kTile < seg_len;
+        const int64_t page = in ? tt * kTile / a.bs : 0;
+        const int blk = in ? a.table[b * a.width + page] : -1;
+        const bool ok = blk >= 0 && blk < a.n_blocks;
+        if (in && !ok && a.err) atomicExch(a.err, 4);  // never read: its tokens are left out
         const int per = a.bs / kTile;
-        mbar_arrive_expect_tx(&full[warp][stage], (p0 >= 0 ? TB : 0) + (p1 >= 0 ? TB : 0));
-        uint8_t* dst = ring + stage * 2 * TB;
-        if (p0 >= 0)
-          bulk_g2s(dst, a.cache + (((int64_t)p0 * a.hkv + kvh) * per + (2 * u) % per) * TB, TB,
-                   &full[warp][stage]);
-        if (p1 >= 0)
-          bulk_g2s(dst + TB, a.cache + (((int64_t)p1 * a.hkv + kvh) * per + (2 * u + 1) % per) * TB,
-                   TB, &full[warp][stage]);
+        src = a.cache + (((int64_t)blk * a.hkv + kvh) * per + (tt - page * per)) * TB;
+        known = __ballot_sync(0xffffffffu, ok);
       }
-      return (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+      const int at2 = 2 * (u - ids_at);
+      const uint32_t has = known >> at2 & 3u;
+      if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], __popc(has) * TB);
+      __syncwarp();
+      if ((lane >> 1) == u - ids_at && (has >> (lane & 1) & 1u))
+        bulk_g2s(ring + (stage * 2 + (lane & 1)) * TB, src, TB, &full[warp][stage]);
+      return has;
     };
-
-    // which of a stage's tiles are there: two bits a stage.  The stage of a
-    // unit follows the ring's position over the warp's whole life.
-    uint32_t there = 0;
+    uint32_t there = 0;                     // which of a stage's tiles are there: two bits a stage
     for (int i = 0; i < kStages; ++i)
       if (u_first + i < u_live) there |= issue(u_first + i, i) << (2 * i);
 
-    // ---- query fragments: two fp16 terms of q * scale * log2(e) * 2^k
-    uint32_t qf[NC][2][4];
-    float qsum[NG], row_f;
-    {
-      float x[NC][8], amax = 0.f;
+    // ---- B operand of the scores: q * scale * log2(e) on an integer grid
+    uint32_t qf[NB][NC][2][2];
+    float qsum[NB][NG], qc[NB][NG][2], row_f[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      int tok, hq;
+      const bool ok = row_at(nb * 4 + (g >> 1), tok, hq);
       const float* qr = a.q + ((s.row0 + tok) * a.h + hq) * D;
+      float x[NC][8], amax = 0.f;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-        if (row_ok) {
+        if (ok) {
           v0 = *reinterpret_cast<const float4*>(qr + 32 * j + 8 * c);
           v1 = *reinterpret_cast<const float4*>(qr + 32 * j + 8 * c + 4);
         }
@@ -326,48 +332,72 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
           amax = fmaxf(amax, fabsf(x[j][i]));
         }
       }
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        float t = 0.f;
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-          if (j * 32 / G == n)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t += x[j][i];
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
-        t += __shfl_xor_sync(0xffffffffu, t, 2);
-        qsum[n] = t;
-      }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // the largest magnitude goes to [2^10, 2^11): integers and their rests
-      const int e = max(14, min(244, exp_field(amax)));
+      // the largest magnitude goes to [2^10, 2^11)
+      const int e = max(14, min(240, exp_field(amax)));
       const float up = pow2_field(264 - e);
-      row_f = pow2_field(e - 10);           // 1 / up
+      float sum[NG], grid[NG];              // of q, and of this column's fp16 values
 #pragma unroll
-      for (int j = 0; j < NC; ++j)
+      for (int n = 0; n < NG; ++n) sum[n] = grid[n] = 0.f;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {       // even nibbles, then odd ones (16 c)
-          const float f = p ? 0.0625f : 1.f;
-          split_int(x[j][p] * up, x[j][p + 4] * up, f, qf[j][p][0], qf[j][p][1]);
-          split_int(x[j][p + 2] * up, x[j][p + 6] * up, f, qf[j][p][2], qf[j][p][3]);
+      for (int j = 0; j < NC; ++j) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sum[j * 32 / G] += x[j][i];
+          const float v = x[j][i] * up, hi = rintf(v);
+          y[i] = g & 1 ? v - hi : hi;
+          if (i & 1) y[i] *= 0.0625f;       // odd nibbles count 16 times
         }
+        // k = 2c, 2c + 1 and 2c + 8, 2c + 9: nibbles 0, 4 and 2, 6 (1, 5 and 3, 7)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            qf[nb][j][p][i] = pack_f16x2(y[p + 2 * i], y[p + 2 * i + 4]);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[nb][j][p][i]));
+            grid[j * 32 / G] += (f.x + f.y) * (p ? 16.f : 1.f);
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
+        sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
+        grid[n] += __shfl_xor_sync(0xffffffffu, grid[n], 1);
+        grid[n] += __shfl_xor_sync(0xffffffffu, grid[n], 2);
+        // from row g / 2 to row c: lanes 8c (integers) and 8c + 4 (rests)
+        qsum[nb][n] = __shfl_sync(0xffffffffu, sum[n], 8 * c);
+        qc[nb][n][0] = __shfl_sync(0xffffffffu, grid[n], 8 * c) * -0x1p-21f;
+        qc[nb][n][1] = __shfl_sync(0xffffffffu, grid[n], 8 * c + 4) * -0x1p-21f;
+      }
+      row_f[nb] = __shfl_sync(0xffffffffu, pow2_field(e + 14), 8 * c);  // 2^24 / up
+    }
+    int limit[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      int tok, hq;
+      const bool ok = row_at(nb * 4 + c, tok, hq);
+      limit[nb] = ok ? max(0, min(s.len, s.len - s.n + tok + 1)) : 0;
     }
 
     // ---- online softmax over the units
-    float m = -INFINITY, l = 0.f, mins[NG];
-    float o[NS][2][4][2];                   // [span][half][nibble][column]
-    int e_run = 20;                         // exponent field of the largest value scale so far
+    float m[NB], l[NB], mins[NB][NG];
+    float o[NB][NS][2][2][2];               // [span][half][pair][nibble], times 2^-12
 #pragma unroll
-    for (int n = 0; n < NG; ++n) mins[n] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = -INFINITY;
+      l[nb] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+      for (int n = 0; n < NG; ++n) mins[nb][n] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][j][k][0] = o[i][j][k][1] = 0.f;
-
-    const int pi = g ^ ((g >> 1) & 1);      // the token of key column g
+        for (int k = 0; k < 8; ++k) o[nb][i][k >> 2][(k >> 1) & 1][k & 1] = 0.f;
+    }
+    // Row i of a tile's MMAs is token i ^ (i >> 1 & 1), so that the value rows
+    // that the four lanes of a quad read together lie in different banks.
+    const int tg = g ^ ((g >> 1) & 1);
     bool failed = false;
     for (int u = u_first, st = 0; u < u_live; ++u, st ^= 1) {
       if (!mbar_wait(&full[warp][st], (phase >> st) & 1u)) {
@@ -377,100 +407,96 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
       }
       phase ^= 1u << st;
       const uint8_t* buf = ring + st * 2 * TB;
-      const uint32_t has = there >> (2 * st);
+      const uint32_t has = there >> (2 * st) & 3u;
+      const bool whole_unit = has == 3u && (u + 1) * kUnit <= all_see;
 
-      // Scores.  Column n of a key tile is token n ^ (n >> 1 & 1): the two
-      // columns of a lane stay two neighbouring tokens, and the value rows
-      // that the four lanes of a quad read lie in different banks.
-      float sc[2][2][2];                    // [tile][8-token half][column]
+      // scores of tokens tg and tg + 8 of both tiles
+      float sc[NB][2][2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        uint32_t wa[NC], wb[NC];
+        lds<NC>(buf + t * TB + tg * (D / 2) + c * NC * 4, wa);
+        lds<NC>(buf + t * TB + (tg + 8) * (D / 2) + c * NC * 4, wb);
+        float acc[NB][NG][4];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t w[NC];
-          lds<NC>(buf + t * TB + (hf * 8 + pi) * (D / 2) + c * NC * 4, w);
-          float acc[NG][4];
+        for (int j = 0; j < NC; ++j) {
+          constexpr int kPer = G / 32;
+          const uint32_t xa = wa[j] >> 8, xb = wb[j] >> 8;
 #pragma unroll
-          for (int n = 0; n < NG; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-#pragma unroll
-          for (int j = 0; j < NC; ++j) {
-            const uint32_t w8 = w[j] >> 8;
-            mma_f16_16816(acc[j * 32 / G], qf[j][0][0], qf[j][0][1], qf[j][0][2], qf[j][0][3],
-                          codes_f16(w[j], false), codes_f16(w8, false));
-            mma_f16_16816(acc[j * 32 / G], qf[j][1][0], qf[j][1][1], qf[j][1][2], qf[j][1][3],
-                          codes_f16(w[j], true), codes_f16(w8, true));
+          for (int nb = 0; nb < NB; ++nb) {
+            float (&d)[4] = acc[nb][j / kPer];
+            const float* z = qc[nb][j / kPer];
+            if (j % kPer == 0)
+              mma_f16_c(d, wa[j] & kEven, wb[j] & kEven, xa & kEven, xb & kEven, qf[nb][j][0][0],
+                        qf[nb][j][0][1], z[0], z[1], z[0], z[1]);
+            else
+              mma_f16_16816(d, wa[j] & kEven, wb[j] & kEven, xa & kEven, xb & kEven,
+                            qf[nb][j][0][0], qf[nb][j][0][1]);
+            mma_f16_16816(d, wa[j] & kOdd, wb[j] & kOdd, xa & kOdd, xb & kOdd, qf[nb][j][1][0],
+                          qf[nb][j][1][1]);
           }
-          float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            const float4 p = *reinterpret_cast<const float4*>(
-                buf + t * TB + k_params_at(D) + (n * kTile + hf * 8 + 2 * c) * 8);
-            const float a0 = (acc[n][0] + acc[n][2]) * row_f, a1 = (acc[n][1] + acc[n][3]) * row_f;
-            const float k0 = c & 1 ? p.z : p.x, k1 = c & 1 ? p.x : p.z;
-            s0 = fmaf(a0, k0, fmaf(qsum[n], fmaf(8.f, k0, c & 1 ? p.w : p.y), s0));
-            s1 = fmaf(a1, k1, fmaf(qsum[n], fmaf(8.f, k1, c & 1 ? p.y : p.w), s1));
-          }
-          const int t0 = u * kUnit + t * kTile + hf * 8 + 2 * c;
-          const bool in = (has >> t) & 1u;
-          sc[t][hf][0] = in && t0 + (c & 1) < limit ? s0 : -INFINITY;
-          sc[t][hf][1] = in && t0 + 1 - (c & 1) < limit ? s1 : -INFINITY;
         }
-      float mu = sc[0][0][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mu = fmaxf(mu, sc[i >> 2][(i >> 1) & 1][i & 1]);
-      mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, 1));
-      mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, 2));
-      const float m_new = fmaxf(m, mu);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = ex2(m - ref);      // 0 while nothing was seen
-      m = m_new;
-
-      // {scale, minimum} of the values of this lane's tokens; tokens past the
-      // end and blocks that are not there count as zeros, whatever lies there
-      auto v_params = [&](int n, int t, int hf) -> float4 {
-        const float4 p = *reinterpret_cast<const float4*>(
-            buf + t * TB + v_params_at(D, NG) + (n * kTile + hf * 8 + 2 * c) * 8);
-        const int t0 = u * kUnit + t * kTile + hf * 8 + 2 * c;
-        const bool in = (has >> t) & 1u;
-        const bool ok0 = in && t0 < seg_len, ok1 = in && t0 + 1 < seg_len;
-        const float4 q = make_float4(ok0 ? p.x : 0.f, ok0 ? p.y : 0.f, ok1 ? p.z : 0.f, ok1 ? p.w : 0.f);
-        return c & 1 ? make_float4(q.z, q.w, q.x, q.y) : q;
-      };
-      float vmax = 0.f;
+        for (int nb = 0; nb < NB; ++nb) sc[nb][t][0] = sc[nb][t][1] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+        for (int n = 0; n < NG; ++n) {
+          const float2* p = reinterpret_cast<const float2*>(buf + t * TB + k_params_at(D)) + n * kTile + tg;
+          const float2 pa = p[0], pb = p[8];
+          const float ma = fmaf(8.f, pa.x, pa.y), mb = fmaf(8.f, pb.x, pb.y);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const float (&d)[4] = acc[nb][n];
+            sc[nb][t][0] = fmaf((d[0] + d[1]) * row_f[nb], pa.x, fmaf(qsum[nb][n], ma, sc[nb][t][0]));
+            sc[nb][t][1] = fmaf((d[2] + d[3]) * row_f[nb], pb.x, fmaf(qsum[nb][n], mb, sc[nb][t][1]));
+          }
+        }
+      }
+      if (!whole_unit)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tt = u * kUnit + (i >> 1) * kTile + (i & 1) * 8 + tg;
+            if (tt >= limit[nb] || !(has >> (i >> 1) & 1u)) sc[nb][i >> 1][i & 1] = -INFINITY;
+          }
+      float corr[NB];
+      bool moved = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float mu = fmaxf(fmaxf(sc[nb][0][0], sc[nb][0][1]), fmaxf(sc[nb][1][0], sc[nb][1][1]));
+        mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, 4));
+        mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, 8));
+        mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, 16));
+        const float m_new = fmaxf(m[nb], mu);
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        corr[nb] = ex2(m[nb] - ref);        // 0 while nothing was seen
+        moved |= m_new != m[nb];
+        m[nb] = m_new;
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 p = v_params(n, i >> 1, i & 1);
-          vmax = fmaxf(vmax, fmaxf(p.x, p.z));
+          float& v = sc[nb][i >> 1][i & 1];
+          const float p = ex2(v - ref);
+          sum += p;
+          v = v == -INFINITY ? -1.f : p;    // a negative p marks a masked token
         }
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-      // p * scale goes to the fp16 range by the power of two that brings the
-      // largest scale so far to [2^14, 2^15)
-      const int e_new = max(e_run, min(254, exp_field(vmax)));
-      const float corr_o = e_new - e_run > 126 ? 0.f : corr * pow2_field(127 - (e_new - e_run));
-      e_run = e_new;
-      const float up = pow2_field(268 - e_run);
+        l[nb] = fmaf(l[nb], corr[nb], sum);
+      }
+      if (__any_sync(0xffffffffu, moved))
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mins[nb][n] *= corr[nb];
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[nb][i][k >> 2][(k >> 1) & 1][k & 1] *= corr[nb];
+        }
 
-      // masked tokens are marked by a negative p
-      l *= corr;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float p = ex2(sc[t][hf][e] - ref);
-            l += p;
-            sc[t][hf][e] = sc[t][hf][e] == -INFINITY ? -1.f : p;
-          }
-
-      // Values, half a span (32 channels, one group) at a time.  A unit's
-      // products are summed apart and then added, so that the tensor core's
-      // own accumulation never runs over more than 32 tokens.
-      uint32_t pa[2][4];
-      uint32_t vw[2][4][NS];                // the rows of this lane's 8 tokens
+      // Values, half a span (32 channels, one group) at a time: rows i of an
+      // MMA are channel 4i + nibble, rows i + 8 the next one.  A unit's
+      // products are summed apart and then added.
+      uint32_t vw[2][4][NS];                // rows of this lane's 8 tokens
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -478,48 +504,76 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
           const int row = (i >> 1) * 8 + 2 * c + ((i & 1) ^ (c & 1));
           lds<NS>(buf + t * TB + v_codes_at(D) + row * (D / 2) + g * NS * 4, vw[t][i]);
         }
+      uint32_t wf[NB][2][2];                // B operand: w of a group
+      float base[NB][4], f_even[NB], f_odd[NB];
 #pragma unroll
       for (int sp = 0; sp < NS; ++sp)
 #pragma unroll
         for (int hv = 0; hv < 2; ++hv) {
           const int n = (64 * sp + 32 * hv) / G;
           if ((64 * sp + 32 * hv) % G == 0) {
-            mins[n] *= corr;
+            float2 vp[4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int i = 0; i < 4; ++i)
+              vp[i] = reinterpret_cast<const float2*>(buf + (i >> 1) * TB + v_params_at(D, NG))[n * kTile + (i & 1) * 8 + tg];
 #pragma unroll
-              for (int hf = 0; hf < 2; ++hf) {
-                const float4 p = v_params(n, t, hf);
-                const float p0 = sc[t][hf][0], p1 = sc[t][hf][1];
-                const float w0 = p0 < 0.f ? 0.f : p0 * (p.x * up);
-                const float w1 = p1 < 0.f ? 0.f : p1 * (p.z * up);
-                if (!(p0 < 0.f)) mins[n] = fmaf(p0, fmaf(8.f, p.x, p.y), mins[n]);
-                if (!(p1 < 0.f)) mins[n] = fmaf(p1, fmaf(8.f, p.z, p.w), mins[n]);
-                split_f16x2(w0, w1, pa[t][2 * hf], pa[t][2 * hf + 1]);
+            for (int nb = 0; nb < NB; ++nb) {
+              float w[4], wmax = 0.f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p = sc[nb][i >> 1][i & 1];
+                const bool in = !(p < 0.f);
+                w[i] = in ? p * vp[i].x : 0.f;
+                mins[nb][n] = in ? fmaf(p, fmaf(8.f, vp[i].x, vp[i].y), mins[nb][n]) : mins[nb][n];
+                wmax = fmaxf(wmax, w[i]);
               }
-          }
-          float acc[4][4];
+              wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 4));
+              wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 8));
+              wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 16));
+              const int e = max(14, min(252, exp_field(wmax)));
+              const float up = pow2_field(264 - e);
+              f_even[nb] = pow2_field(e + 2);   // 2^24 / up, times 2^-12
+              f_odd[nb] = f_even[nb] * 0.0625f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+              for (int i = 0; i < 4; ++i) {
+                const float v = w[i] * up, hi = int_part(v);
+                wf[nb][i >> 1][i & 1] = transpose8(pack_f16x2(hi, v - hi));
+              }
+              // -8 sum(w), for the rows of even and of odd nibbles
+              const uint32_t z0 = 0x80088008u, z1 = 0x80808080u;  // -8, -128 times 2^-24
+              mma_f16_c(base[nb], z0, z1, z0, z1, wf[nb][0][0], wf[nb][0][1], 0.f, 0.f, 0.f, 0.f);
+              mma_f16_16816(base[nb], z0, z1, z0, z1, wf[nb][1][0], wf[nb][1][1]);
+            }
+          }
+          uint32_t x[2][2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const uint32_t x0 = prmt(vw[t][0][sp], vw[t][1][sp], hv ? 0x7632 : 0x5410);
-            const uint32_t x1 = prmt(vw[t][2][sp], vw[t][3][sp], hv ? 0x7632 : 0x5410);
-            const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-            mma_f16_16816(acc[0], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(x0, false), codes_f16(x1, false));
-            mma_f16_16816(acc[1], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(x0, true), codes_f16(x1, true));
-            mma_f16_16816(acc[2], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(y0, false), codes_f16(y1, false));
-            mma_f16_16816(acc[3], pa[t][0], pa[t][1], pa[t][2], pa[t][3], codes_f16(y0, true), codes_f16(y1, true));
+            x[t][0] = prmt(vw[t][0][sp], vw[t][1][sp], hv ? 0x7632 : 0x5410);
+            x[t][1] = prmt(vw[t][2][sp], vw[t][3][sp], hv ? 0x7632 : 0x5410);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[sp][hv][i][0] = fmaf(o[sp][hv][i][0], corr_o, acc[i][0] + acc[i][2]);
-            o[sp][hv][i][1] = fmaf(o[sp][hv][i][1], corr_o, acc[i][1] + acc[i][3]);
+          for (int pr = 0; pr < 2; ++pr) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              float d[4];
+              mma_f16_c(d, x[0][0] & kEven, x[0][0] & kOdd, x[0][1] & kEven, x[0][1] & kOdd,
+                        wf[nb][0][0], wf[nb][0][1], base[nb][0], base[nb][1], base[nb][2], base[nb][3]);
+              mma_f16_16816(d, x[1][0] & kEven, x[1][0] & kOdd, x[1][1] & kEven, x[1][1] & kOdd,
+                            wf[nb][1][0], wf[nb][1][1]);
+              float (&oo)[2] = o[nb][sp][hv][pr];
+              oo[0] = fmaf(d[0] + d[1], f_even[nb], oo[0]);
+              oo[1] = fmaf(d[2] + d[3], f_odd[nb], oo[1]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              x[t][0] >>= 8;
+              x[t][1] >>= 8;
+            }
           }
         }
       __syncwarp();                         // the stage's readers are done
       if (u + kStages < u_live)
-        there = (there & ~(3u << (2 * st))) | (uint32_t)issue(u + kStages, st) << (2 * st);
+        there = (there & ~(3u << (2 * st))) | issue(u + kStages, st) << (2 * st);
     }
     if (failed) {  // the copies still in flight, then out; the answer is not valid
       for (int st = 0; st < kStages; ++st) (void)mbar_wait(&full[warp][st], (phase >> st) & 1u);
@@ -527,50 +581,46 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     }
 
     // ---- the piece's sums, in real units
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      mins[n] += __shfl_xor_sync(0xffffffffu, mins[n], 1);
-      mins[n] += __shfl_xor_sync(0xffffffffu, mins[n], 2);
-    }
-    const float f_even = pow2_field(e_run - 14), f_odd = pow2_field(e_run - 18);
     const bool whole = u_count == nu;
     const int64_t u0 = at - u_first;
     const int k = u0 <= w_a ? 0 : 1;
     // a piece at the warp's last unit lies in the ring, whose copies are all read
     float* piece = k ? reinterpret_cast<float*>(ring) : kept;
-    float* dst = whole ? a.out + ((s.row0 + tok) * a.h + hq) * D : piece + g * D;
-    const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-    if (row_ok || !whole)
 #pragma unroll
-      for (int sp = 0; sp < NS; ++sp)
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int hv = 0; hv < 2; ++hv) {
-          const float mn = mins[(64 * sp + 32 * hv) / G];
-          float r8[8];
+      for (int x = 4; x < 32; x <<= 1) {
+        l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              r8[4 * e + i] = fmaf(o[sp][hv][i][e], i & 1 ? f_odd : f_even, mn) * inv;
-          float4* p4 = reinterpret_cast<float4*>(dst + 64 * sp + 32 * hv + 8 * c);
-          p4[0] = make_float4(r8[0], r8[1], r8[2], r8[3]);
-          p4[1] = make_float4(r8[4], r8[5], r8[6], r8[7]);
-        }
-    if (!whole) {
-      if (c == 0) {
-        piece[kRows * D + g] = m;
-        piece[kRows * D + kRows + g] = l;
+        for (int n = 0; n < NG; ++n) mins[nb][n] += __shfl_xor_sync(0xffffffffu, mins[nb][n], x);
       }
-      if (lane == 0) {
-        SegInfo& si = s_seg[warp][k];
-        si.u0 = u0;
-        si.u1 = u0 + nu;
-        si.b = (int32_t)b;
-        si.kvh = kvh;
-        si.tile = tile;
+      int tok, hq;
+      const bool ok = row_at(nb * 4 + c, tok, hq);
+      float* dst = whole ? a.out + ((s.row0 + tok) * a.h + hq) * D : piece + (nb * 4 + c) * D;
+      const float inv = !whole ? 1.f : l[nb] == 0.f ? 0.f : 1.f / l[nb];
+      if (ok || !whole)
+#pragma unroll
+        for (int sp = 0; sp < NS; ++sp)
+#pragma unroll
+          for (int hv = 0; hv < 2; ++hv) {
+            const float mn = mins[nb][(64 * sp + 32 * hv) / G];
+            const float (&oo)[2][2] = o[nb][sp][hv];
+            *reinterpret_cast<float4*>(dst + 64 * sp + 32 * hv + 4 * g) =
+                make_float4(fmaf(oo[0][0], 4096.f, mn) * inv, fmaf(oo[0][1], 4096.f, mn) * inv,
+                            fmaf(oo[1][0], 4096.f, mn) * inv, fmaf(oo[1][1], 4096.f, mn) * inv);
+          }
+      if (!whole && g == 0) {
+        piece[ROWS * D + nb * 4 + c] = m[nb];
+        piece[ROWS * D + ROWS + nb * 4 + c] = l[nb];
       }
+    }
+    if (!whole && lane == 0) {
+      SegInfo& si = s_seg[warp][k];
+      si.u0 = u0;
+      si.u1 = u0 + nu;
+      si.b = (int32_t)b;
+      si.kvh = kvh;
+      si.tile = tile;
     }
     at += u_count;
     off += u_count;
@@ -593,22 +643,22 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
     const Seq s = seq_of(a, si.b);
     float* slot = parts + (size_t)(2 * cta + (si.u0 <= cta_a ? 0 : 1)) * PF;
-    for (int x = tid; x < kRows * D; x += W * 32) {
+    for (int x = tid; x < ROWS * D; x += W * 32) {
       const int row = x / D, d = x - row * D;
       float M = -INFINITY;
       for (int j = i; j < end; ++j)
-        if (s_seg[j >> 1][j & 1].u0 >= 0) M = fmaxf(M, piece_at(j)[kRows * D + row]);
+        if (s_seg[j >> 1][j & 1].u0 >= 0) M = fmaxf(M, piece_at(j)[ROWS * D + row]);
       const float ref = M == -INFINITY ? 0.f : M;
       float L = 0.f, acc = 0.f;
       for (int j = i; j < end; ++j)
         if (s_seg[j >> 1][j & 1].u0 >= 0) {
           const float* p = piece_at(j);
-          const float f = ex2(p[kRows * D + row] - ref);
-          L = fmaf(f, p[kRows * D + kRows + row], L);
+          const float f = ex2(p[ROWS * D + row] - ref);
+          L = fmaf(f, p[ROWS * D + ROWS + row], L);
           acc = fmaf(f, p[x], acc);
         }
       if (whole) {
-        const int rr = si.tile * kRows + row;
+        const int rr = si.tile * ROWS + row;
         if (rr < s.n * a.r) {
           const int tok = rr / a.r, hq = si.kvh * a.r + rr - tok * a.r;
           a.out[((s.row0 + tok) * a.h + hq) * D + d] = L == 0.f ? 0.f : acc / L;
@@ -616,8 +666,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
       } else {
         slot[x] = acc;
         if (d == 0) {
-          slot[kRows * D + row] = M;
-          slot[kRows * D + kRows + row] = L;
+          slot[ROWS * D + row] = M;
+          slot[ROWS * D + ROWS + row] = L;
         }
       }
     }
@@ -629,9 +679,9 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
 // that CTA i's beginning cuts, if that is the segment's first cut.  Its parts
 // are taken in the order of the CTAs, so the result does not depend on timing.
 constexpr int kJoinThreads = 256;
-template <int D>
+template <int D, int NB>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
-  constexpr int PF = part_floats(D), GR = kJoinThreads / D;
+  constexpr int PF = part_floats(D, NB), ROWS = rows_of(NB), GR = kJoinThreads / D;
   extern __shared__ __align__(16) float wgt[];  // one weight per part
   __shared__ float red[kJoinThreads];
   __shared__ float s_m[32], s_l[32];
@@ -644,7 +694,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
   const SegInfo si = info[cta];
   if (si.u0 < 0) return;
   const Seq s = seq_of(a, si.b);
-  const int rr = si.tile * kRows + row;
+  const int rr = si.tile * ROWS + row;
   if (rr >= s.n * a.r) return;
   const WsHead hd = *reinterpret_cast<const WsHead*>(a.ws);
   // the segment's parts: CTA cta - 1, then cta .. up to the one that holds its end
@@ -659,7 +709,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
     return parts + (size_t)(2 * x + (second ? 1 : 0)) * PF;
   };
   float M = -INFINITY;
-  for (int j = tid; j < n; j += kJoinThreads) M = fmaxf(M, part(j)[kRows * D + row]);
+  for (int j = tid; j < n; j += kJoinThreads) M = fmaxf(M, part(j)[ROWS * D + row]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if ((tid & 31) == 0) s_m[tid >> 5] = M;
@@ -670,9 +720,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
   float L = 0.f;
   for (int j = tid; j < n; j += kJoinThreads) {
     const float* p = part(j);
-    const float f = ex2(p[kRows * D + row] - ref);
+    const float f = ex2(p[ROWS * D + row] - ref);
     wgt[j] = f;
-    L = fmaf(f, p[kRows * D + kRows + row], L);
+    L = fmaf(f, p[ROWS * D + ROWS + row], L);
   }
   L = warp_sum(L);
   if ((tid & 31) == 0) s_l[tid >> 5] = L;
@@ -700,13 +750,20 @@ int grid_of(int d) {
   return (c ? c->num_sms : 148) * (d <= 128 ? 2 : 1);
 }
 
-template <int D, int NG>
-int run_attn(const Args& a, cudaStream_t st) {
-  const int smem = attn_smem(D, NG);
-  NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG>, smem));
+template <int D, int NG, int NB>
+int run_nb(const Args& a, cudaStream_t st) {
+  const int smem = attn_smem(D, NG, NB);
+  NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
   const int ctas = grid_of(D);
-  NIMF_TRY(launch(attn_kernel<D, NG>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
-  return launch(join_kernel<D>, dim3(ctas, kRows), kJoinThreads, (size_t)ctas * 4, st, 1, a);
+  NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
+  return launch(join_kernel<D, NB>, dim3(ctas, rows_of(NB)), kJoinThreads, (size_t)ctas * 4, st, 1, a);
+}
+
+// 4 rows a segment where no sequence should have more of them for a KV head:
+// half the tensor work, registers and partial results of 8.
+template <int D, int NG>
+int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
+  return max_new * a.r <= 4 ? run_nb<D, NG, 1>(a, st) : run_nb<D, NG, 2>(a, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -775,14 +832,14 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   a.bs = s.bs;
   a.scale2 = (float)((double)scale * 1.4426950408889634);
   switch (s.d * 16 + s.d / s.group) {
-    case 64 * 16 + 1: return kv4::run_attn<64, 1>(a, st);
-    case 64 * 16 + 2: return kv4::run_attn<64, 2>(a, st);
-    case 128 * 16 + 1: return kv4::run_attn<128, 1>(a, st);
-    case 128 * 16 + 2: return kv4::run_attn<128, 2>(a, st);
-    case 128 * 16 + 4: return kv4::run_attn<128, 4>(a, st);
-    case 256 * 16 + 2: return kv4::run_attn<256, 2>(a, st);
-    case 256 * 16 + 4: return kv4::run_attn<256, 4>(a, st);
-    default: return kv4::run_attn<256, 8>(a, st);
+    case 64 * 16 + 1: return kv4::run_attn<64, 1>(a, max_new, st);
+    case 64 * 16 + 2: return kv4::run_attn<64, 2>(a, max_new, st);
+    case 128 * 16 + 1: return kv4::run_attn<128, 1>(a, max_new, st);
+    case 128 * 16 + 2: return kv4::run_attn<128, 2>(a, max_new, st);
+    case 128 * 16 + 4: return kv4::run_attn<128, 4>(a, max_new, st);
+    case 256 * 16 + 2: return kv4::run_attn<256, 2>(a, max_new, st);
+    case 256 * 16 + 4: return kv4::run_attn<256, 4>(a, max_new, st);
+    default: return kv4::run_attn<256, 8>(a, max_new, st);
   }
 }
 

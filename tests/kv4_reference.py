@@ -135,19 +135,22 @@ def attention(pool, table, length, q, scale):
     off, by element.
 
     With u = 2^-24 (half a float32 step): a score is sum over channels of
-    (q scale) ((c - 8) s + (m + 8 s)).  q's two fp16 terms are off by 2^-22 of it; the tensor
-    core cuts each of its D / 8 partial sums (two terms, 16 channels a step) by
-    at most 2u of it; scale, row factor, log2(e), the sums of q and the FMAs add
-    at most 16u more.  So with A = sum |q scale| (|c - 8| s + |m + 8 s|) log2(e) a base-2
-    score is off by E = A (2^-22 + 2u D / 8 + 16u).  A probability is off by
-    E ln 2 for its own score and the same for the maximum's, by the exponent's
-    rounding |s - max| 2u and by ex2's own 2^-22, so relatively by
-    e = 2 E ln 2 + 2^-22 + 2u |s - max|; its product with the value scale is
-    rounded twice and held in two fp16 terms (2^-22 + 2u).  The weighted sums
-    run over 32 tokens in the tensor core (4 steps, 2u each) and over at most
-    n / 32 + 3 warps' and CTAs' pieces in float32, each with a rescaling (4u);
-    the denominator the same.  Out of that, with V = sum p (|c - 8| s + |m + 8 s|):
-    |error| <= V (2 max e + 2^-22 + 2u + 8u + 2 * 4u (n / 32 + 8))."""
+    (q scale) ((c - 8) s + (m + 8 s)).  q enters on a grid of 2^-10 of its row's
+    largest magnitude Q at most, the rest of a grid step in fp16: off by 2^-23 Q
+    a channel.  The tensor core cuts each of its D / 8 partial sums by at most
+    2u of it; scale, row factor, log2(e), the sums of q and the FMAs add at most
+    16u more.  So with A = sum |q scale| (|c - 8| s + |m + 8 s|) log2(e) a base-2
+    score is off by E = A (2u D / 8 + 16u) + 2^-23 Q scale log2(e) sum |c - 8| s.
+    A probability is off by E ln 2 for its own score and the same for the
+    maximum's, by the exponent's rounding |s - max| 2u and by ex2's own 2^-22,
+    so relatively by e = 2 E ln 2 + 2^-22 + 2u |s - max|; w = p s is rounded
+    twice (2u) and enters as q does, on a grid of the largest w of 32 tokens:
+    2^-23 of that a token.  The weighted sums run over 32 tokens in the tensor
+    core (4 steps, 2u each) and over at most n / 32 + 3 units, warps' and CTAs'
+    pieces in float32, each with a rescaling (4u); the denominator the same.
+    With V = sum p (|c - 8| s + |m + 8 s|):
+    |error| <= V (2 max e + 2^-22 + 2u + 8u + 2 * 4u (n / 32 + 8))
+               + 2^-23 sum over units (max w) (sum |c - 8|)."""
     n, heads, dim = q.shape
     hkv, u = pool.hkv, 2.0 ** -24
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -158,8 +161,9 @@ def attention(pool, table, length, q, scale):
     for key in (True, False):
         code, sc, low = pool.tokens(table, length, key)
         sc, low = (v.astype(np.float64).repeat(pool.group, -1) for v in (sc, low))
-        full.append((code * sc + low, np.abs(code - 8.0) * sc + np.abs(low + 8 * sc)))
-    (k, ka), (v, va) = full
+        full.append((code * sc + low, np.abs(code - 8.0) * sc + np.abs(low + 8 * sc), np.abs(code - 8.0), sc))
+    (k, ka, kc, ks), (v, va, vc, vs) = full
+    units = -(-length // 32)
     seen = np.arange(length)[None, :] <= (length - n + np.arange(n))[:, None]
     with np.errstate(all="ignore"):
         for h in range(heads):
@@ -177,9 +181,16 @@ def attention(pool, table, length, q, scale):
             vaz = np.where(seen.any(0)[:, None], va[:, g], 0.0)
             out[:, h] = pv @ vz
             far = np.where(seen & (p > 0), np.abs(s - top), 0.0) * math.log2(math.e)
-            e = 2 * big.max(-1, keepdims=True) * (2.0 ** -22 + u * dim / 4 + 16 * u) * math.log(2) + 2.0 ** -22
+            grid = np.where(seen, np.abs(qs).max(-1, keepdims=True) * (kc[:, g] * ks[:, g]).sum(-1), 0.0) * math.log2(math.e) * 2.0 ** -23
+            e = 2 * (big * (u * dim / 4 + 16 * u) + grid).max(-1, keepdims=True) * math.log(2) + 2.0 ** -22
             rel = 2 * (e + 2 * u * (pv * far).sum(-1, keepdims=True)) + 2.0 ** -22 + 10 * u + 8 * u * (length / 32 + 8)
-            tol[:, h] = (pv @ vaz) * rel
+            for n0 in range(0, dim, pool.group):       # the grid of w, unit by unit
+                w = np.zeros((n, units * 32))
+                w[:, :length] = np.where(seen, pv * np.where(seen.any(0), vs[:, g, n0], 0.0), 0.0)
+                c8 = np.zeros((units * 32, pool.group))
+                c8[:length] = vc[:, g, n0:n0 + pool.group]
+                tol[:, h, n0:n0 + pool.group] = 2.0 ** -23 * w.reshape(n, units, 32).max(-1) @ c8.reshape(units, 32, -1).sum(1)
+            tol[:, h] += (pv @ vaz) * rel
     return out, tol + 1e-30
 
 
