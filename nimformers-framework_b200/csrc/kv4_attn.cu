@@ -35,15 +35,15 @@ constexpr int kStages = 2;       // units in flight per warp
 // Warps of a CTA: with the ring of a 256-channel tile, six fill the shared memory.
 __host__ __device__ constexpr int warps_of(int d) { return d <= 128 ? 8 : 6; }
 
-// One CTA's share that begins inside a segment; written for the join.
+// A kept piece of a segment, and (in the workspace) the segment that a CTA's
+// beginning cuts first: u0 its first unit on the line, -1 for none.
 struct SegInfo {
-  int64_t u0, u1;   // the segment's units; u0 < 0: this CTA starts no join
-  int32_t b, kvh, tile, pad;
+  int64_t u0, u1;
+  int32_t b, kvh, tile;
+  int32_t parts;    // join: CTAs that hold a part, counted from the one before
+  int32_t second;   // join: the first of them holds it as its last segment
+  int32_t pad;
 };
-struct WsHead {
-  int64_t units, ctas;
-};
-constexpr int kWsHeadBytes = 64;
 
 // A segment's query rows: 4 per column tile of the MMA's B operand.
 __host__ __device__ constexpr int rows_of(int nb) { return 4 * nb; }
@@ -56,7 +56,7 @@ constexpr int attn_smem(int d, int ng, int nb) {
 }
 
 size_t ws_bytes(int ctas, int d) {
-  return kWsHeadBytes + (size_t)ctas * sizeof(SegInfo) + (size_t)ctas * 2 * part_floats(d, kMaxNB) * 4;
+  return (size_t)ctas * sizeof(SegInfo) + (size_t)ctas * 2 * part_floats(d, kMaxNB) * 4;
 }
 
 struct Args {
@@ -131,6 +131,15 @@ __device__ __forceinline__ void mma_f16_c(float (&d)[4], uint32_t a0, uint32_t a
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
+// a / b for a >= 0, b > 0: the 32-bit division, a quarter of the 64-bit one's
+// time, wherever it serves.
+__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+// The first unit of part i of n of a line of `total` units.
+__device__ __forceinline__ int64_t cut(int64_t i, int64_t each, int64_t more) {
+  return i * each + min(i, more);
+}
 // 2^(e - 127) for an exponent field e clamped to the normal range.
 __device__ __forceinline__ float pow2_field(int e) {
   return __int_as_float(max(1, min(254, e)) << 23);
@@ -158,6 +167,45 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// Joins partial results of one row (maximum, sum, unnormalised outputs of this
+// lane's V channels), in the order in which they are taken.
+template <int V>
+struct Merged {
+  float m = -INFINITY, l = 0.f, o[V] = {};
+  __device__ __forceinline__ void take(float pm, float pl, const float (&po)[V]) {
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(m - ref), pf = ex2(pm - ref);
+    m = top;
+    l = fmaf(l, f, pl * pf);
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], f, po[i] * pf);
+  }
+};
+template <int V>
+__device__ __forceinline__ void load_v(const float* p, float (&x)[V]) {
+  if constexpr (V == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x;
+    x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) {
+  if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(x[0] * f, x[1] * f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f);
+  }
+}
+
 // Work: a segment is 4 NB query rows (tokens x heads of one KV head) of one
 // sequence over all its tokens; its units are 32 tokens.  All units of all
 // segments lie on one line that is cut evenly among the warps of a grid that
@@ -173,9 +221,6 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
   constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // codes, and 16 times them
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[W][kStages];
-  __shared__ int64_t sh[33];
-  __shared__ int64_t s_start[W + 1];        // the warps' first units
-  __shared__ int64_t s_b[W], s_off[W];      // where on the line those are
   __shared__ SegInfo s_seg[W][2];           // kept pieces: at the warp's first unit, at its last
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -186,72 +231,103 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
   }
   griddep_wait();
 
-  // ---- the line of units, and where this CTA's warps begin on it
+  // ---- the line of units, and where this warp begins on it.  Every warp sums
+  // all sequences for itself, eight a lane: no barrier, one latency for 256.
   auto line_units = [&](int64_t b) -> int64_t {
     if (b >= a.n_seqs) return 0;
     const Seq s = seq_of(a, b);
     return (int64_t)seq_units(s.len) * seq_tiles<ROWS>(s.n, a.r) * a.hkv;
   };
-  int64_t total = 0;
-  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += W * 32) {
-    int64_t sum;
-    block_scan<int64_t>(line_units(b0 + tid), sh, &sum);
-    total += sum;
-  }
-  const int64_t ctas = max((int64_t)1, min((int64_t)gridDim.x, (total + W - 1) / W));
   const int64_t cta = blockIdx.x;
-  SegInfo* info = reinterpret_cast<SegInfo*>(a.ws + kWsHeadBytes);
-  float* parts = reinterpret_cast<float*>(a.ws + kWsHeadBytes + (size_t)gridDim.x * sizeof(SegInfo));
-  if (cta == 0 && tid == 0) {
-    WsHead* hd = reinterpret_cast<WsHead*>(a.ws);
-    hd->units = total;
-    hd->ctas = ctas;
+  SegInfo* info = reinterpret_cast<SegInfo*>(a.ws);
+  float* parts = reinterpret_cast<float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
+  int64_t mine[8], total = 0, upto = 0;     // of the last 256 sequences summed
+  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) {
+    int64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mine[i] = line_units(b0 + lane * 8 + i);
+      sum += mine[i];
+    }
+    upto = sum;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += v;
+    }
+    upto += total;
+    total = __shfl_sync(0xffffffffu, upto, 31);
   }
+  const int64_t ctas = max((int64_t)1, min((int64_t)gridDim.x, quot(total + W - 1, W)));
   if (cta >= ctas || total == 0) {
     if (tid == 0) info[cta].u0 = -1;
     return;
   }
-  const int64_t cta_a = cta * total / ctas, cta_b = (cta + 1) * total / ctas;
-  if (tid <= W) s_start[tid] = cta_a + tid * (cta_b - cta_a) / W;
-  if (tid < W * 2) s_seg[tid >> 1][tid & 1].u0 = -1;
-  __syncthreads();
-  for (int64_t b0 = 0, base = 0; b0 < a.n_seqs && base < cta_b; b0 += W * 32) {
-    const int64_t u = line_units(b0 + tid);
-    int64_t sum;
-    const int64_t end = base + block_scan<int64_t>(u, sh, &sum);
-    for (int w = 0; w < W; ++w)
-      if (s_start[w] >= end - u && s_start[w] < end) {
-        s_b[w] = b0 + tid;
-        s_off[w] = s_start[w] - (end - u);
+  const int64_t each = quot(total, ctas), more = total - each * ctas;
+  const int64_t cta_a = cut(cta, each, more), cta_b = cut(cta + 1, each, more);
+  const int64_t w_each = quot(cta_b - cta_a, W), w_more = cta_b - cta_a - w_each * W;
+  const int64_t w_a = cta_a + cut(warp, w_each, w_more), w_b = cta_a + cut(warp + 1, w_each, w_more);
+  if (lane < 2) s_seg[warp][lane].u0 = -1;
+  int64_t b = 0, off = 0;                   // the sequence of unit w_a, and the unit within it
+  for (int64_t b0 = a.n_seqs > 256 ? 0 : -1, base = 0; b0 < a.n_seqs; b0 += 256) {
+    if (b0 >= 0) {                          // more than 256 sequences: sum again up to w_a
+      int64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        mine[i] = line_units(b0 + lane * 8 + i);
+        sum += mine[i];
       }
-    base += sum;
+      upto = sum;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += v;
+      }
+      upto += base;
+      base = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, upto > w_a);
+    if (!past) continue;
+    const int who = __ffs(past) - 1;
+    int64_t from = upto;
+    int at = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {          // the last of this lane's that begins at or before w_a
+      const int64_t end = from;
+      from -= mine[i];
+      if (from <= w_a && w_a < end) {
+        at = i;
+        off = w_a - from;
+      }
+    }
+    b = __shfl_sync(0xffffffffu, max(b0, (int64_t)0) + lane * 8 + at, who);
+    off = __shfl_sync(0xffffffffu, off, who);
+    break;
   }
-  __syncthreads();
-  if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if it is the first cut
-    const int64_t b = s_b[0], off = s_off[0];
+  if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
     const Seq s = seq_of(a, b);
     const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
-    const int64_t seg = off / nu;
+    const int64_t seg = quot(off, nu);
     SegInfo si;
     si.u0 = cta_a - (off - seg * nu);
     si.u1 = si.u0 + nu;
     si.b = (int32_t)b;
-    si.kvh = (int32_t)(seg / tiles);
-    si.tile = (int32_t)(seg % tiles);
+    si.kvh = (int32_t)quot(seg, tiles);
+    si.tile = (int32_t)(seg - (int64_t)si.kvh * tiles);
+    const int64_t before = cut(cta - 1, each, more);
+    int64_t last = cta;                     // the CTA that holds its last unit
+    if (each > 0) last = max(cta, quot(si.u1 - 1, each + 1));
+    while (last + 1 < ctas && cut(last + 1, each, more) < si.u1) ++last;
+    si.parts = (int32_t)(last - (cta - 1) + 1);
+    si.second = si.u0 > before;
     si.pad = 0;
-    if (si.u0 == cta_a || si.u0 < (cta - 1) * total / ctas) si.u0 = -1;
+    if (si.u0 == cta_a || si.u0 < before) si.u0 = -1;
     info[cta] = si;
   }
 
-  const int64_t w_a = s_start[warp], w_b = s_start[warp + 1];
   uint8_t* ring = smem + (size_t)warp * kStages * 2 * TB;
   float* kept = reinterpret_cast<float*>(smem + (size_t)W * kStages * 2 * TB) + warp * PF;
   uint32_t phase = 0;                       // parity of each stage's next use
-  int64_t b = 0, off = 0;
-  if (w_a < w_b) {
-    b = s_b[warp];
-    off = s_off[warp];
-  }
   for (int64_t at = w_a; at < w_b;) {
     const Seq s = seq_of(a, b);
     const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
@@ -260,16 +336,16 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
       ++b;
       continue;
     }
-    const int64_t seg = off / nu;
+    const int64_t seg = quot(off, nu);
     const int u_first = (int)(off - seg * nu);
     const int u_count = (int)min((int64_t)(nu - u_first), w_b - at);
-    const int kvh = (int)(seg / tiles), tile = (int)(seg - (int64_t)kvh * tiles);
+    const int kvh = (int)quot(seg, tiles), tile = (int)(seg - (int64_t)kvh * tiles);
 
     // Rows of the tile: lane column g of B is row g / 2 (integer part, then
     // rest); scores, softmax and outputs of row c are with the lanes c.
     auto row_at = [&](int i, int& tok, int& hq) -> bool {
       const int rr = tile * ROWS + i;
-      tok = rr / a.r;
+      tok = a.r == 1 ? rr : (int)((uint32_t)rr / (uint32_t)a.r);
       hq = kvh * a.r + rr - tok * a.r;
       return rr < s.n * a.r;
     };
@@ -277,6 +353,25 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     const int seg_len = max(0, min(s.len, s.len - s.n + last_tok + 1));  // no row sees further
     const int all_see = s.len - s.n + tile * ROWS / a.r + 1;             // every row sees these
     const int u_live = min(u_first + u_count, (seg_len + kUnit - 1) / kUnit);
+
+    // this lane's part of the query rows, on its way while the tiles are found
+    float x[NB][NC][8];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      int tok, hq;
+      const bool ok = row_at(nb * 4 + (g >> 1), tok, hq);
+      const float* qr = a.q + ((s.row0 + tok) * a.h + hq) * D + 8 * c;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+        if (ok) {
+          v0 = *reinterpret_cast<const float4*>(qr + 32 * j);
+          v1 = *reinterpret_cast<const float4*>(qr + 32 * j + 4);
+        }
+        x[nb][j][0] = v0.x; x[nb][j][1] = v0.y; x[nb][j][2] = v0.z; x[nb][j][3] = v0.w;
+        x[nb][j][4] = v1.x; x[nb][j][5] = v1.y; x[nb][j][6] = v1.z; x[nb][j][7] = v1.w;
+      }
+    }
 
     // Tiles are fetched by the lanes that know where they are: lane i has the
     // place of tile 2 ids_at + i.
@@ -286,13 +381,12 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     auto issue = [&](int u, int stage) -> uint32_t {
       if (u - ids_at >= 16) {
         ids_at = u;
-        const int64_t tt = 2 * (int64_t)u + lane;
-        const bool in = tt * kTile < seg_len;
-        const int64_t page = in ? tt * kTile / a.bs : 0;
+        const uint32_t tt = 2 * (uint32_t)u + lane, per = (uint32_t)a.bs / kTile;
+        const bool in = tt < (uint32_t)(seg_len + kTile - 1) / kTile;
+        const uint32_t page = in ? tt / per : 0;
         const int blk = in ? a.table[b * a.width + page] : -1;
         const bool ok = blk >= 0 && blk < a.n_blocks;
         if (in && !ok && a.err) atomicExch(a.err, 4);  // never read: its tokens are left out
-        const int per = a.bs / kTile;
         src = a.cache + (((int64_t)blk * a.hkv + kvh) * per + (tt - page * per)) * TB;
         known = __ballot_sync(0xffffffffu, ok);
       }
@@ -313,25 +407,14 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     float qsum[NB][NG], qc[NB][NG][2], row_f[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      int tok, hq;
-      const bool ok = row_at(nb * 4 + (g >> 1), tok, hq);
-      const float* qr = a.q + ((s.row0 + tok) * a.h + hq) * D;
-      float x[NC][8], amax = 0.f;
+      float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-        if (ok) {
-          v0 = *reinterpret_cast<const float4*>(qr + 32 * j + 8 * c);
-          v1 = *reinterpret_cast<const float4*>(qr + 32 * j + 8 * c + 4);
-        }
-        x[j][0] = v0.x; x[j][1] = v0.y; x[j][2] = v0.z; x[j][3] = v0.w;
-        x[j][4] = v1.x; x[j][5] = v1.y; x[j][6] = v1.z; x[j][7] = v1.w;
+      for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[j][i] *= a.scale2;
-          amax = fmaxf(amax, fabsf(x[j][i]));
+          x[nb][j][i] *= a.scale2;
+          amax = fmaxf(amax, fabsf(x[nb][j][i]));
         }
-      }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // the largest magnitude goes to [2^10, 2^11)
@@ -345,8 +428,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          sum[j * 32 / G] += x[j][i];
-          const float v = x[j][i] * up, hi = rintf(v);
+          sum[j * 32 / G] += x[nb][j][i];
+          const float v = x[nb][j][i] * up, hi = rintf(v);
           y[i] = g & 1 ? v - hi : hi;
           if (i & 1) y[i] *= 0.0625f;       // odd nibbles count 16 times
         }
@@ -626,123 +709,108 @@ __global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kerne
     off += u_count;
   }
 
-  // ---- pieces of one segment in neighbouring warps
+  // ---- pieces of one segment in neighbouring warps, a row a warp
   __syncthreads();
+  constexpr int V = D / 32;
   auto piece_at = [&](int i) -> const float* {
     return i & 1 ? reinterpret_cast<const float*>(smem + (size_t)(i >> 1) * kStages * 2 * TB)
                  : reinterpret_cast<const float*>(smem + (size_t)W * kStages * 2 * TB) + (i >> 1) * PF;
   };
-  for (int i = 0; i < 2 * W;) {
-    const SegInfo si = s_seg[i >> 1][i & 1];
-    if (si.u0 < 0) {
-      ++i;
-      continue;
-    }
-    int end = i + 1;
-    while (end < 2 * W && (s_seg[end >> 1][end & 1].u0 < 0 || s_seg[end >> 1][end & 1].u0 == si.u0)) ++end;
-    const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
+  // which of the 2 W places hold a piece, and which begin another segment
+  const int64_t my_u0 = lane < 2 * W ? s_seg[lane >> 1][lane & 1].u0 : -1;
+  const unsigned used = __ballot_sync(0xffffffffu, my_u0 >= 0);
+  const int prev = 31 - __clz(used & ((1u << lane) - 1u));
+  const int64_t prev_u0 = __shfl_sync(0xffffffffu, my_u0, max(prev, 0));
+  const unsigned first = __ballot_sync(0xffffffffu, my_u0 >= 0 && (prev < 0 || prev_u0 != my_u0));
+  int task = 0;
+  for (unsigned todo = first; todo; todo &= todo - 1) {
+    const int i0 = __ffs(todo) - 1;
+    const unsigned later = todo & (todo - 1);
+    const unsigned members = used & ~((1u << i0) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : ~0u);
+    const SegInfo si = s_seg[i0 >> 1][i0 & 1];
     const Seq s = seq_of(a, si.b);
+    const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
     float* slot = parts + (size_t)(2 * cta + (si.u0 <= cta_a ? 0 : 1)) * PF;
-    for (int x = tid; x < ROWS * D; x += W * 32) {
-      const int row = x / D, d = x - row * D;
-      float M = -INFINITY;
-      for (int j = i; j < end; ++j)
-        if (s_seg[j >> 1][j & 1].u0 >= 0) M = fmaxf(M, piece_at(j)[ROWS * D + row]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc = 0.f;
-      for (int j = i; j < end; ++j)
-        if (s_seg[j >> 1][j & 1].u0 >= 0) {
-          const float* p = piece_at(j);
-          const float f = ex2(p[ROWS * D + row] - ref);
-          L = fmaf(f, p[ROWS * D + ROWS + row], L);
-          acc = fmaf(f, p[x], acc);
-        }
+    const int rows = min(ROWS, s.n * a.r - si.tile * ROWS);
+    for (int row = 0; row < rows; ++row, ++task) {
+      if (task % W != warp) continue;
+      Merged<V> all;
+      for (unsigned rest = members; rest; rest &= rest - 1) {
+        const float* p = piece_at(__ffs(rest) - 1);
+        float po[V];
+        load_v<V>(p + row * D + lane * V, po);
+        all.take(p[ROWS * D + row], p[ROWS * D + ROWS + row], po);
+      }
       if (whole) {
-        const int rr = si.tile * ROWS + row;
-        if (rr < s.n * a.r) {
-          const int tok = rr / a.r, hq = si.kvh * a.r + rr - tok * a.r;
-          a.out[((s.row0 + tok) * a.h + hq) * D + d] = L == 0.f ? 0.f : acc / L;
-        }
+        const int rr = si.tile * ROWS + row, tok = (int)((uint32_t)rr / (uint32_t)a.r);
+        const int hq = si.kvh * a.r + rr - tok * a.r;
+        store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
       } else {
-        slot[x] = acc;
-        if (d == 0) {
-          slot[ROWS * D + row] = M;
-          slot[ROWS * D + ROWS + row] = L;
+        store_v<V>(slot + row * D + lane * V, all.o, 1.f);
+        if (lane == 0) {
+          slot[ROWS * D + row] = all.m;
+          slot[ROWS * D + ROWS + row] = all.l;
         }
       }
     }
-    i = end;
   }
 }
 
-// Joins the segments that several CTAs share.  Block (i, row): the segment
-// that CTA i's beginning cuts, if that is the segment's first cut.  Its parts
-// are taken in the order of the CTAs, so the result does not depend on timing.
-constexpr int kJoinThreads = 256;
+// Joins the segments that several CTAs share.  Block i: the segment that CTA
+// i's beginning cuts, if that is the segment's first cut.  Its rows are shared
+// by the warps, several warps a row where there are few; every result is taken
+// in a fixed order, so it does not depend on timing.
+constexpr int kJoinWarps = 16;
 template <int D, int NB>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
-  constexpr int PF = part_floats(D, NB), ROWS = rows_of(NB), GR = kJoinThreads / D;
-  extern __shared__ __align__(16) float wgt[];  // one weight per part
-  __shared__ float red[kJoinThreads];
-  __shared__ float s_m[32], s_l[32];
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
+  constexpr int PF = part_floats(D, NB), ROWS = rows_of(NB), V = D / 32;
+  __shared__ __align__(16) float s_o[kJoinWarps][D];
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = threadIdx.x, row = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t cta = blockIdx.x;
-  const SegInfo* info = reinterpret_cast<const SegInfo*>(a.ws + kWsHeadBytes);
-  const float* parts = reinterpret_cast<const float*>(a.ws + kWsHeadBytes + (size_t)gridDim.x * sizeof(SegInfo));
-  const SegInfo si = info[cta];
+  const SegInfo si = reinterpret_cast<const SegInfo*>(a.ws)[cta];
+  const float* parts = reinterpret_cast<const float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
   if (si.u0 < 0) return;
   const Seq s = seq_of(a, si.b);
-  const int rr = si.tile * ROWS + row;
-  if (rr >= s.n * a.r) return;
-  const WsHead hd = *reinterpret_cast<const WsHead*>(a.ws);
-  // the segment's parts: CTA cta - 1, then cta .. up to the one that holds its end
-  const int64_t last = (si.u1 - 1) * hd.ctas / hd.units;  // a first guess, put right below
-  int64_t hi = last;
-  while (hi + 1 < hd.ctas && (hi + 1) * hd.units / hd.ctas < si.u1) ++hi;
-  while (hi * hd.units / hd.ctas >= si.u1) --hi;
-  const int n = (int)(hi - (cta - 1) + 1);
-  auto part = [&](int j) -> const float* {
-    const int64_t x = cta - 1 + j;
-    const bool second = j == 0 && si.u0 > x * hd.units / hd.ctas;
-    return parts + (size_t)(2 * x + (second ? 1 : 0)) * PF;
-  };
-  float M = -INFINITY;
-  for (int j = tid; j < n; j += kJoinThreads) M = fmaxf(M, part(j)[ROWS * D + row]);
+  const int rows = min(ROWS, s.n * a.r - si.tile * ROWS);
+  const int groups = rows == 1 ? kJoinWarps : rows == 2 ? kJoinWarps / 2 : kJoinWarps / (rows <= 4 ? 4 : 8);
+  const int row = warp / groups, grp = warp - row * groups;
+  Merged<V> all;
+  if (row < rows) {
+    // the first part lies in CTA cta - 1, the others at the beginning of theirs
+    auto part = [&](int j) { return parts + (size_t)(2 * (cta - 1 + j) + (j == 0 ? si.second : 0)) * PF; };
+    for (int j0 = grp; j0 < si.parts; j0 += 4 * groups) {
+      float pm[4], pl[4], po[4][V];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if ((tid & 31) == 0) s_m[tid >> 5] = M;
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + i * groups;
+        const float* p = part(min(j, si.parts - 1));
+        pm[i] = j < si.parts ? p[ROWS * D + row] : -INFINITY;
+        pl[i] = j < si.parts ? p[ROWS * D + ROWS + row] : 0.f;
+        load_v<V>(p + row * D + lane * V, po[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j0 + i * groups < si.parts) all.take(pm[i], pl[i], po[i]);
+    }
+    store_v<V>(&s_o[warp][lane * V], all.o, 1.f);
+    if (lane == 0) {
+      s_m[warp] = all.m;
+      s_l[warp] = all.l;
+    }
+  }
   __syncthreads();
-  M = s_m[0];
-  for (int i = 1; i < kJoinThreads / 32; ++i) M = fmaxf(M, s_m[i]);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  for (int j = tid; j < n; j += kJoinThreads) {
-    const float* p = part(j);
-    const float f = ex2(p[ROWS * D + row] - ref);
-    wgt[j] = f;
-    L = fmaf(f, p[ROWS * D + ROWS + row], L);
+  if (row >= rows || grp != 0) return;
+  for (int i = 1; i < min(groups, si.parts); ++i) {
+    float po[V];
+    load_v<V>(&s_o[warp + i][lane * V], po);
+    all.take(s_m[warp + i], s_l[warp + i], po);
   }
-  L = warp_sum(L);
-  if ((tid & 31) == 0) s_l[tid >> 5] = L;
-  __syncthreads();
-  L = 0.f;
-  for (int i = 0; i < kJoinThreads / 32; ++i) L += s_l[i];
-  const int d = tid % D, gr = tid / D;
-  float acc = 0.f;
-#pragma unroll 4
-  for (int j = gr; j < n; j += GR) acc = fmaf(wgt[j], part(j)[row * D + d], acc);
-  if (GR > 1) {
-    red[tid] = acc;
-    __syncthreads();
-    if (gr == 0)
-      for (int i = 1; i < GR; ++i) acc += red[i * D + d];
-  }
-  if (gr == 0) {
-    const int tok = rr / a.r, hq = si.kvh * a.r + rr - tok * a.r;
-    a.out[((s.row0 + tok) * a.h + hq) * D + d] = L == 0.f ? 0.f : acc / L;
-  }
+  const int rr = si.tile * ROWS + row, tok = (int)((uint32_t)rr / (uint32_t)a.r);
+  const int hq = si.kvh * a.r + rr - tok * a.r;
+  store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
 }
 
 int grid_of(int d) {
@@ -756,7 +824,7 @@ int run_nb(const Args& a, cudaStream_t st) {
   NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
   const int ctas = grid_of(D);
   NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
-  return launch(join_kernel<D, NB>, dim3(ctas, rows_of(NB)), kJoinThreads, (size_t)ctas * 4, st, 1, a);
+  return launch(join_kernel<D, NB>, dim3(ctas), kJoinWarps * 32, 0, st, 1, a);
 }
 
 // 4 rows a segment where no sequence should have more of them for a KV head:
