@@ -47,9 +47,11 @@ struct SegInfo {
 
 // A segment's query rows: 4 per column tile of the MMA's B operand.
 __host__ __device__ constexpr int rows_of(int nb) { return 4 * nb; }
-constexpr int kMaxNB = 2;
+constexpr int kMaxNB = 4;
 __host__ __device__ constexpr int part_floats(int d, int nb) { return rows_of(nb) * (d + 2); }
 
+// CTAs of an SM: two where 128 registers a thread hold a segment's state.
+__host__ __device__ constexpr int ctas_per_sm(int d, int nb) { return d <= 128 && nb == 1 ? 2 : 1; }
 // Rings, then one kept piece per warp.
 constexpr int attn_smem(int d, int ng, int nb) {
   return warps_of(d) * (kStages * 2 * tile_bytes(d, ng) + part_floats(d, nb) * 4);
@@ -215,7 +217,7 @@ __device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) 
 //
 // Each warp streams its tiles with bulk copies into its own two-stage ring.
 template <int D, int NG, int NB>
-__global__ void __launch_bounds__(warps_of(D) * 32, D <= 128 ? 2 : 1) attn_kernel(const Args a) {
+__global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_kernel(const Args a) {
   constexpr int NC = D / 32, NS = D / 64, G = D / NG, W = warps_of(D);
   constexpr int TB = tile_bytes(D, NG), PF = part_floats(D, NB), ROWS = rows_of(NB);
   constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // codes, and 16 times them
@@ -775,7 +777,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
   if (si.u0 < 0) return;
   const Seq s = seq_of(a, si.b);
   const int rows = min(ROWS, s.n * a.r - si.tile * ROWS);
-  const int groups = rows == 1 ? kJoinWarps : rows == 2 ? kJoinWarps / 2 : kJoinWarps / (rows <= 4 ? 4 : 8);
+  const int groups = rows == 1 ? kJoinWarps : rows == 2 ? kJoinWarps / 2 : kJoinWarps / (rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
   const int row = warp / groups, grp = warp - row * groups;
   Merged<V> all;
   if (row < rows) {
@@ -813,25 +815,30 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
   store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
 }
 
-int grid_of(int d) {
+int grid_of(int d, int nb) {
   Context* c = ctx();
-  return (c ? c->num_sms : 148) * (d <= 128 ? 2 : 1);
+  return (c ? c->num_sms : 148) * ctas_per_sm(d, nb);
 }
 
 template <int D, int NG, int NB>
 int run_nb(const Args& a, cudaStream_t st) {
   const int smem = attn_smem(D, NG, NB);
   NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
-  const int ctas = grid_of(D);
+  const int ctas = grid_of(D, NB);
   NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
   return launch(join_kernel<D, NB>, dim3(ctas), kJoinWarps * 32, 0, st, 1, a);
 }
 
-// 4 rows a segment where no sequence should have more of them for a KV head:
-// half the tensor work, registers and partial results of 8.
+// 4 rows a segment where no sequence should have more of them for a KV head,
+// 8 or 16 where one may: each pass over a sequence's tiles serves more rows,
+// at more registers and partial results.
 template <int D, int NG>
 int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
-  return max_new * a.r <= 4 ? run_nb<D, NG, 1>(a, st) : run_nb<D, NG, 2>(a, st);
+  const int64_t rows = max_new * a.r;
+  if (rows <= 4) return run_nb<D, NG, 1>(a, st);
+  if constexpr (D <= 128)
+    if (rows > 8) return run_nb<D, NG, 4>(a, st);
+  return run_nb<D, NG, 2>(a, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -853,7 +860,7 @@ int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int
                      (long long)n_heads, s.hkv);
   if (!bytes) return set_error(NIMF_ERR_ARG, "kv4_attention_workspace: NULL result");
   NIMF_TRY(require_ctx(&c));
-  *bytes = (int64_t)kv4::ws_bytes(kv4::grid_of(s.d), s.d);
+  *bytes = (int64_t)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d);
   return NIMF_OK;
 }
 
@@ -878,9 +885,9 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   if (!kv4::aligned16(cache) || !kv4::aligned16(q) || !kv4::aligned16(out) || !kv4::aligned16(workspace))
     return set_error(NIMF_ERR_ARG, "kv4_attention: buffers must be 16-byte aligned");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  if (workspace_bytes < (int64_t)kv4::ws_bytes(kv4::grid_of(s.d), s.d))
+  if (workspace_bytes < (int64_t)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d))
     return set_error(NIMF_ERR_ARG, "kv4_attention: %lld bytes of workspace, nimf_kv4_attention_workspace asks for %lld",
-                     (long long)workspace_bytes, (long long)kv4::ws_bytes(kv4::grid_of(s.d), s.d));
+                     (long long)workspace_bytes, (long long)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d));
   kv4::Args a = {};
   a.cache = (const uint8_t*)cache;
   a.q = q;
