@@ -127,5 +127,108 @@ __device__ __forceinline__ T block_scan(T v, T* sh, T* total) {
   return v;
 }
 
+// ------------------------------------------------------------------ attention
+// What attention's kernels are given.
+struct Args {
+  const uint8_t* cache;
+  const float* q;
+  const int32_t* cu_rows;     // NULL: one row per sequence
+  const int32_t* lens;
+  const int32_t* table;
+  float* out;
+  unsigned char* ws;
+  int* err;
+  int64_t n_seqs, rows, width, n_blocks;
+  int h, hkv, r, bs;
+  float scale2;               // softmax scale * log2(e)
+  int big;                    // sequences with more rows a KV head than this go to kv4_tc.cu
+};
+
+// Sequence b as the kernels see it: its rows [row0, row0 + n) and its cached
+// tokens, both held inside the caller's buffers.
+struct Seq {
+  int64_t row0;
+  int n, len;
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int64_t b) {
+  Seq s;
+  int64_t e;
+  if (a.cu_rows) {
+    s.row0 = min((int64_t)max(a.cu_rows[b], 0), a.rows);
+    e = min((int64_t)max(a.cu_rows[b + 1], 0), a.rows);
+  } else {
+    s.row0 = min(b, a.rows);
+    e = min(b + 1, a.rows);
+  }
+  s.n = (int)max(e - s.row0, (int64_t)0);
+  s.len = (int)min((int64_t)max(a.lens[b], 0), a.width * a.bs);
+  return s;
+}
+// a / b for a >= 0, b > 0: the 32-bit division, a quarter of the 64-bit one's
+// time, wherever it serves.
+__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+// 2^(e - 127) for an exponent field e clamped to the normal range.
+__device__ __forceinline__ float pow2_field(int e) {
+  return __int_as_float(max(1, min(254, e)) << 23);
+}
+__device__ __forceinline__ int exp_field(float x) { return (__float_as_int(x) >> 23) & 255; }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+  return d;
+}
+// Joins partial results of one row (maximum, sum, unnormalised outputs of this
+// lane's V channels), in the order in which they are taken.
+template <int V>
+struct Merged {
+  float m = -INFINITY, l = 0.f, o[V] = {};
+  __device__ __forceinline__ void take(float pm, float pl, const float (&po)[V]) {
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(m - ref), pf = ex2(pm - ref);
+    m = top;
+    l = fmaf(l, f, pl * pf);
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], f, po[i] * pf);
+  }
+};
+template <int V>
+__device__ __forceinline__ void load_v(const float* p, float (&x)[V]) {
+  if constexpr (V == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x;
+    x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) {
+  if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(x[0] * f, x[1] * f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f);
+  }
+}
+
+// Attention of sequences with more than a.big rows a KV head, on tcgen05
+// (kv4_tc.cu): head dims and groups served, workspace, launch.
+bool tc_serves(int d);
+size_t tc_ws_bytes(int d);
+int run_tc(const Args& a, int d, int ng, int64_t max_blocks, unsigned char* ws, cudaStream_t st);
+
 }  // namespace kv4
 }  // namespace nimf

@@ -61,56 +61,12 @@ size_t ws_bytes(int ctas, int d) {
   return (size_t)ctas * sizeof(SegInfo) + (size_t)ctas * 2 * part_floats(d, kMaxNB) * 4;
 }
 
-struct Args {
-  const uint8_t* cache;
-  const float* q;
-  const int32_t* cu_rows;     // NULL: one row per sequence
-  const int32_t* lens;
-  const int32_t* table;
-  float* out;
-  unsigned char* ws;
-  int* err;
-  int64_t n_seqs, rows, width, n_blocks;
-  int h, hkv, r, bs;
-  float scale2;               // softmax scale * log2(e)
-};
-
-// Sequence b as the kernels see it: its rows [row0, row0 + n) and its cached
-// tokens, both held inside the caller's buffers.
-struct Seq {
-  int64_t row0;
-  int n, len;
-};
-__device__ __forceinline__ Seq seq_of(const Args& a, int64_t b) {
-  Seq s;
-  int64_t e;
-  if (a.cu_rows) {
-    s.row0 = min((int64_t)max(a.cu_rows[b], 0), a.rows);
-    e = min((int64_t)max(a.cu_rows[b + 1], 0), a.rows);
-  } else {
-    s.row0 = min(b, a.rows);
-    e = min(b + 1, a.rows);
-  }
-  s.n = (int)max(e - s.row0, (int64_t)0);
-  s.len = (int)min((int64_t)max(a.lens[b], 0), a.width * a.bs);
-  return s;
-}
 __device__ __forceinline__ int seq_units(int len) { return max(1, (len + kUnit - 1) / kUnit); }
 template <int ROWS>
 __device__ __forceinline__ int seq_tiles(int n, int r) {
   return (int)(((int64_t)n * r + ROWS - 1) / ROWS);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-  return d;
-}
 // An integer up to 2^11 (nearest, halves to even) and the rest of x.
 __device__ __forceinline__ float int_part(float x) { return __fadd_rn(__fadd_rn(x, 12582912.f), -12582912.f); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -133,21 +89,10 @@ __device__ __forceinline__ void mma_f16_c(float (&d)[4], uint32_t a0, uint32_t a
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-// a / b for a >= 0, b > 0: the 32-bit division, a quarter of the 64-bit one's
-// time, wherever it serves.
-__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
-  return ((uint64_t)(a | b) >> 32) ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
 // The first unit of part i of n of a line of `total` units.
 __device__ __forceinline__ int64_t cut(int64_t i, int64_t each, int64_t more) {
   return i * each + min(i, more);
 }
-// 2^(e - 127) for an exponent field e clamped to the normal range.
-__device__ __forceinline__ float pow2_field(int e) {
-  return __int_as_float(max(1, min(254, e)) << 23);
-}
-__device__ __forceinline__ int exp_field(float x) { return (__float_as_int(x) >> 23) & 255; }
-
 // N consecutive words of shared memory.
 template <int N>
 __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
@@ -166,45 +111,6 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
       w[4 * i + 2] = v.z;
       w[4 * i + 3] = v.w;
     }
-  }
-}
-
-// Joins partial results of one row (maximum, sum, unnormalised outputs of this
-// lane's V channels), in the order in which they are taken.
-template <int V>
-struct Merged {
-  float m = -INFINITY, l = 0.f, o[V] = {};
-  __device__ __forceinline__ void take(float pm, float pl, const float (&po)[V]) {
-    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
-    const float f = ex2(m - ref), pf = ex2(pm - ref);
-    m = top;
-    l = fmaf(l, f, pl * pf);
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], f, po[i] * pf);
-  }
-};
-template <int V>
-__device__ __forceinline__ void load_v(const float* p, float (&x)[V]) {
-  if constexpr (V == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x;
-    x[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
-    }
-  }
-}
-template <int V>
-__device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) {
-  if constexpr (V == 2) {
-    *reinterpret_cast<float2*>(p) = make_float2(x[0] * f, x[1] * f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-      reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f);
   }
 }
 
@@ -235,10 +141,11 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
 
   // ---- the line of units, and where this warp begins on it.  Every warp sums
   // all sequences for itself, eight a lane: no barrier, one latency for 256.
+  auto tiles_of = [&](int n) { return n * a.r > a.big ? 0 : seq_tiles<ROWS>(n, a.r); };
   auto line_units = [&](int64_t b) -> int64_t {
     if (b >= a.n_seqs) return 0;
     const Seq s = seq_of(a, b);
-    return (int64_t)seq_units(s.len) * seq_tiles<ROWS>(s.n, a.r) * a.hkv;
+    return (int64_t)seq_units(s.len) * tiles_of(s.n) * a.hkv;
   };
   const int64_t cta = blockIdx.x;
   SegInfo* info = reinterpret_cast<SegInfo*>(a.ws);
@@ -308,7 +215,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
   }
   if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
     const Seq s = seq_of(a, b);
-    const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
+    const int tiles = tiles_of(s.n), nu = seq_units(s.len);
     const int64_t seg = quot(off, nu);
     SegInfo si;
     si.u0 = cta_a - (off - seg * nu);
@@ -332,7 +239,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
   uint32_t phase = 0;                       // parity of each stage's next use
   for (int64_t at = w_a; at < w_b;) {
     const Seq s = seq_of(a, b);
-    const int tiles = seq_tiles<ROWS>(s.n, a.r), nu = seq_units(s.len);
+    const int tiles = tiles_of(s.n), nu = seq_units(s.len);
     if (off >= (int64_t)nu * tiles * a.hkv) {  // the next sequence
       off = 0;
       ++b;
@@ -485,7 +392,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
     const int tg = g ^ ((g >> 1) & 1);
     bool failed = false;
     for (int u = u_first, st = 0; u < u_live; ++u, st ^= 1) {
-      if (!mbar_wait(&full[warp][st], (phase >> st) & 1u)) {
+      if (!mbar_wait_t<0>(&full[warp][st], (phase >> st) & 1u)) {
         if (a.err) atomicExch(a.err, 6);
         failed = true;
         break;
@@ -661,7 +568,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
         there = (there & ~(3u << (2 * st))) | issue(u + kStages, st) << (2 * st);
     }
     if (failed) {  // the copies still in flight, then out; the answer is not valid
-      for (int st = 0; st < kStages; ++st) (void)mbar_wait(&full[warp][st], (phase >> st) & 1u);
+      for (int st = 0; st < kStages; ++st) (void)mbar_wait_t<0>(&full[warp][st], (phase >> st) & 1u);
       break;
     }
 
@@ -834,12 +741,20 @@ int run_nb(const Args& a, cudaStream_t st) {
 // at more registers and partial results.
 template <int D, int NG>
 int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
-  const int64_t rows = max_new * a.r;
+  const int64_t rows = std::min<int64_t>(max_new * a.r, a.big);
   if (rows <= 4) return run_nb<D, NG, 1>(a, st);
   if constexpr (D <= 128)
     if (rows > 8) return run_nb<D, NG, 4>(a, st);
   return run_nb<D, NG, 2>(a, st);
 }
+
+size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 1), d) + 255) / 256 * 256; }
+size_t all_ws_bytes(int d) { return few_ws_bytes(d) + (tc_serves(d) ? tc_ws_bytes(d) : 0); }
+
+// Rows a KV head from which a sequence is worth the tensor-core kernel's tiles
+// of 128: such a tile costs about what 16 rows cost here (1.1 against 1.2 us
+// for 128 tokens of a 128-channel head).
+constexpr int kBigRows = 16;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -860,7 +775,7 @@ int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int
                      (long long)n_heads, s.hkv);
   if (!bytes) return set_error(NIMF_ERR_ARG, "kv4_attention_workspace: NULL result");
   NIMF_TRY(require_ctx(&c));
-  *bytes = (int64_t)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d);
+  *bytes = (int64_t)kv4::all_ws_bytes(s.d);
   return NIMF_OK;
 }
 
@@ -885,9 +800,9 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   if (!kv4::aligned16(cache) || !kv4::aligned16(q) || !kv4::aligned16(out) || !kv4::aligned16(workspace))
     return set_error(NIMF_ERR_ARG, "kv4_attention: buffers must be 16-byte aligned");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  if (workspace_bytes < (int64_t)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d))
+  if (workspace_bytes < (int64_t)kv4::all_ws_bytes(s.d))
     return set_error(NIMF_ERR_ARG, "kv4_attention: %lld bytes of workspace, nimf_kv4_attention_workspace asks for %lld",
-                     (long long)workspace_bytes, (long long)kv4::ws_bytes(kv4::grid_of(s.d, 1), s.d));
+                     (long long)workspace_bytes, (long long)kv4::all_ws_bytes(s.d));
   kv4::Args a = {};
   a.cache = (const uint8_t*)cache;
   a.q = q;
@@ -906,6 +821,11 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   a.r = (int)(n_heads / s.hkv);
   a.bs = s.bs;
   a.scale2 = (float)((double)scale * 1.4426950408889634);
+  a.big = INT32_MAX;
+  if (kv4::tc_serves(s.d) && max_new * a.r > kv4::kBigRows) {
+    a.big = kv4::kBigRows;
+    NIMF_TRY(kv4::run_tc(a, s.d, s.d / s.group, max_blocks, a.ws + kv4::few_ws_bytes(s.d), st));
+  }
   switch (s.d * 16 + s.d / s.group) {
     case 64 * 16 + 1: return kv4::run_attn<64, 1>(a, max_new, st);
     case 64 * 16 + 2: return kv4::run_attn<64, 2>(a, max_new, st);

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   int above = 0;
   bool ok = true;
   for (int i = 0; i < kLpChunks; ++i) {
-    ok = ok && mbar_wait(&bar[i], 0);
+    ok = ok && mbar_wait_t<0>(&bar[i], 0);
     const int f1 = min(nf, (i + 1) * per);
     for (int f = i * per + tid; f < f1; f += kLpThreads) {
       const float4 v = b4[f];
