@@ -12,13 +12,16 @@
 // run in TMEM over one tile of tokens only and are added to float32 registers
 // between, so that the tensor core's cut-off additions stay few.
 //
-// Roles: two softmax warpgroups take turns at the tiles (even and odd ones),
-// each with its own S and O columns, running maximum and sums, joined at the
-// end, so the tensor core works on one tile while the other is in softmax; one
-// warpgroup unpacks codes into the K and V operands (two buffers each); one
-// warp issues the MMAs.  P overwrites S in place: 32 columns of scores become
-// 16 columns of high and 16 of low terms.
+// Roles: eight softmax warps, a warp 32 rows x half of a tile's tokens; four warps
+// unpack codes into the K and V operands (two buffers each); one warp issues the
+// MMAs.  S and O have two buffers too: while tile t is in softmax the tensor core
+// multiplies the values of tile t - 1 and the keys of tile t + 1.  P overwrites
+// S in place: 16 columns of scores become 8 of high and 8 of low terms.
+// Softmax reads TMEM in the MMA fragment shape (a lane 4 rows x every fourth pair
+// of columns): scales and minima are per column, and a lane with whole rows loads
+// four times as many of them, which alone took longer than the products.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "tc_util.cuh"
@@ -29,7 +32,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 512;     // 2 softmax warpgroups, unpack, MMA
+constexpr int kTcThreads = 512;     // 8 softmax warps, 4 of unpack, 1 of MMA issue
 constexpr int kUnpack0 = 256;       // first unpack thread
 constexpr int kPrmSlots = 4;        // tiles whose scales and minima are held
 constexpr int kFails = 6;           // error word of an expired wait
@@ -41,10 +44,12 @@ struct TcLayout {
   static constexpr int Q = 0;                                   // [2 terms][128][D] fp16
   static constexpr int K = Q + 2 * kTcRows * D * 2;             // [2 buffers][N][D]
   static constexpr int V = K + 2 * N * D * 2;                   // [2 buffers][D][N]
-  static constexpr int PRM = V + 2 * N * D * 2;                 // [slots][ks, km, vs, vm][128] float
+  static constexpr int PRM = V + 2 * N * D * 2;                 // [slots][K, V][64] {s, s, m, m}
   static constexpr int F = PRM + kPrmSlots * 4 * 128 * 4;       // [slots][NG] float
   static constexpr int RED = F + kPrmSlots * 4 * 4;             // [2][4] uint32
-  static constexpr int BAR = RED + 32;                          // barriers
+  static constexpr int ROW = RED + 32;                          // [1 + NG][128]: row_f, sums of q
+  static constexpr int MAX = ROW + (1 + NG) * 128 * 4;          // [2][2][128]: maxima of the halves
+  static constexpr int BAR = MAX + 4 * 128 * 4;                 // barriers
   static constexpr int SIZE = BAR + 256;
 };
 
@@ -60,18 +65,45 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uin
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
 }
-// 32 consecutive columns of this thread's TMEM lane
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
+// 16 TMEM lanes x 8 columns a group: lane t holds columns 2 (t % 4), + 1 of row
+// t / 4 (registers 0, 1) and of row t / 4 + 8 (2, 3).
+__device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[8]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
-        "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]),
-        "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
-        "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]),
-        "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
-      : "r"(taddr));
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(at));
+}
+// 16 TMEM lanes x 4 columns a group: lane t holds column t % 4 of rows t / 4 and
+// t / 4 + 8.
+__device__ __forceinline__ void tmem_st_frag(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
 }
 // Two floats in one 64-bit register, and packed arithmetic on them.
 typedef unsigned long long f2;
@@ -183,7 +215,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 256);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kPrmSlots; ++i) mbar_init(&prm_full[i], 128);
@@ -252,17 +284,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int x = t & 1;
         if (!warp_wait(&k_full[x], (t >> 1) & 1)) return false;
         tc_fence_after();
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int j = 0; j < G / 16; ++j)
-              if (elect_one())
-                umma_f16_ss(tmem + x * 128 + g * N,
-                            dq + ((term * kTcRows * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4),
-                            dk + ((x * N * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4), id_s,
-                            term + j > 0 ? 1u : 0u);
+        // rolled: the loops' code stays in the instruction cache beside softmax
+#pragma unroll 1
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t d = tmem + x * 128 + g * N;
+          uint64_t qd = dq + ((g * G / 8 * 128) >> 4), kd = dk + ((x * N * D * 2 + g * G / 8 * 128) >> 4);
+          uint32_t more = 0;
+#pragma unroll 1
+          for (int term = 0; term < 2; ++term) {
+#pragma unroll 2
+            for (int j = 0; j < G / 16; ++j) {
+              if (elect_one()) umma_f16_ss(d, qd + j * 16, kd + j * 16, id_s, more);
+              more = 1;
+            }
+            qd += (kTcRows * D * 2) >> 4;
+          }
+        }
         if (elect_one()) {
           umma_commit(&s_full[x]);
           umma_commit(&k_empty[x]);
@@ -278,17 +315,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = warp_wait(&v_full[x], ph) && warp_wait(&p_full[x], ph);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int j = 0; j < N / 16; ++j)
-#pragma unroll
-            for (int term = 0; term < 2; ++term)
-              if (elect_one())
-                umma_f16_ts(tmem + 256 + x * D + g * G,
-                            tmem + x * 128 + g * N + (j >> 1) * 32 + term * 16 + (j & 1) * 8,
-                            dv + ((x * N * D * 2 + (g * G / 8) * SB_N + j * 256) >> 4), id_o,
-                            term + j > 0 ? 1u : 0u);
+#pragma unroll 1
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t d = tmem + 256 + x * D + g * G, pa = tmem + x * 128 + g * N;
+          const uint64_t vd = dv + ((x * N * D * 2 + (g * G / 8) * SB_N) >> 4);
+          uint32_t more = 0;
+#pragma unroll 1
+          for (int j = 0; j < N / 16; ++j) {
+            if (elect_one()) umma_f16_ts(d, pa + j * 16, vd + j * 16, id_o, more);
+            if (elect_one()) umma_f16_ts(d, pa + j * 16 + 8, vd + j * 16, id_o, 1u);
+            more = 1;
+          }
+        }
         if (elect_one()) {
           umma_commit(&o_full[x]);
           umma_commit(&v_empty[x]);
@@ -306,16 +344,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int pt = tid - kUnpack0, pw = pt >> 5;
     const uint32_t per = (uint32_t)a.bs / kTile;
-    // tile of 16 tokens at token position tok, or NULL
-    auto place = [&](int tok, bool report) -> const uint8_t* {
-      if (tok >= seg_len) return nullptr;
-      const uint32_t tt = (uint32_t)tok / kTile, page = tt / per;
-      const int blk = a.table[(int64_t)b * a.width + page];
-      if (blk < 0 || blk >= a.n_blocks) {
-        if (report && a.err) atomicExch(a.err, 4);
-        return nullptr;
+    // The place of a token that moves on by N a tile: its block-table entry and
+    // its tile within the block, kept without divisions.
+    struct Walk {
+      int tok;
+      uint32_t page, rem;
+    };
+    auto walk_at = [&](int tok) -> Walk {
+      const uint32_t tt = (uint32_t)tok / kTile;
+      return Walk{tok, tt / per, tt % per};
+    };
+    const int32_t* row_of_table = a.table + (int64_t)b * a.width;
+    auto step = [&](Walk& w, bool report) -> const uint8_t* {
+      const uint8_t* p = nullptr;
+      if (w.tok < seg_len) {
+        const int blk = row_of_table[w.page];
+        if (blk >= 0 && blk < a.n_blocks)
+          p = a.cache + (((int64_t)blk * a.hkv + kvh) * per + w.rem) * TB;
+        else if (report && a.err)
+          atomicExch(a.err, 4);                 // never read: its tokens count as absent
       }
-      return a.cache + (((int64_t)blk * a.hkv + kvh) * per + (tt - page * per)) * TB;
+      w.tok += N;
+      w.rem += N / kTile;
+      while (w.rem >= per) {
+        w.rem -= per;
+        ++w.page;
+      }
+      return p;
     };
     constexpr int KI = N * D / 32 / 128;        // 16-byte pieces of K rows a thread
     constexpr int VI = (N * NS + 127) / 128;    // 8 x 8 blocks of V a thread
@@ -326,39 +381,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint4 kw[KI];
     float2 kp, vp;
     uint32_t vw[VI][8];
-    // one tile's rows of K with all scales and minima, and its rows of V
-    auto load_k = [&](int base) {
-#pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int it = pt + i * 128, tok = it % N, part = it / N;
-        const uint8_t* p = place(base + tok, part == 0);
-        kw[i] = p ? *reinterpret_cast<const uint4*>(p + (tok % kTile) * (D / 2) + part * 16)
-                  : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-      }
-      const int tok = pt % N, n = pt / N;
-      const uint8_t* p = place(base + tok, false);
+    // K: token pt % N, every NG-th 16-byte piece of its row from pt / N on, and
+    // the scales and minima of its group pt / N.  V: 8 tokens from 8 kb on, the
+    // words of lane group g of one span or both.
+    const int k_tok = pt % N, k_part = pt / N, vg = pt & 7, v_kb = (pt >> 3) % (N / 8), v_sp = pt / N;
+    Walk wk = walk_at(t_first * N + k_tok), wv = walk_at(t_first * N + v_kb * 8);
+    auto load_k = [&]() {
+      const uint8_t* p = step(wk, k_part == 0);
       kp = vp = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < KI; ++i) kw[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
       if (p) {
-        kp = *reinterpret_cast<const float2*>(p + k_params_at(D) + (n * kTile + tok % kTile) * 8);
-        vp = *reinterpret_cast<const float2*>(p + v_params_at(D, NG) + (n * kTile + tok % kTile) * 8);
+        const uint4* row = reinterpret_cast<const uint4*>(p + (k_tok % kTile) * (D / 2)) + k_part;
+#pragma unroll
+        for (int i = 0; i < KI; ++i) kw[i] = row[i * NG];
+        kp = *reinterpret_cast<const float2*>(p + k_params_at(D) + (k_part * kTile + k_tok % kTile) * 8);
+        vp = *reinterpret_cast<const float2*>(p + v_params_at(D, NG) + (k_part * kTile + k_tok % kTile) * 8);
       }
     };
-    auto load_v = [&](int base) {
+    auto load_v = [&]() {
+      const int left = seg_len - wv.tok;        // of these 8 tokens
+      const uint8_t* p = step(wv, false);
+      if (VI * 128 > N * NS && pt >= N * NS) p = nullptr;
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const int it = pt + i * 128, g = it & 7, kb = (it >> 3) % (N / 8), sp = it / N;
-        const uint8_t* p = it < N * NS ? place(base + kb * 8, false) : nullptr;
+      for (int i = 0; i < VI; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          vw[i][e] = p && base + kb * 8 + e < seg_len
-                         ? *reinterpret_cast<const uint32_t*>(p + v_codes_at(D) + ((kb & 1) * 8 + e) * (D / 2) + (g * NS + sp) * 4)
-                         : 0x88888888u;
-      }
+        for (int e = 0; e < 8; ++e) {
+          vw[i][e] = 0x88888888u;
+          if (p && e < left)
+            vw[i][e] = *reinterpret_cast<const uint32_t*>(p + v_codes_at(D) + ((v_kb & 1) * 8 + e) * (D / 2) +
+                                                          (vg * NS + v_sp + i) * 4);
+        }
     };
-    load_k(t_first * N);
-    load_v(t_first * N);
+    load_k();
+    load_v();
     for (int t = 0; t < nt; ++t) {
-      const int x = t & 1, slot = t % kPrmSlots, base = (t_first + t) * N;
+      const int x = t & 1, slot = t % kPrmSlots;
       // The parameters' slot was last used four tiles ago; that tile's values
       // were found used up when V of the tile before last was written.
       // w = p s is brought to fp16's range by the largest s of the tile
@@ -370,10 +428,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int i = 0; i < N / 32; ++i) most = max(most, red[x * 4 + (pw * 32 / N) * (N / 32) + i]);
       const int e = max(20, min(254, (int)(most >> 23)));
-      prm[slot * 512 + pt] = kp.x;
-      prm[slot * 512 + 128 + pt] = fmaf(8.f, kp.x, kp.y);
-      prm[slot * 512 + 256 + pt] = vp.x * pow2_field(268 - e);  // largest in [2^14, 2^15)
-      prm[slot * 512 + 384 + pt] = fmaf(8.f, vp.x, vp.y);
+      float* pp = prm + slot * 512 + (pt >> 1) * 4 + (pt & 1);
+      pp[0] = kp.x;
+      pp[2] = fmaf(8.f, kp.x, kp.y);
+      pp[256] = vp.x * pow2_field(268 - e);     // largest in [2^14, 2^15)
+      pp[258] = fmaf(8.f, vp.x, vp.y);
       if (pt % N == 0) fac[slot * 4 + pt / N] = pow2_field(e - 14);
       mbar_arrive(&prm_full[slot]);
       // K: 8 channels of a token a 16-byte piece, in the order of Q's
@@ -381,27 +440,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint8_t* kd = smem + L::K + x * N * D * 2;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
-        const int it = pt + i * 128, tok = it % N, part = it / N;
+        const int part = k_part + i * NG;
         const uint32_t w4[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int m = part * 4 + q, c = m / NC, j = m % NC;
           const uint32_t w = w4[q], w8 = w >> 8;
-          *reinterpret_cast<uint4*>(kd + (tok >> 3) * SB_D + (j * 4 + c) * 128 + (tok & 7) * 16) =
+          *reinterpret_cast<uint4*>(kd + (k_tok >> 3) * SB_D + (j * 4 + c) * 128 + (k_tok & 7) * 16) =
               make_uint4(code_even(w), code_even(w8), code_odd(w), code_odd(w8));
         }
       }
       fence_async_shared();
       mbar_arrive(&k_full[x]);
-      load_k(base + N);                         // on its way through the wait for V's buffer
+      load_k();                       // on its way through the wait for V's buffer
       // V: 8 tokens of a channel a 16-byte piece; row n = 64 s + 8 i + g is
       // channel 64 s + 32 (i / 4) + 4 g + i % 4
       if (t >= 2) ok = ok && wait(&v_empty[x], ((t >> 1) - 1) & 1);
       uint8_t* vd = smem + L::V + x * N * D * 2;
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
-        const int it = pt + i * 128, g = it & 7, kb = (it >> 3) % (N / 8), sp = it / N;
-        if (it < N * NS) {
+        if (VI * 128 <= N * NS || pt < N * NS) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t xx[4];
@@ -414,29 +472,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               o.y = k & 1 ? code_odd(xx[1] >> (k & 2) * 4) : code_even(xx[1] >> (k & 2) * 4);
               o.z = k & 1 ? code_odd(xx[2] >> (k & 2) * 4) : code_even(xx[2] >> (k & 2) * 4);
               o.w = k & 1 ? code_odd(xx[3] >> (k & 2) * 4) : code_even(xx[3] >> (k & 2) * 4);
-              *reinterpret_cast<uint4*>(vd + (sp * 8 + h * 4 + k) * SB_N + kb * 128 + g * 16) = o;
+              *reinterpret_cast<uint4*>(vd + ((v_sp + i) * 8 + h * 4 + k) * SB_N + v_kb * 128 + vg * 16) = o;
             }
           }
         }
       }
       fence_async_shared();
       mbar_arrive(&v_full[x]);
-      load_v(base + N);
+      load_v();
     }
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int wg = warp >> 2, row = tid & 127;  // both warpgroups hold the same rows
-    const uint32_t lane_at = tmem + ((uint32_t)(warp & 3) << 21);
-    const bool row_ok = row < rows;
-    const int rr = tile * kTcRows + row;
-    const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
-    const int limit = row_ok ? max(0, min(s.len, s.len - s.n + tok + 1)) : 0;
-    const int64_t at = ((s.row0 + tok) * a.h + hq) * D;
-    float qs[NG], row_f;
     {
-      // this row of q: the warpgroups write its high and its low terms
-      const float4* q4 = reinterpret_cast<const float4*>(a.q + (row_ok ? at : 0));
+      // this thread's row of q: the two warpgroups write its two terms
+      const int term = warp >> 2, row = tid & 127;
+      const bool row_ok = row < rows;
+      const int rr = tile * kTcRows + row;
+      const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
+      float qs[NG], row_f;
+      const float4* q4 = reinterpret_cast<const float4*>(a.q + (row_ok ? ((s.row0 + tok) * a.h + hq) * D : 0));
       float amax = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
@@ -455,7 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       row_f = pow2_field(e - 14);
 #pragma unroll
       for (int n = 0; n < NG; ++n) qs[n] *= up;
-      uint8_t* qd = smem + L::Q + wg * kTcRows * D * 2 + (row >> 3) * SB_D + (row & 7) * 16;
+      uint8_t* qd = smem + L::Q + term * kTcRows * D * 2 + (row >> 3) * SB_D + (row & 7) * 16;
 #pragma unroll 4
       for (int j = 0; j < D / 8; ++j) {
         const float4 v0 = row_ok ? q4[2 * j] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -465,195 +520,252 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < 8; ++i) {
           y[i] = y[i] * a.scale2 * up;
           const float h = __half2float(__float2half_rn(y[i]));
-          y[i] = wg ? y[i] - h : h;
+          y[i] = term ? y[i] - h : h;
         }
         *reinterpret_cast<uint4*>(qd + j * 128) =
             make_uint4(pack_h2(y[0], y[4]), pack_h2(y[2], y[6]), pack_h2(y[1], y[5]), pack_h2(y[3], y[7]));
       }
+      if (term == 0) {
+        float* rc = reinterpret_cast<float*>(smem + L::ROW) + row;
+        rc[0] = row_f;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) rc[(1 + n) * 128] = qs[n];
+      }
       fence_async_shared();
       mbar_arrive(q_full);
+      named_barrier(2, 256);
     }
-    float m = -INFINITY;
-    f2 l2 = pk(0.f, 0.f), mins[NG], o[D / 2];
+    // This warp: rows 32 quad .. + 31, half hc of a tile's tokens and of the
+    // channels.  This lane: rows row0 + 8 i (i = 0 .. 3), of every 8 columns the
+    // pair 2 c, 2 c + 1.
+    constexpr int CW = N / 2, NP = CW / 8, OW = D / 2, OP = OW / 8;
+    const int quad = warp & 3, hc = warp >> 2, c = lane & 3, row0 = quad * 32 + (lane >> 2);
+    const uint32_t quad_at = tmem + ((uint32_t)quad << 21);
+    f2 qs[NG][4], rf[4], l2[4], mins[NG][4], o[2][OP][2];
+    float m[4], corr[4] = {1.f, 1.f, 1.f, 1.f}, fac[NG] = {};
+    int limit[4];
 #pragma unroll
-    for (int n = 0; n < NG; ++n) mins[n] = l2;
-#pragma unroll
-    for (int i = 0; i < D / 2; ++i) o[i] = l2;
-    const f2 rf2 = pk(row_f, row_f);
-    bool ok = true;
-    for (int t = wg; ok && t < nt; t += 2) {
-      const uint32_t ph = (uint32_t)(t >> 1) & 1u;
-      const int slot = t % kPrmSlots, base = (t_first + t) * N;
-      const float* prm = reinterpret_cast<const float*>(smem + L::PRM) + slot * 512;
-      ok = wait(&prm_full[slot], (uint32_t)(t / kPrmSlots) & 1u) && wait(&s_full[wg], ph);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const bool cut = base + N > all_see;      // some row does not see all of the tile
-      // x of chunk k's 32 tokens, out of the scores of every group
-      auto scores = [&](f2 (&x)[16], int k) {
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          float sc[32];
-          tmem_ld32(lane_at + wg * 128 + n * N + 32 * k, sc);
-          tmem_wait_ld();
-          const f2 q2 = pk(qs[n], qs[n]);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(prm + n * N + 32 * k + i);
-            const ulonglong2 km = *reinterpret_cast<const ulonglong2*>(prm + 128 + n * N + 32 * k + i);
-            x[i / 2] = fma2(pk(sc[i], sc[i + 1]), ks.x, n ? fma2(q2, km.x, x[i / 2]) : mul2(q2, km.x));
-            x[i / 2 + 1] = fma2(pk(sc[i + 2], sc[i + 3]), ks.y, n ? fma2(q2, km.y, x[i / 2 + 1]) : mul2(q2, km.y));
-          }
-        }
-        if (cut) {
-          const int seen = limit - (base + 32 * k);  // this row sees so many of them
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[i] = pk(2 * i < seen ? lo_of(x[i]) : -INFINITY, 2 * i + 1 < seen ? hi_of(x[i]) : -INFINITY);
-        }
-      };
-      // pass 1: the largest x
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int k = 0; k < N / 32; ++k) {
-        f2 x[16];
-        scores(x, k);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(lo_of(x[i]), hi_of(x[i])));
-      }
-      const float m_new = fmaxf(m, top * row_f);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = ex2(m - ref);          // 0 while nothing was seen
-      m = m_new;
-      const f2 corr2 = pk(corr, corr), neg = pk(-ref, -ref), minus = pk(-1.f, -1.f);
-      l2 = mul2(l2, corr2);
-#pragma unroll
-      for (int n = 0; n < NG; ++n) mins[n] = mul2(mins[n], corr2);
-      // pass 2: probabilities, and w's two terms in place of the scores.  The
-      // loops over chunks stay loops: unrolled, the two warpgroups' code does
-      // not fit the instruction cache and fetching it takes five times longer
-      // than running it.
-#pragma unroll 1
-      for (int k = 0; k < N / 32; ++k) {
-        f2 x[16];
-        scores(x, k);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = fma2(x[i], rf2, neg);
-          x[i] = pk(ex2(lo_of(x[i])), ex2(hi_of(x[i])));
-          l2 = add2(l2, x[i]);
-        }
-        const int seen = limit - (base + 32 * k);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          const float* pv = prm + 256 + n * N + 32 * k;
-          uint32_t w[32];                       // high terms, then low ones
-          if (cut) {                            // 0 times a NaN that this row does not see is 0
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const f2 vm = *reinterpret_cast<const f2*>(pv + 128 + 2 * i), u = mul2(x[i], vm);
-              mins[n] = add2(mins[n], pk(2 * i < seen ? lo_of(u) : 0.f, 2 * i + 1 < seen ? hi_of(u) : 0.f));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const ulonglong2 vm = *reinterpret_cast<const ulonglong2*>(pv + 128 + 2 * i);
-              mins[n] = fma2(x[i], vm.x, mins[n]);
-              mins[n] = fma2(x[i + 1], vm.y, mins[n]);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(pv + 2 * i);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              f2 w2 = mul2(x[i + e], e ? vs.y : vs.x);
-              if (cut) w2 = pk(2 * (i + e) < seen ? lo_of(w2) : 0.f, 2 * (i + e) + 1 < seen ? hi_of(w2) : 0.f);
-              // the high term is w cut to 11 bits (exact in fp16), the low one the rest
-              const float h0 = __uint_as_float((uint32_t)w2 & 0xFFFFE000u);
-              const float h1 = __uint_as_float((uint32_t)(w2 >> 32) & 0xFFFFE000u);
-              const f2 rest = fma2(pk(h0, h1), minus, w2);
-              w[i + e] = pack_h2(h0, h1);
-              w[16 + i + e] = pack_h2(lo_of(rest), hi_of(rest));
-            }
-          }
-          tmem_st32(lane_at + wg * 128 + n * N + 32 * k, w);
-        }
-      }
-      // what the slot holds is in registers before the unpack warps may fill it again
-      f2 f[NG];
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + 8 * i;
+      const float* rc = reinterpret_cast<const float*>(smem + L::ROW) + row;
+      rf[i] = pk(rc[0], rc[0]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const float v = reinterpret_cast<const float*>(smem + L::F)[slot * 4 + n];
-        f[n] = pk(v, v);
+        qs[n][i] = pk(rc[(1 + n) * 128], rc[(1 + n) * 128]);
+        mins[n][i] = 0;
       }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[wg]);
-      if (__any_sync(0xffffffffu, corr != 1.f))
+      l2[i] = 0;
+      m[i] = -INFINITY;
+      const int tok = (int)((uint32_t)(tile * kTcRows + row) / (uint32_t)a.r);
+      limit[i] = row < rows ? max(0, min(s.len, s.len - s.n + tok + 1)) : 0;
+    }
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) o[i] = mul2(o[i], corr2);
-      // the tile's sums of values
-      ok = __all_sync(0xffffffffu, wait(&o_full[wg], ph));
-      if (!ok) break;
+    for (int i = 0; i < OP; ++i) o[0][i][0] = o[0][i][1] = o[1][i][0] = o[1][i][1] = 0;
+    bool ok = true;                             // after an expired wait the rounds go on without waits
+    // the sums of values of tile t, added to what was there before
+    auto flush = [&](int t) {
+      const int x = t & 1;
+      ok = __all_sync(0xffffffffu, ok && wait(&o_full[x], (uint32_t)(t >> 1) & 1u));
+      if (!ok) return;
       tc_fence_after();
+      const bool moved = corr[0] != 1.f || corr[1] != 1.f || corr[2] != 1.f || corr[3] != 1.f;
+      if (__any_sync(0xffffffffu, moved))
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        float acc[32];
-        tmem_ld32(lane_at + 256 + wg * D + 32 * k, acc);
+        for (int i = 0; i < 4; ++i) {
+          const f2 c2 = pk(corr[i], corr[i]);
+#pragma unroll
+          for (int j = 0; j < OP; ++j) o[i >> 1][j][i & 1] = mul2(o[i >> 1][j][i & 1], c2);
+        }
+#pragma unroll
+      for (int rh = 0; rh < 2; ++rh) {
+        float acc[OP * 4];
+        tmem_ld_frag(quad_at + ((uint32_t)rh << 20) + 256 + x * D + hc * OW, acc);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[16 * k + i] = fma2(pk(acc[2 * i], acc[2 * i + 1]), f[32 * k / G], o[16 * k + i]);
+        for (int j = 0; j < OP; ++j) {
+          float f1 = fac[0];
+#pragma unroll
+          for (int n = 1; n < NG; ++n) f1 = (hc * OW + 8 * j) / G == n ? fac[n] : f1;
+          const f2 f = pk(f1, f1);
+          o[rh][j][0] = fma2(pk(acc[4 * j], acc[4 * j + 1]), f, o[rh][j][0]);
+          o[rh][j][1] = fma2(pk(acc[4 * j + 2], acc[4 * j + 3]), f, o[rh][j][1]);
+        }
       }
       tc_fence_before();
-    }
-    // ---- the two warpgroups' results; the operands' memory is free
-    named_barrier(2, 256);
-    float l = lo_of(l2) + hi_of(l2);
-    float* xo = reinterpret_cast<float*>(smem + L::Q);      // [D][128]
-    float* xs = reinterpret_cast<float*>(smem + L::PRM);    // m, l, minima [128]
-    if (wg == 1) {
+    };
+    for (int t = 0; t < nt; ++t) {
+      const int b2 = t & 1, slot = t % kPrmSlots, base = (t_first + t) * N + hc * CW + 2 * c;
+      const float4* prm = reinterpret_cast<const float4*>(smem + L::PRM) + slot * 128 + hc * (CW / 2) + c;
+      ok = ok && wait(&prm_full[slot], (uint32_t)(t / kPrmSlots) & 1u) && wait(&s_full[b2], (uint32_t)(t >> 1) & 1u);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const uint32_t s_at = quad_at + b2 * 128 + hc * CW;
+      // x of 4 rows x NP pairs of tokens
+      f2 x[2][NP][2];
 #pragma unroll
-      for (int i = 0; i < D / 2; ++i) {
-        xo[(2 * i) * 128 + row] = lo_of(o[i]);
-        xo[(2 * i + 1) * 128 + row] = hi_of(o[i]);
-      }
-      xs[row] = m;
-      xs[128 + row] = l;
+      for (int n = 0; n < NG; ++n) {
+        float sc[2][NP * 4];
+        tmem_ld_frag(s_at + n * N, sc[0]);
+        tmem_ld_frag(s_at + (1u << 20) + n * N, sc[1]);
+        tmem_wait_ld();
 #pragma unroll
-      for (int n = 0; n < NG; ++n) xs[(2 + n) * 128 + row] = lo_of(mins[n]) + hi_of(mins[n]);
-    }
-    named_barrier(2, 256);
-    if (wg == 0 && row_ok) {
-      const float m1 = xs[row], top = fmaxf(m, m1), ref = top == -INFINITY ? 0.f : top;
-      const float f0 = ex2(m - ref), f1 = ex2(m1 - ref);
-      l = l * f0 + xs[128 + row] * f1;
-      const bool whole = splits == 1;
-      float* part = reinterpret_cast<float*>(parts + (size_t)blockIdx.x * kTcRows * (D + 2) * 4);
-      float* dst = whole ? a.out + at : part + row * D;
-      const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        for (int j = 0; j < NP; ++j) {
+          const float4 p = prm[n * (N / 2) + 4 * j];
+          const f2 ks = pk(p.x, p.y), km = pk(p.z, p.w);
 #pragma unroll
-      for (int sp = 0; sp < NS; ++sp)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int n = (64 * sp + 32 * h) / G;
-          const float mn = (lo_of(mins[n]) + hi_of(mins[n])) * f0 + xs[(2 + n) * 128 + row] * f1;
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int c = 64 * sp + 8 * (4 * h + i) + g;
-              const float mine = c & 1 ? hi_of(o[c / 2]) : lo_of(o[c / 2]);
-              v[i] = (mine * f0 + xo[c * 128 + row] * f1 + mn) * inv;
-            }
-            *reinterpret_cast<float4*>(dst + 64 * sp + 32 * h + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+          for (int i = 0; i < 4; ++i) {
+            f2& v = x[i >> 1][j][i & 1];
+            const f2 b = n ? fma2(qs[n][i], km, v) : mul2(qs[n][i], km);
+            v = fma2(pk(sc[i >> 1][4 * j + 2 * (i & 1)], sc[i >> 1][4 * j + 2 * (i & 1) + 1]), ks, b);
           }
         }
-      if (!whole) {
-        part[kTcRows * D + row] = top;
-        part[kTcRows * (D + 1) + row] = l;
+      }
+      const bool cut = (t_first + t + 1) * N > all_see;  // some row does not see all of the tile
+      if (cut)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            f2& v = x[i >> 1][j][i & 1];
+            v = pk(base + 8 * j < limit[i] ? lo_of(v) : -INFINITY, base + 8 * j + 1 < limit[i] ? hi_of(v) : -INFINITY);
+          }
+      // the rows' maxima over both halves
+      float top[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        top[i] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) top[i] = fmaxf(top[i], fmaxf(lo_of(x[i >> 1][j][i & 1]), hi_of(x[i >> 1][j][i & 1])));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      }
+      float* mx = reinterpret_cast<float*>(smem + L::MAX) + b2 * 256 + row0;
+      mx[hc * 128 + 8 * c] = c == 0 ? top[0] : c == 1 ? top[1] : c == 2 ? top[2] : top[3];
+      named_barrier(3 + quad, 64);
+      float keep[4];
+      f2 ref2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float m_new = fmaxf(m[i], fmaxf(top[i], mx[(hc ^ 1) * 128 + 8 * i]) * lo_of(rf[i]));
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        keep[i] = ex2(m[i] - ref);              // 0 while nothing was seen
+        m[i] = m_new;
+        ref2[i] = pk(-ref, -ref);
+        const f2 k2 = pk(keep[i], keep[i]);
+        l2[i] = mul2(l2[i], k2);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mins[n][i] = mul2(mins[n][i], k2);
+      }
+      // probabilities
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f2& v = x[i >> 1][j][i & 1];
+          v = fma2(v, rf[i], ref2[i]);
+          v = pk(ex2(lo_of(v)), ex2(hi_of(v)));
+          l2[i] = add2(l2[i], v);
+        }
+      // w in two terms over the scores, and the minima's sums
+      auto weights = [&](auto part_seen) {
+        constexpr bool kCut = decltype(part_seen)::value;
+        const f2 minus = pk(-1.f, -1.f);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          uint32_t w[2][NP * 4];
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const float4 p = prm[64 + n * (N / 2) + 4 * j];
+            const f2 vs = pk(p.x, p.y), vm = pk(p.z, p.w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f2 v = x[i >> 1][j][i & 1];
+              f2 w2 = mul2(v, vs);
+              if (kCut) {                       // 0 times a NaN that this row does not see is 0
+                const bool in0 = base + 8 * j < limit[i], in1 = base + 8 * j + 1 < limit[i];
+                const f2 u = mul2(v, vm);
+                mins[n][i] = add2(mins[n][i], pk(in0 ? lo_of(u) : 0.f, in1 ? hi_of(u) : 0.f));
+                w2 = pk(in0 ? lo_of(w2) : 0.f, in1 ? hi_of(w2) : 0.f);
+              } else {
+                mins[n][i] = fma2(v, vm, mins[n][i]);
+              }
+              // the high term is w cut to 11 bits (exact in fp16), the low one the rest
+              const f2 high = w2 & 0xFFFFE000FFFFE000ull, rest = fma2(high, minus, w2);
+              // 16 tokens: two groups of 4 columns of high terms, two of low ones
+              uint32_t* d = &w[i >> 1][(j >> 1) * 8 + (j & 1) * 2 + (i & 1)];
+              d[0] = pack_h2(lo_of(high), hi_of(high));
+              d[4] = pack_h2(lo_of(rest), hi_of(rest));
+            }
+          }
+          tmem_st_frag(s_at + n * N, w[0]);
+          tmem_st_frag(s_at + (1u << 20) + n * N, w[1]);
+        }
+      };
+      if (cut)
+        weights(std::true_type());
+      else
+        weights(std::false_type());
+      float fac_new[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) fac_new[n] = reinterpret_cast<const float*>(smem + L::F)[slot * 4 + n];
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[b2]);
+      if (t > 0) flush(t - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) corr[i] = keep[i];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) fac[n] = fac_new[n];
+    }
+    if (nt > 0) flush(nt - 1);
+    // ---- sums over the quad's lanes and both halves' warps
+    float* xs = reinterpret_cast<float*>(smem + L::PRM);    // [halves][1 + NG][128]
+    named_barrier(2, 256);
+    float l[4], mn[NG][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      l[i] = lo_of(l2[i]) + hi_of(l2[i]);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if (c == 0) xs[hc * (1 + NG) * 128 + row0 + 8 * i] = l[i];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        mn[n][i] = lo_of(mins[n][i]) + hi_of(mins[n][i]);
+        mn[n][i] += __shfl_xor_sync(0xffffffffu, mn[n][i], 1);
+        mn[n][i] += __shfl_xor_sync(0xffffffffu, mn[n][i], 2);
+        if (c == 0) xs[(hc * (1 + NG) + 1 + n) * 128 + row0 + 8 * i] = mn[n][i];
+      }
+    }
+    named_barrier(2, 256);
+    const bool whole = splits == 1;
+    float* part = reinterpret_cast<float*>(parts + (size_t)blockIdx.x * kTcRows * (D + 2) * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + 8 * i;
+      if (row >= rows) continue;
+      // in the order of the halves, so that both warps have the same sums
+      const float L0 = xs[row], L1 = xs[(1 + NG) * 128 + row], total = L0 + L1;
+      const int rr = tile * kTcRows + row;
+      const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
+      float* dst = whole ? a.out + ((s.row0 + tok) * a.h + hq) * D : part + row * D;
+      const float inv = !whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+      for (int j = 0; j < OP; j += 4) {         // 4 nibbles x 2 lanes' g: 8 channels in a row
+        const int at = hc * OW / 8 + j, ch = 64 * (at / 8) + 32 * (at % 8 / 4) + 8 * c;
+        const float* pm = xs + (1 + (64 * (at / 8) + 32 * (at % 8 / 4)) / G) * 128 + row;
+        const float mean = pm[0] + pm[(1 + NG) * 128];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = (lo_of(o[i >> 1][j + k][i & 1]) + mean) * inv;
+          v[4 + k] = (hi_of(o[i >> 1][j + k][i & 1]) + mean) * inv;
+        }
+        reinterpret_cast<float4*>(dst + ch)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(dst + ch)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      if (!whole && hc == 0 && c == 0) {
+        part[kTcRows * D + row] = m[i];
+        part[kTcRows * (D + 1) + row] = total;
       }
     }
   }
