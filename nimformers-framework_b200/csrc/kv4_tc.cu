@@ -12,12 +12,12 @@
 // run in TMEM over one tile of tokens only and are added to float32 registers
 // between, so that the tensor core's cut-off additions stay few.
 //
-// Roles: eight softmax warps, a warp 32 rows x half of a tile's tokens; four warps
-// unpack codes into the K and V operands (two buffers each); one warp issues the
-// MMAs.  S and O have two buffers too: while tile t is in softmax the tensor core
-// multiplies the values of tile t - 1 and the keys of tile t + 1.  P overwrites
-// S in place: 16 columns of scores become 8 of high and 8 of low terms.
-// Softmax reads TMEM in the MMA fragment shape (a lane 4 rows x every fourth pair
+// Roles: eight softmax warps of 16 rows; four warps that unpack codes into the K
+// and V operands (two buffers each); one warp that issues the MMAs.  S and O have
+// two buffers too: while tile t is in softmax the tensor core multiplies the
+// values of tile t - 1 and the keys of tile t + 1.  P overwrites S in place: 16
+// columns of scores become 8 of high and 8 of low terms.
+// Softmax reads TMEM in the MMA fragment shape (a lane 2 rows x every fourth pair
 // of columns): scales and minima are per column, and a lane with whole rows loads
 // four times as many of them, which alone took longer than the products.
 #include <algorithm>
@@ -48,8 +48,7 @@ struct TcLayout {
   static constexpr int F = PRM + kPrmSlots * 4 * 128 * 4;       // [slots][NG] float
   static constexpr int RED = F + kPrmSlots * 4 * 4;             // [2][4] uint32
   static constexpr int ROW = RED + 32;                          // [1 + NG][128]: row_f, sums of q
-  static constexpr int MAX = ROW + (1 + NG) * 128 * 4;          // [2][2][128]: maxima of the halves
-  static constexpr int BAR = MAX + 4 * 128 * 4;                 // barriers
+  static constexpr int BAR = ROW + (1 + NG) * 128 * 4;                 // barriers
   static constexpr int SIZE = BAR + 256;
 };
 
@@ -67,12 +66,6 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uin
 }
 // 16 TMEM lanes x 8 columns a group: lane t holds columns 2 (t % 4), + 1 of row
 // t / 4 (registers 0, 1) and of row t / 4 + 8 (2, 3).
-__device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
-      : "r"(at));
-}
 __device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -87,12 +80,6 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t at, float (&r)[32]) {
 }
 // 16 TMEM lanes x 4 columns a group: lane t holds column t % 4 of rows t / 4 and
 // t / 4 + 8.
-__device__ __forceinline__ void tmem_st_frag(uint32_t at, const uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_frag(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
@@ -267,6 +254,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     return false;
   };
 
+  // The unpack warps are ahead: their polls leave the issue slots to softmax.
+  auto slow_wait = [&](uint64_t* m, uint32_t parity) -> bool {
+    for (uint32_t i = 0; i < kMaxSpin; ++i) {
+      if (mbar_try_wait_sleep(m, parity, 100u)) return true;
+      if (stopped()) return false;
+    }
+    return wait(m, parity);
+  };
+
   if (warp >= 12) {
     // ---------------------------------------------------------------- MMA issue
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -436,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (pt % N == 0) fac[slot * 4 + pt / N] = pow2_field(e - 14);
       mbar_arrive(&prm_full[slot]);
       // K: 8 channels of a token a 16-byte piece, in the order of Q's
-      if (t >= 2) ok = ok && wait(&k_empty[x], ((t >> 1) - 1) & 1);
+      if (t >= 2) ok = ok && slow_wait(&k_empty[x], ((t >> 1) - 1) & 1);
       uint8_t* kd = smem + L::K + x * N * D * 2;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
@@ -455,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       load_k();                       // on its way through the wait for V's buffer
       // V: 8 tokens of a channel a 16-byte piece; row n = 64 s + 8 i + g is
       // channel 64 s + 32 (i / 4) + 4 g + i % 4
-      if (t >= 2) ok = ok && wait(&v_empty[x], ((t >> 1) - 1) & 1);
+      if (t >= 2) ok = ok && slow_wait(&v_empty[x], ((t >> 1) - 1) & 1);
       uint8_t* vd = smem + L::V + x * N * D * 2;
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
@@ -484,74 +480,79 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    {
-      // this thread's row of q: the two warpgroups write its two terms
-      const int term = warp >> 2, row = tid & 127;
-      const bool row_ok = row < rows;
-      const int rr = tile * kTcRows + row;
+    // ---- the rows of q: 8 rows x 4 pieces of 8 channels at a time
+    const int quad = warp & 3, half = warp >> 2, c = lane & 3;
+    float* rc = reinterpret_cast<float*>(smem + L::ROW);
+#pragma unroll 1
+    for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 8) {
+      const int row = r0 + (lane & 7), rr = tile * kTcRows + row;
       const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
-      float qs[NG], row_f;
-      const float4* q4 = reinterpret_cast<const float4*>(a.q + (row_ok ? ((s.row0 + tok) * a.h + hq) * D : 0));
-      float amax = 0.f;
+      const float* qr = a.q + ((s.row0 + tok) * a.h + hq) * D + (lane >> 3) * 8;
+      float y[NC][8], amax = 0.f, sum[NG];
 #pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        float t = 0.f;
-#pragma unroll 8
-        for (int j = 0; j < G / 4; ++j) {
-          const float4 v = row_ok ? q4[n * (G / 4) + j] : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float x0 = v.x * a.scale2, x1 = v.y * a.scale2, x2 = v.z * a.scale2, x3 = v.w * a.scale2;
-          amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x0), fabsf(x1))), fmaxf(fabsf(x2), fabsf(x3)));
-          t += (x0 + x1) + (x2 + x3);
+      for (int k = 0; k < NC; ++k) {
+        float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+        if (row < rows) {
+          v0 = *reinterpret_cast<const float4*>(qr + 32 * k);
+          v1 = *reinterpret_cast<const float4*>(qr + 32 * k + 4);
         }
-        qs[n] = t;
+        y[k][0] = v0.x; y[k][1] = v0.y; y[k][2] = v0.z; y[k][3] = v0.w;
+        y[k][4] = v1.x; y[k][5] = v1.y; y[k][6] = v1.z; y[k][7] = v1.w;
       }
-      const int e = max(20, min(240, exp_field(amax)));
-      const float up = pow2_field(268 - e);     // the largest magnitude in [2^14, 2^15)
-      row_f = pow2_field(e - 14);
 #pragma unroll
-      for (int n = 0; n < NG; ++n) qs[n] *= up;
-      uint8_t* qd = smem + L::Q + term * kTcRows * D * 2 + (row >> 3) * SB_D + (row & 7) * 16;
-#pragma unroll 4
-      for (int j = 0; j < D / 8; ++j) {
-        const float4 v0 = row_ok ? q4[2 * j] : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 v1 = row_ok ? q4[2 * j + 1] : make_float4(0.f, 0.f, 0.f, 0.f);
-        float y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+      for (int n = 0; n < NG; ++n) sum[n] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          y[i] = y[i] * a.scale2 * up;
-          const float h = __half2float(__float2half_rn(y[i]));
-          y[i] = term ? y[i] - h : h;
+          y[k][i] *= a.scale2;
+          amax = fmaxf(amax, fabsf(y[k][i]));
+          sum[k * 32 / G] += y[k][i];
         }
-        *reinterpret_cast<uint4*>(qd + j * 128) =
-            make_uint4(pack_h2(y[0], y[4]), pack_h2(y[2], y[6]), pack_h2(y[1], y[5]), pack_h2(y[3], y[7]));
-      }
-      if (term == 0) {
-        float* rc = reinterpret_cast<float*>(smem + L::ROW) + row;
-        rc[0] = row_f;
-#pragma unroll
-        for (int n = 0; n < NG; ++n) rc[(1 + n) * 128] = qs[n];
-      }
-      fence_async_shared();
-      mbar_arrive(q_full);
-      named_barrier(2, 256);
-    }
-    // This warp: rows 32 quad .. + 31, half hc of a tile's tokens and of the
-    // channels.  This lane: rows row0 + 8 i (i = 0 .. 3), of every 8 columns the
-    // pair 2 c, 2 c + 1.
-    constexpr int CW = N / 2, NP = CW / 8, OW = D / 2, OP = OW / 8;
-    const int quad = warp & 3, hc = warp >> 2, c = lane & 3, row0 = quad * 32 + (lane >> 2);
-    const uint32_t quad_at = tmem + ((uint32_t)quad << 21);
-    f2 qs[NG][4], rf[4], l2[4], mins[NG][4], o[2][OP][2];
-    float m[4], corr[4] = {1.f, 1.f, 1.f, 1.f}, fac[NG] = {};
-    int limit[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + 8 * i;
-      const float* rc = reinterpret_cast<const float*>(smem + L::ROW) + row;
-      rf[i] = pk(rc[0], rc[0]);
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+      const int e = max(20, min(240, exp_field(amax)));
+      const float up = pow2_field(268 - e);     // the largest magnitude in [2^14, 2^15)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        qs[n][i] = pk(rc[(1 + n) * 128], rc[(1 + n) * 128]);
+        sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 8);
+        sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 16);
+        if (lane < 8) rc[(1 + n) * 128 + row] = sum[n] * up;
+      }
+      if (lane < 8) rc[row] = pow2_field(e - 14);
+      uint8_t* qd = smem + L::Q + (row >> 3) * SB_D + (lane >> 3) * 128 + (lane & 7) * 16;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        float h[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[k][i] *= up;
+          h[i] = __half2float(__float2half_rn(y[k][i]));
+          l[i] = y[k][i] - h[i];
+        }
+        *reinterpret_cast<uint4*>(qd + k * 512) =
+            make_uint4(pack_h2(h[0], h[4]), pack_h2(h[2], h[6]), pack_h2(h[1], h[5]), pack_h2(h[3], h[7]));
+        *reinterpret_cast<uint4*>(qd + kTcRows * D * 2 + k * 512) =
+            make_uint4(pack_h2(l[0], l[4]), pack_h2(l[2], l[6]), pack_h2(l[1], l[5]), pack_h2(l[3], l[7]));
+      }
+    }
+    fence_async_shared();
+    mbar_arrive(q_full);
+    named_barrier(2, 256);
+    // This lane: rows row0 and row0 + 8, of every 8 columns the pair 2 c, 2 c + 1.
+    constexpr int NP = N / 8, OP = D / 8;
+    const int row0 = quad * 32 + half * 16 + (lane >> 2);
+    const uint32_t my_at = tmem + ((uint32_t)quad << 21) + ((uint32_t)half << 20);
+    f2 qs[NG][2], rf[2], l2[2], mins[NG][2], o[OP][2];
+    float m[2], corr[2] = {1.f, 1.f}, fac[NG] = {};
+    int limit[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + 8 * i;
+      rf[i] = pk(rc[row], rc[row]);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        qs[n][i] = pk(rc[(1 + n) * 128 + row], rc[(1 + n) * 128 + row]);
         mins[n][i] = 0;
       }
       l2[i] = 0;
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       limit[i] = row < rows ? max(0, min(s.len, s.len - s.n + tok + 1)) : 0;
     }
 #pragma unroll
-    for (int i = 0; i < OP; ++i) o[0][i][0] = o[0][i][1] = o[1][i][0] = o[1][i][1] = 0;
+    for (int j = 0; j < OP; ++j) o[j][0] = o[j][1] = 0;
     bool ok = true;                             // after an expired wait the rounds go on without waits
     // the sums of values of tile t, added to what was there before
     auto flush = [&](int t) {
@@ -568,85 +569,75 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ok = __all_sync(0xffffffffu, ok && wait(&o_full[x], (uint32_t)(t >> 1) & 1u));
       if (!ok) return;
       tc_fence_after();
-      const bool moved = corr[0] != 1.f || corr[1] != 1.f || corr[2] != 1.f || corr[3] != 1.f;
-      if (__any_sync(0xffffffffu, moved))
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f))
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const f2 c2 = pk(corr[i], corr[i]);
 #pragma unroll
-          for (int j = 0; j < OP; ++j) o[i >> 1][j][i & 1] = mul2(o[i >> 1][j][i & 1], c2);
+          for (int j = 0; j < OP; ++j) o[j][i] = mul2(o[j][i], c2);
         }
 #pragma unroll
-      for (int rh = 0; rh < 2; ++rh) {
-        float acc[OP * 4];
-        tmem_ld_frag(quad_at + ((uint32_t)rh << 20) + 256 + x * D + hc * OW, acc);
+      for (int k = 0; k < NS; ++k) {
+        float acc[32];
+        tmem_ld_frag(my_at + 256 + x * D + 64 * k, acc);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < OP; ++j) {
-          float f1 = fac[0];
-#pragma unroll
-          for (int n = 1; n < NG; ++n) f1 = (hc * OW + 8 * j) / G == n ? fac[n] : f1;
+        for (int j = 0; j < 8; ++j) {
+          const float f1 = fac[(64 * k + 8 * j) / G];
           const f2 f = pk(f1, f1);
-          o[rh][j][0] = fma2(pk(acc[4 * j], acc[4 * j + 1]), f, o[rh][j][0]);
-          o[rh][j][1] = fma2(pk(acc[4 * j + 2], acc[4 * j + 3]), f, o[rh][j][1]);
+          o[8 * k + j][0] = fma2(pk(acc[4 * j], acc[4 * j + 1]), f, o[8 * k + j][0]);
+          o[8 * k + j][1] = fma2(pk(acc[4 * j + 2], acc[4 * j + 3]), f, o[8 * k + j][1]);
         }
       }
       tc_fence_before();
     };
+    constexpr int CH = N < 64 ? N : 64, CP = CH / 8;  // columns, pairs of a lane, of a TMEM access
     for (int t = 0; t < nt; ++t) {
-      const int b2 = t & 1, slot = t % kPrmSlots, base = (t_first + t) * N + hc * CW + 2 * c;
-      const float4* prm = reinterpret_cast<const float4*>(smem + L::PRM) + slot * 128 + hc * (CW / 2) + c;
+      const int b2 = t & 1, slot = t % kPrmSlots, base = (t_first + t) * N + 2 * c;
+      const float4* prm = reinterpret_cast<const float4*>(smem + L::PRM) + slot * 128 + c;
       ok = ok && wait(&prm_full[slot], (uint32_t)(t / kPrmSlots) & 1u) && wait(&s_full[b2], (uint32_t)(t >> 1) & 1u);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const uint32_t s_at = quad_at + b2 * 128 + hc * CW;
-      // x of 4 rows x NP pairs of tokens
-      f2 x[2][NP][2];
+      const uint32_t s_at = my_at + b2 * 128;
+      // x of 2 rows x NP pairs of tokens
+      f2 x[NP][2];
 #pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        float sc[2][NP * 4];
-        tmem_ld_frag(s_at + n * N, sc[0]);
-        tmem_ld_frag(s_at + (1u << 20) + n * N, sc[1]);
-        tmem_wait_ld();
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          const float4 p = prm[n * (N / 2) + 4 * j];
-          const f2 ks = pk(p.x, p.y), km = pk(p.z, p.w);
+        for (int k = 0; k < N / CH; ++k) {
+          float sc[CP * 4];
+          tmem_ld_frag(s_at + n * N + k * CH, sc);
+          tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f2& v = x[i >> 1][j][i & 1];
-            const f2 b = n ? fma2(qs[n][i], km, v) : mul2(qs[n][i], km);
-            v = fma2(pk(sc[i >> 1][4 * j + 2 * (i & 1)], sc[i >> 1][4 * j + 2 * (i & 1) + 1]), ks, b);
+          for (int j = 0; j < CP; ++j) {
+            const float4 p = prm[n * (N / 2) + 4 * (k * CP + j)];
+            const f2 ks = pk(p.x, p.y), km = pk(p.z, p.w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              f2& v = x[k * CP + j][i];
+              const f2 b = n ? fma2(qs[n][i], km, v) : mul2(qs[n][i], km);
+              v = fma2(pk(sc[4 * j + 2 * i], sc[4 * j + 2 * i + 1]), ks, b);
+            }
           }
         }
-      }
       const bool cut = (t_first + t + 1) * N > all_see;  // some row does not see all of the tile
       if (cut)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            f2& v = x[i >> 1][j][i & 1];
-            v = pk(base + 8 * j < limit[i] ? lo_of(v) : -INFINITY, base + 8 * j + 1 < limit[i] ? hi_of(v) : -INFINITY);
-          }
-      // the rows' maxima over both halves
-      float top[4];
+          for (int j = 0; j < NP; ++j)
+            x[j][i] = pk(base + 8 * j < limit[i] ? lo_of(x[j][i]) : -INFINITY,
+                         base + 8 * j + 1 < limit[i] ? hi_of(x[j][i]) : -INFINITY);
+      float keep[2];
+      f2 ref2[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        top[i] = -INFINITY;
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) top[i] = fmaxf(top[i], fmaxf(lo_of(x[i >> 1][j][i & 1]), hi_of(x[i >> 1][j][i & 1])));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      }
-      float* mx = reinterpret_cast<float*>(smem + L::MAX) + b2 * 256 + row0;
-      mx[hc * 128 + 8 * c] = c == 0 ? top[0] : c == 1 ? top[1] : c == 2 ? top[2] : top[3];
-      named_barrier(3 + quad, 64);
-      float keep[4];
-      f2 ref2[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float m_new = fmaxf(m[i], fmaxf(top[i], mx[(hc ^ 1) * 128 + 8 * i]) * lo_of(rf[i]));
+        for (int j = 0; j < NP; ++j) top = fmaxf(top, fmaxf(lo_of(x[j][i]), hi_of(x[j][i])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(m[i], top * lo_of(rf[i]));
         const float ref = m_new == -INFINITY ? 0.f : m_new;
         keep[i] = ex2(m[i] - ref);              // 0 while nothing was seen
         m[i] = m_new;
@@ -657,49 +648,56 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int n = 0; n < NG; ++n) mins[n][i] = mul2(mins[n][i], k2);
       }
       // probabilities
+      f2 more[2] = {0, 0};                      // a second chain of additions
 #pragma unroll
       for (int j = 0; j < NP; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f2& v = x[i >> 1][j][i & 1];
+        for (int i = 0; i < 2; ++i) {
+          f2& v = x[j][i];
           v = fma2(v, rf[i], ref2[i]);
           v = pk(ex2(lo_of(v)), ex2(hi_of(v)));
-          l2[i] = add2(l2[i], v);
+          if (j & 1)
+            more[i] = add2(more[i], v);
+          else
+            l2[i] = add2(l2[i], v);
         }
+      l2[0] = add2(l2[0], more[0]);
+      l2[1] = add2(l2[1], more[1]);
       // w in two terms over the scores, and the minima's sums
       auto weights = [&](auto part_seen) {
         constexpr bool kCut = decltype(part_seen)::value;
         const f2 minus = pk(-1.f, -1.f);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          uint32_t w[2][NP * 4];
+        for (int n = 0; n < NG; ++n)
 #pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            const float4 p = prm[64 + n * (N / 2) + 4 * j];
-            const f2 vs = pk(p.x, p.y), vm = pk(p.z, p.w);
+          for (int k = 0; k < N / CH; ++k) {
+            uint32_t w[CP * 4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f2 v = x[i >> 1][j][i & 1];
-              f2 w2 = mul2(v, vs);
-              if (kCut) {                       // 0 times a NaN that this row does not see is 0
-                const bool in0 = base + 8 * j < limit[i], in1 = base + 8 * j + 1 < limit[i];
-                const f2 u = mul2(v, vm);
-                mins[n][i] = add2(mins[n][i], pk(in0 ? lo_of(u) : 0.f, in1 ? hi_of(u) : 0.f));
-                w2 = pk(in0 ? lo_of(w2) : 0.f, in1 ? hi_of(w2) : 0.f);
-              } else {
-                mins[n][i] = fma2(v, vm, mins[n][i]);
+            for (int jj = 0; jj < CP; ++jj) {
+              const int j = k * CP + jj;
+              const float4 p = prm[64 + n * (N / 2) + 4 * j];
+              const f2 vs = pk(p.x, p.y), vm = pk(p.z, p.w);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                f2 w2 = mul2(x[j][i], vs);
+                if (kCut) {                     // 0 times a NaN that this row does not see is 0
+                  const bool in0 = base + 8 * j < limit[i], in1 = base + 8 * j + 1 < limit[i];
+                  const f2 u = mul2(x[j][i], vm);
+                  mins[n][i] = add2(mins[n][i], pk(in0 ? lo_of(u) : 0.f, in1 ? hi_of(u) : 0.f));
+                  w2 = pk(in0 ? lo_of(w2) : 0.f, in1 ? hi_of(w2) : 0.f);
+                } else {
+                  mins[n][i] = fma2(x[j][i], vm, mins[n][i]);
+                }
+                // the high term is w cut to 11 bits (exact in fp16), the low one the rest
+                const f2 high = w2 & 0xFFFFE000FFFFE000ull, rest = fma2(high, minus, w2);
+                // 16 tokens: two groups of 4 columns of high terms, two of low ones
+                uint32_t* d = &w[(jj >> 1) * 8 + (jj & 1) * 2 + i];
+                d[0] = pack_h2(lo_of(high), hi_of(high));
+                d[4] = pack_h2(lo_of(rest), hi_of(rest));
               }
-              // the high term is w cut to 11 bits (exact in fp16), the low one the rest
-              const f2 high = w2 & 0xFFFFE000FFFFE000ull, rest = fma2(high, minus, w2);
-              // 16 tokens: two groups of 4 columns of high terms, two of low ones
-              uint32_t* d = &w[i >> 1][(j >> 1) * 8 + (j & 1) * 2 + (i & 1)];
-              d[0] = pack_h2(lo_of(high), hi_of(high));
-              d[4] = pack_h2(lo_of(rest), hi_of(rest));
             }
+            tmem_st_frag(s_at + n * N + k * CH, w);
           }
-          tmem_st_frag(s_at + n * N, w[0]);
-          tmem_st_frag(s_at + (1u << 20) + n * N, w[1]);
-        }
       };
       if (cut)
         weights(std::true_type());
@@ -712,60 +710,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_before();
       mbar_arrive(&p_full[b2]);
       if (t > 0) flush(t - 1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) corr[i] = keep[i];
+      corr[0] = keep[0];
+      corr[1] = keep[1];
 #pragma unroll
       for (int n = 0; n < NG; ++n) fac[n] = fac_new[n];
     }
     if (nt > 0) flush(nt - 1);
-    // ---- sums over the quad's lanes and both halves' warps
-    float* xs = reinterpret_cast<float*>(smem + L::PRM);    // [halves][1 + NG][128]
-    named_barrier(2, 256);
-    float l[4], mn[NG][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      l[i] = lo_of(l2[i]) + hi_of(l2[i]);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      if (c == 0) xs[hc * (1 + NG) * 128 + row0 + 8 * i] = l[i];
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        mn[n][i] = lo_of(mins[n][i]) + hi_of(mins[n][i]);
-        mn[n][i] += __shfl_xor_sync(0xffffffffu, mn[n][i], 1);
-        mn[n][i] += __shfl_xor_sync(0xffffffffu, mn[n][i], 2);
-        if (c == 0) xs[(hc * (1 + NG) + 1 + n) * 128 + row0 + 8 * i] = mn[n][i];
-      }
-    }
-    named_barrier(2, 256);
+    // ---- sums over the quad's lanes, and out
     const bool whole = splits == 1;
     float* part = reinterpret_cast<float*>(parts + (size_t)blockIdx.x * kTcRows * (D + 2) * 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int row = row0 + 8 * i;
-      if (row >= rows) continue;
-      // in the order of the halves, so that both warps have the same sums
-      const float L0 = xs[row], L1 = xs[(1 + NG) * 128 + row], total = L0 + L1;
-      const int rr = tile * kTcRows + row;
-      const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
-      float* dst = whole ? a.out + ((s.row0 + tok) * a.h + hq) * D : part + row * D;
-      const float inv = !whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
+      float l = lo_of(l2[i]) + hi_of(l2[i]), mn[NG];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
 #pragma unroll
-      for (int j = 0; j < OP; j += 4) {         // 4 nibbles x 2 lanes' g: 8 channels in a row
-        const int at = hc * OW / 8 + j, ch = 64 * (at / 8) + 32 * (at % 8 / 4) + 8 * c;
-        const float* pm = xs + (1 + (64 * (at / 8) + 32 * (at % 8 / 4)) / G) * 128 + row;
-        const float mean = pm[0] + pm[(1 + NG) * 128];
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[k] = (lo_of(o[i >> 1][j + k][i & 1]) + mean) * inv;
-          v[4 + k] = (hi_of(o[i >> 1][j + k][i & 1]) + mean) * inv;
-        }
-        reinterpret_cast<float4*>(dst + ch)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst + ch)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      for (int n = 0; n < NG; ++n) {
+        mn[n] = lo_of(mins[n][i]) + hi_of(mins[n][i]);
+        mn[n] += __shfl_xor_sync(0xffffffffu, mn[n], 1);
+        mn[n] += __shfl_xor_sync(0xffffffffu, mn[n], 2);
       }
-      if (!whole && hc == 0 && c == 0) {
-        part[kTcRows * D + row] = m[i];
-        part[kTcRows * (D + 1) + row] = total;
+      if (row < rows) {
+        const int rr = tile * kTcRows + row;
+        const int tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
+        float* dst = (whole ? a.out + ((s.row0 + tok) * a.h + hq) * D : part + row * D) + 8 * c;
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int j = 0; j < OP; j += 4) {       // 4 nibbles x 2 lanes' g: 8 channels in a row
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] = (lo_of(o[j + k][i]) + mn[8 * j / G]) * inv;
+            v[4 + k] = (hi_of(o[j + k][i]) + mn[8 * j / G]) * inv;
+          }
+          reinterpret_cast<float4*>(dst + 8 * j)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(dst + 8 * j)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+        if (!whole && c == 0) {
+          part[kTcRows * D + row] = m[i];
+          part[kTcRows * (D + 1) + row] = l;
+        }
       }
     }
   }
