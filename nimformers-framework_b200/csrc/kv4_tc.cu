@@ -55,13 +55,27 @@ struct TcLayout {
 size_t part_bytes(int d) { return (size_t)kTcRows * (d + 2) * 4; }
 
 // ------------------------------------------------------------ PTX
-__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// Descriptors (smem_desc's) as their two halves: the upper one is a constant of
+// the operand, the lower one an address that offsets are added to.
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo) { return ((sbo >> 4) & 0x3FFFu) | 1u << 14; }
+__device__ __forceinline__ uint32_t desc_lo(const void* p, uint32_t lbo) {
+  return ((smem_addr(p) >> 4) & 0x3FFFu) | ((lbo >> 4) & 0x3FFFu) << 16;
+}
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a, uint32_t a_hi, uint32_t b,
+                                       uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}" ::"r"(
-          tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n"
+      " setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, {%7, %7, %7, %7}, p;\n}" ::"r"(tmem_d),
+      "r"(a), "r"(a_hi), "r"(b), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, {%6, %6, %6, %6}, p;\n}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
 }
 // 16 TMEM lanes x 8 columns a group: lane t holds columns 2 (t % 4), + 1 of row
@@ -267,35 +281,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------------------------------------------------------- MMA issue
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 12) {
+      // Everything an MMA is given is a constant away from warp-uniform values
+      // (the buffer is a template argument, TMEM's base went through a warp
+      // reduction): operands in per-thread registers cost six moves to uniform
+      // ones an MMA, and the issue then takes twice the MMAs' own time.
+      const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
       const uint32_t id_s = idesc_n(N), id_o = idesc_n(G);
-      const uint64_t dq = smem_desc(smem + L::Q, 128, SB_D);
-      const uint64_t dk = smem_desc(smem + L::K, 128, SB_D);
-      const uint64_t dv = smem_desc(smem + L::V, 128, SB_N);
+      const uint32_t dq0 = desc_lo(smem + L::Q, 128), dk0 = desc_lo(smem + L::K, 128), dv0 = desc_lo(smem + L::V, 128);
       auto warp_wait = [&](uint64_t* m, uint32_t parity) -> bool {
-        int ok = lane == 0 ? (int)wait(m, parity) : 0;
-        return __shfl_sync(0xffffffffu, ok, 0) != 0;
+        return __all_sync(0xffffffffu, wait(m, parity)) != 0;
       };
-      // S_x = q . k of tile t (x = t & 1)
-      auto scores = [&](int t) -> bool {
-        const int x = t & 1;
+      // S = q . k of tile t in buffer x = t & 1
+      auto scores = [&](auto buffer, int t) -> bool {
+        constexpr int x = decltype(buffer)::value;
         if (!warp_wait(&k_full[x], (t >> 1) & 1)) return false;
         tc_fence_after();
-        // rolled: the loops' code stays in the instruction cache beside softmax
-#pragma unroll 1
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t d = tmem + x * 128 + g * N;
-          uint64_t qd = dq + ((g * G / 8 * 128) >> 4), kd = dk + ((x * N * D * 2 + g * G / 8 * 128) >> 4);
-          uint32_t more = 0;
-#pragma unroll 1
-          for (int term = 0; term < 2; ++term) {
-#pragma unroll 2
-            for (int j = 0; j < G / 16; ++j) {
-              if (elect_one()) umma_f16_ss(d, qd + j * 16, kd + j * 16, id_s, more);
-              more = 1;
-            }
-            qd += (kTcRows * D * 2) >> 4;
-          }
-        }
+        uint32_t td = tm, dq = dq0, dk = dk0;   // opaque: not to be hoisted as 32 sums and spilled
+        asm volatile("" : "+r"(td), "+r"(dq), "+r"(dk));
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int term = 0; term < 2; ++term)
+#pragma unroll
+            for (int j = 0; j < G / 16; ++j)
+              if (elect_one())
+                mma_ss(td + (x * 128 + g * N), dq + ((term * kTcRows * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4),
+                       desc_hi(SB_D), dk + ((x * N * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4), desc_hi(SB_D),
+                       id_s, term + j > 0 ? 1u : 0u);
         if (elect_one()) {
           umma_commit(&s_full[x]);
           umma_commit(&k_empty[x]);
@@ -303,33 +315,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         return true;
       };
-      bool ok = warp_wait(q_full, 0);
-      if (ok && nt > 0) ok = scores(0);
-      if (ok && nt > 1) ok = scores(1);
-      for (int t = 0; ok && t < nt; ++t) {
-        const int x = t & 1, ph = (t >> 1) & 1;
-        ok = warp_wait(&v_full[x], ph) && warp_wait(&p_full[x], ph);
-        if (!ok) break;
+      auto values = [&](auto buffer, int t) -> bool {
+        constexpr int x = decltype(buffer)::value;
+        const uint32_t ph = (t >> 1) & 1;
+        if (!warp_wait(&v_full[x], ph) || !warp_wait(&p_full[x], ph)) return false;
         tc_fence_after();
-#pragma unroll 1
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t d = tmem + 256 + x * D + g * G, pa = tmem + x * 128 + g * N;
-          const uint64_t vd = dv + ((x * N * D * 2 + (g * G / 8) * SB_N) >> 4);
-          uint32_t more = 0;
-#pragma unroll 1
-          for (int j = 0; j < N / 16; ++j) {
-            if (elect_one()) umma_f16_ts(d, pa + j * 16, vd + j * 16, id_o, more);
-            if (elect_one()) umma_f16_ts(d, pa + j * 16 + 8, vd + j * 16, id_o, 1u);
-            more = 1;
-          }
-        }
+        uint32_t td = tm, dv = dv0;
+        asm volatile("" : "+r"(td), "+r"(dv));
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int j = 0; j < N / 16; ++j)
+#pragma unroll
+            for (int term = 0; term < 2; ++term)
+              if (elect_one())
+                mma_ts(td + (256 + x * D + g * G), td + (x * 128 + g * N + j * 16 + term * 8),
+                       dv + ((x * N * D * 2 + (g * G / 8) * SB_N + j * 256) >> 4), desc_hi(SB_N), id_o,
+                       term + j > 0 ? 1u : 0u);
         if (elect_one()) {
           umma_commit(&o_full[x]);
           umma_commit(&v_empty[x]);
         }
         __syncwarp();
         // the next scores of these columns wait until P there was used
-        if (t + 2 < nt) ok = warp_wait(&o_full[x], ph) && scores(t + 2);
+        return t + 2 >= nt || (warp_wait(&o_full[x], ph) && scores(buffer, t + 2));
+      };
+      const std::integral_constant<int, 0> even{};
+      const std::integral_constant<int, 1> odd{};
+      bool ok = warp_wait(q_full, 0);
+      if (ok && nt > 0) ok = scores(even, 0);
+      if (ok && nt > 1) ok = scores(odd, 1);
+      for (int t = 0; ok && t < nt; t += 2) {
+        ok = values(even, t);
+        if (ok && t + 1 < nt) ok = values(odd, t + 1);
       }
       if (elect_one()) umma_commit(all_done);
       __syncwarp();
@@ -342,19 +360,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t per = (uint32_t)a.bs / kTile;
     // The place of a token that moves on by N a tile: its block-table entry and
     // its tile within the block, kept without divisions.
+    // The entry is loaded a tile ahead: it has to be there to load the codes.
     struct Walk {
-      int tok;
+      int tok, blk;
       uint32_t page, rem;
     };
-    auto walk_at = [&](int tok) -> Walk {
-      const uint32_t tt = (uint32_t)tok / kTile;
-      return Walk{tok, tt / per, tt % per};
-    };
     const int32_t* row_of_table = a.table + (int64_t)b * a.width;
+    auto walk_at = [&](int tok) -> Walk {
+      const uint32_t tt = (uint32_t)tok / kTile, page = tt / per;
+      return Walk{tok, tok < seg_len ? row_of_table[page] : -1, page, tt - page * per};
+    };
     auto step = [&](Walk& w, bool report) -> const uint8_t* {
       const uint8_t* p = nullptr;
       if (w.tok < seg_len) {
-        const int blk = row_of_table[w.page];
+        const int blk = w.blk;
         if (blk >= 0 && blk < a.n_blocks)
           p = a.cache + (((int64_t)blk * a.hkv + kvh) * per + w.rem) * TB;
         else if (report && a.err)
@@ -366,6 +385,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         w.rem -= per;
         ++w.page;
       }
+      w.blk = w.tok < seg_len ? row_of_table[w.page] : -1;
       return p;
     };
     constexpr int KI = N * D / 32 / 128;        // 16-byte pieces of K rows a thread
@@ -413,6 +433,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     load_v();
     for (int t = 0; t < nt; ++t) {
       const int x = t & 1, slot = t % kPrmSlots;
+      // K: 8 channels of a token a 16-byte piece, in the order of Q's
+      if (t >= 2) ok = ok && slow_wait(&k_empty[x], ((t >> 1) - 1) & 1);
+      uint8_t* kd = smem + L::K + x * N * D * 2;
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int part = k_part + i * NG;
+        const uint32_t w4[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = part * 4 + q, c = m / NC, j = m % NC;
+          const uint32_t w = w4[q], w8 = w >> 8;
+          *reinterpret_cast<uint4*>(kd + (k_tok >> 3) * SB_D + (j * 4 + c) * 128 + (k_tok & 7) * 16) =
+              make_uint4(code_even(w), code_even(w8), code_odd(w), code_odd(w8));
+        }
+      }
+      fence_async_shared();
+      mbar_arrive(&k_full[x]);
       // The parameters' slot was last used four tiles ago; that tile's values
       // were found used up when V of the tile before last was written.
       // w = p s is brought to fp16's range by the largest s of the tile
@@ -431,23 +468,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       pp[258] = fmaf(8.f, vp.x, vp.y);
       if (pt % N == 0) fac[slot * 4 + pt / N] = pow2_field(e - 14);
       mbar_arrive(&prm_full[slot]);
-      // K: 8 channels of a token a 16-byte piece, in the order of Q's
-      if (t >= 2) ok = ok && slow_wait(&k_empty[x], ((t >> 1) - 1) & 1);
-      uint8_t* kd = smem + L::K + x * N * D * 2;
-#pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int part = k_part + i * NG;
-        const uint32_t w4[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = part * 4 + q, c = m / NC, j = m % NC;
-          const uint32_t w = w4[q], w8 = w >> 8;
-          *reinterpret_cast<uint4*>(kd + (k_tok >> 3) * SB_D + (j * 4 + c) * 128 + (k_tok & 7) * 16) =
-              make_uint4(code_even(w), code_even(w8), code_odd(w), code_odd(w8));
-        }
-      }
-      fence_async_shared();
-      mbar_arrive(&k_full[x]);
       load_k();                       // on its way through the wait for V's buffer
       // V: 8 tokens of a channel a 16-byte piece; row n = 64 s + 8 i + g is
       // channel 64 s + 32 (i / 4) + 4 g + i % 4
