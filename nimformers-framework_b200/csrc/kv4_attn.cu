@@ -39,7 +39,9 @@ __host__ __device__ constexpr int warps_of(int d) { return d <= 128 ? 8 : 6; }
 // beginning cuts first: u0 its first unit on the line, -1 for none.
 struct SegInfo {
   int64_t u0, u1;
-  int32_t b, kvh, tile;
+  int64_t row0;     // the sequence's first row
+  int32_t n;        // and its rows
+  int32_t kvh, tile;
   int32_t parts;    // join: CTAs that hold a part, counted from the one before
   int32_t second;   // join: the first of them holds it as its last segment
   int32_t pad;
@@ -140,31 +142,37 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
   griddep_wait();
 
   // ---- the line of units, and where this warp begins on it.  Every warp sums
-  // all sequences for itself, eight a lane: no barrier, one latency for 256.
+  // all sequences for itself: no barrier, one latency for 256 of them.
   auto tiles_of = [&](int n) { return n * a.r > a.big ? 0 : seq_tiles<ROWS>(n, a.r); };
   auto line_units = [&](int64_t b) -> int64_t {
     if (b >= a.n_seqs) return 0;
     const Seq s = seq_of(a, b);
     return (int64_t)seq_units(s.len) * tiles_of(s.n) * a.hkv;
   };
+  auto scan = [&](int64_t v) -> int64_t {   // inclusive, over the lanes
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, x);
+      if (lane >= x) v += u;
+    }
+    return v;
+  };
   const int64_t cta = blockIdx.x;
   SegInfo* info = reinterpret_cast<SegInfo*>(a.ws);
   float* parts = reinterpret_cast<float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
-  int64_t mine[8], total = 0, upto = 0;     // of the last 256 sequences summed
-  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) {
-    int64_t sum = 0;
+  int64_t total = 0, mine = 0, upto = 0;    // of the last 32 sequences scanned
+#pragma unroll 1
+  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
+    mine = line_units(b0 + lane);
+    if (b0 + 32 < a.n_seqs) {               // only sums are needed of all but the last ones
+      int64_t more = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mine[i] = line_units(b0 + lane * 8 + i);
-      sum += mine[i];
+      for (int i = 1; i < 8; ++i)
+        if (b0 + 32 * i < a.n_seqs) more += line_units(b0 + 32 * i + lane);
+      mine += more;
+      b0 += 32 * 7;
     }
-    upto = sum;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
-      if (lane >= x) upto += v;
-    }
-    upto += total;
+    upto = scan(mine) + total;
     total = __shfl_sync(0xffffffffu, upto, 31);
   }
   const int64_t ctas = max((int64_t)1, min((int64_t)gridDim.x, quot(total + W - 1, W)));
@@ -178,40 +186,24 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
   const int64_t w_a = cta_a + cut(warp, w_each, w_more), w_b = cta_a + cut(warp + 1, w_each, w_more);
   if (lane < 2) s_seg[warp][lane].u0 = -1;
   int64_t b = 0, off = 0;                   // the sequence of unit w_a, and the unit within it
-  for (int64_t b0 = a.n_seqs > 256 ? 0 : -1, base = 0; b0 < a.n_seqs; b0 += 256) {
-    if (b0 >= 0) {                          // more than 256 sequences: sum again up to w_a
-      int64_t sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mine[i] = line_units(b0 + lane * 8 + i);
-        sum += mine[i];
+  if (a.n_seqs > 1) {
+#pragma unroll 1
+    for (int64_t b0 = 0, base = 0; b0 < a.n_seqs; b0 += 32) {
+      if (a.n_seqs > 32) {                  // otherwise they are still there
+        mine = line_units(b0 + lane);
+        upto = scan(mine) + base;
+        base = __shfl_sync(0xffffffffu, upto, 31);
       }
-      upto = sum;
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
-        if (lane >= x) upto += v;
-      }
-      upto += base;
-      base = __shfl_sync(0xffffffffu, upto, 31);
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, upto > w_a);
-    if (!past) continue;
-    const int who = __ffs(past) - 1;
-    int64_t from = upto;
-    int at = 0;
-#pragma unroll
-    for (int i = 7; i >= 0; --i) {          // the last of this lane's that begins at or before w_a
-      const int64_t end = from;
-      from -= mine[i];
-      if (from <= w_a && w_a < end) {
-        at = i;
-        off = w_a - from;
+      const unsigned past = __ballot_sync(0xffffffffu, upto > w_a);
+      if (past) {
+        const int who = __ffs(past) - 1;
+        b = b0 + who;
+        off = w_a - __shfl_sync(0xffffffffu, upto - mine, who);
+        break;
       }
     }
-    b = __shfl_sync(0xffffffffu, max(b0, (int64_t)0) + lane * 8 + at, who);
-    off = __shfl_sync(0xffffffffu, off, who);
-    break;
+  } else {
+    off = w_a;
   }
   if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
     const Seq s = seq_of(a, b);
@@ -220,7 +212,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
     SegInfo si;
     si.u0 = cta_a - (off - seg * nu);
     si.u1 = si.u0 + nu;
-    si.b = (int32_t)b;
+    si.row0 = s.row0;
+    si.n = s.n;
     si.kvh = (int32_t)quot(seg, tiles);
     si.tile = (int32_t)(seg - (int64_t)si.kvh * tiles);
     const int64_t before = cut(cta - 1, each, more);
@@ -610,7 +603,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
       SegInfo& si = s_seg[warp][k];
       si.u0 = u0;
       si.u1 = u0 + nu;
-      si.b = (int32_t)b;
+      si.row0 = s.row0;
+      si.n = s.n;
       si.kvh = kvh;
       si.tile = tile;
     }
@@ -637,23 +631,39 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
     const unsigned later = todo & (todo - 1);
     const unsigned members = used & ~((1u << i0) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : ~0u);
     const SegInfo si = s_seg[i0 >> 1][i0 & 1];
-    const Seq s = seq_of(a, si.b);
     const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
     float* slot = parts + (size_t)(2 * cta + (si.u0 <= cta_a ? 0 : 1)) * PF;
-    const int rows = min(ROWS, s.n * a.r - si.tile * ROWS);
+    const int rows = min(ROWS, si.n * a.r - si.tile * ROWS);
     for (int row = 0; row < rows; ++row, ++task) {
       if (task % W != warp) continue;
+      // the members' maxima and sums, a lane each; then their outputs
       Merged<V> all;
+      const bool in = members >> lane & 1u;
+      const float* mine_p = piece_at(in ? lane : i0);
+      const float pm = in ? mine_p[ROWS * D + row] : -INFINITY;
+      float top = pm;
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top = __shfl_sync(0xffffffffu, top, 0);
+      const float f = ex2(pm - (top == -INFINITY ? 0.f : top));
+      float pl = in ? mine_p[ROWS * D + ROWS + row] * f : 0.f;
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, x);
+      all.m = top;
+      all.l = __shfl_sync(0xffffffffu, pl, 0);
+#pragma unroll 1
       for (unsigned rest = members; rest; rest &= rest - 1) {
-        const float* p = piece_at(__ffs(rest) - 1);
+        const int who = __ffs(rest) - 1;
         float po[V];
-        load_v<V>(p + row * D + lane * V, po);
-        all.take(p[ROWS * D + row], p[ROWS * D + ROWS + row], po);
+        load_v<V>(piece_at(who) + row * D + lane * V, po);
+        const float w = __shfl_sync(0xffffffffu, f, who);
+#pragma unroll
+        for (int x = 0; x < V; ++x) all.o[x] = fmaf(w, po[x], all.o[x]);
       }
       if (whole) {
         const int rr = si.tile * ROWS + row, tok = (int)((uint32_t)rr / (uint32_t)a.r);
         const int hq = si.kvh * a.r + rr - tok * a.r;
-        store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
+        store_v<V>(a.out + ((si.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
       } else {
         store_v<V>(slot + row * D + lane * V, all.o, 1.f);
         if (lane == 0) {
@@ -682,8 +692,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
   const SegInfo si = reinterpret_cast<const SegInfo*>(a.ws)[cta];
   const float* parts = reinterpret_cast<const float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
   if (si.u0 < 0) return;
-  const Seq s = seq_of(a, si.b);
-  const int rows = min(ROWS, s.n * a.r - si.tile * ROWS);
+  const int rows = min(ROWS, si.n * a.r - si.tile * ROWS);
   const int groups = rows == 1 ? kJoinWarps : rows == 2 ? kJoinWarps / 2 : kJoinWarps / (rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
   const int row = warp / groups, grp = warp - row * groups;
   Merged<V> all;
@@ -719,7 +728,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
   }
   const int rr = si.tile * ROWS + row, tok = (int)((uint32_t)rr / (uint32_t)a.r);
   const int hq = si.kvh * a.r + rr - tok * a.r;
-  store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
+  store_v<V>(a.out + ((si.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
 }
 
 int grid_of(int d, int nb) {
@@ -738,10 +747,11 @@ int run_nb(const Args& a, cudaStream_t st) {
 
 // 4 rows a segment where no sequence should have more of them for a KV head,
 // 8 or 16 where one may: each pass over a sequence's tiles serves more rows,
-// at more registers and partial results.
+// at more registers and partial results.  Beside sequences of many rows, which
+// go elsewhere, the others are taken for decoding ones with one row a head.
 template <int D, int NG>
 int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
-  const int64_t rows = std::min<int64_t>(max_new * a.r, a.big);
+  const int64_t rows = a.big < INT32_MAX ? a.r : max_new * a.r;
   if (rows <= 4) return run_nb<D, NG, 1>(a, st);
   if constexpr (D <= 128)
     if (rows > 8) return run_nb<D, NG, 4>(a, st);

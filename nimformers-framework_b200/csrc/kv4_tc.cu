@@ -8,9 +8,10 @@
 //   x_j = sum_g S_g s_gj + (m_gj + 8 s_gj) sum_g(q)
 //   O_g += [wh | wl] . (c - 8),  w_j = p_j s_gj    in two fp16 terms from TMEM
 // so each product runs twice, which is what float32's accuracy costs here; the
-// floor is twice the plain flops at the tensor rate.  An output tile's sums
-// run in TMEM over one tile of tokens only and are added to float32 registers
-// between, so that the tensor core's cut-off additions stay few.
+// floor is twice the plain flops at the tensor rate.  The tensor core cuts what
+// an addition shifts out, always towards zero: so the low terms are summed first,
+// while the sum is small, and an output tile's sums run in TMEM over one tile of
+// tokens only and are added to float32 registers between.
 //
 // Roles: eight softmax warps of 16 rows; four warps that unpack codes into the K
 // and V operands (two buffers each); one warp that issues the MMAs.  S and O have
@@ -301,13 +302,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-          for (int term = 0; term < 2; ++term)
+          for (int term = 1; term >= 0; --term)
 #pragma unroll
             for (int j = 0; j < G / 16; ++j)
               if (elect_one())
                 mma_ss(td + (x * 128 + g * N), dq + ((term * kTcRows * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4),
                        desc_hi(SB_D), dk + ((x * N * D * 2 + (g * G / 8 + 2 * j) * 128) >> 4), desc_hi(SB_D),
-                       id_s, term + j > 0 ? 1u : 0u);
+                       id_s, term == 0 || j > 0 ? 1u : 0u);
         if (elect_one()) {
           umma_commit(&s_full[x]);
           umma_commit(&k_empty[x]);
@@ -325,13 +326,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-          for (int j = 0; j < N / 16; ++j)
+          for (int term = 1; term >= 0; --term)
 #pragma unroll
-            for (int term = 0; term < 2; ++term)
+            for (int j = 0; j < N / 16; ++j)
               if (elect_one())
                 mma_ts(td + (256 + x * D + g * G), td + (x * 128 + g * N + j * 16 + term * 8),
                        dv + ((x * N * D * 2 + (g * G / 8) * SB_N + j * 256) >> 4), desc_hi(SB_N), id_o,
-                       term + j > 0 ? 1u : 0u);
+                       term == 0 || j > 0 ? 1u : 0u);
         if (elect_one()) {
           umma_commit(&o_full[x]);
           umma_commit(&v_empty[x]);
