@@ -7,11 +7,14 @@
 // The largest entry's own 1 stays out of s, so a row that is all but certain
 // keeps the small probabilities that make up its entropy.
 //
-// The logits are read once: a cluster of CTAs holds one row in shared memory
-// (bulk copies), and the passes over it (maxima, sums, candidates) stay there.
-// The n-th largest of the threads' maxima is a lower bound of the row's n-th
-// largest entry that few other entries reach, so the alternatives are chosen
-// among little more than n candidates.
+// The logits are read once from HBM: a thread streams its share with a running
+// maximum and sums (four float4 loads ahead of their use), a CTA takes a row, a
+// cluster of CTAs shares one where rows are few or long.  The n-th largest of the
+// threads' maxima is a lower bound of the row's n-th largest entry that few other
+// entries reach, so the alternatives are chosen among little more than n
+// candidates, for which the threads that reach the bound read their shares again
+// (out of L2).  Bounded by HBM; a slice kept in shared memory instead cost 64 KB
+// a CTA, loads and passes took turns, and 4,096 rows of 32,000 took 230 us.
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -20,14 +23,19 @@ namespace nimf {
 namespace {
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
-constexpr int kLpChunks = 4;      // bulk copies (and barriers) per slice
+constexpr int kLpAhead = 4;       // float4s of a thread in flight
 constexpr int kLpMaxTop = 32;
 constexpr int kLpCand = 1024;     // candidates kept before the slow path
 constexpr int kLpMaxCluster = 8;
 
+// Entries seen, relative to a reference r >= all of them: top = e^(max - r), the
+// sum s of all other terms and z of all (x - r) e^(x - r).  Whatever is added,
+// the smaller of two tops joins s and the larger stays out of it, so at the end,
+// where r is the maximum and top is 1, s holds exactly the other entries.  z is
+// NaN once a NaN or +inf was seen.
 struct LpPart {
-  float m, s, z;                  // of one CTA's slice; s without the slice's maximum
-  int nan, above;                 // a NaN in the slice; entries above the given logit
+  float r, top, s, z;
+  int above;                      // entries above the given logit
 };
 
 struct LpArgs {
@@ -55,6 +63,39 @@ __device__ __forceinline__ float exp_term(float& t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t * 1.44269504f));
   return e;
+}
+
+// Moves the reference up to r (r = -inf: nothing seen, all sums are 0).
+__device__ __forceinline__ void lp_raise(LpPart& a, float r) {
+  if (r == a.r) return;
+  if (a.r > -INFINITY) {
+    float d = a.r - r;
+    const float f = exp_term(d);
+    a.z = f * fmaf(d, a.s + a.top, a.z);
+    a.s *= f;
+    a.top *= f;
+  }
+  a.r = r;
+}
+__device__ __forceinline__ void lp_add(LpPart& a, float top, float s, float z) {
+  a.s += s + fminf(a.top, top);
+  a.top = fmaxf(a.top, top);
+  a.z += z;
+}
+
+// The parts of disjoint sets, in their order.
+__device__ __forceinline__ LpPart lp_join(const LpPart* p, int n) {
+  float r = p[0].r;
+  for (int i = 1; i < n; ++i) r = fmaxf(r, p[i].r);
+  LpPart all = p[0];
+  lp_raise(all, r);
+  for (int i = 1; i < n; ++i) {
+    LpPart b = p[i];
+    lp_raise(b, r);
+    lp_add(all, b.top, b.s, b.z);
+    all.above += b.above;
+  }
+  return all;
 }
 
 // Falling order over the warp's lanes of one float each.
@@ -96,15 +137,39 @@ __device__ __forceinline__ bool before(float v, int i, float w, int j) {
   return v > w || (v == w && i < j);
 }
 
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
-  extern __shared__ __align__(128) float buf[];
-  __shared__ uint64_t bar[kLpChunks];
-  __shared__ float s_f[kLpWarps * 3];
+// A slice of a row as float4s: entry i is element i + pad of them.
+struct LpSlice {
+  const float* x;                 // 16-byte aligned: pad entries before the slice
+  int pad, cnt, nf;
+  __device__ __forceinline__ float4 load_whole(int f) const {
+    float4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "l"(x + 4 * (int64_t)f));
+    return v;
+  }
+  __device__ __forceinline__ float4 load(int f) const {
+    const int i = 4 * f - pad;
+    if (i >= 0 && i + 4 <= cnt) return load_whole(f);
+    float4 v;                     // an end of the slice, or nothing
+    const float* p = x + 4 * (int64_t)f;
+    v.x = i >= 0 && i < cnt ? p[0] : -INFINITY;
+    v.y = i + 1 >= 0 && i + 1 < cnt ? p[1] : -INFINITY;
+    v.z = i + 2 >= 0 && i + 2 < cnt ? p[2] : -INFINITY;
+    v.w = i + 3 >= 0 && i + 3 < cnt ? p[3] : -INFINITY;
+    return v;
+  }
+};
+
+__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a) {
+  __shared__ LpPart s_part[kLpWarps];
+  __shared__ float s_f[kLpWarps];
   __shared__ int s_i[kLpWarps];
   __shared__ float s_sort[kLpWarps][32];
   __shared__ float c_v[kLpCand];
   __shared__ int c_i[kLpCand];
-  __shared__ int c_n;
+  __shared__ int c_n, s_n;
+  __shared__ int s_who[kLpThreads];                // threads whose share holds candidates
   __shared__ LpPart part[kLpMaxCluster];           // in the first CTA
   __shared__ float list_v[kLpMaxCluster * kLpMaxTop];
   __shared__ int list_i[kLpMaxCluster * kLpMaxTop];
@@ -114,169 +179,126 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   const unsigned rank = kv4::cluster_rank(), ctas = kv4::cluster_size();
   const int64_t row = blockIdx.x / ctas;
   const int64_t lo = (int64_t)rank * a.slice;
-  const int cnt = (int)max((int64_t)0, min((int64_t)a.slice, a.vocab - lo));
+  LpSlice sl;
+  sl.cnt = (int)max((int64_t)0, min((int64_t)a.slice, a.vocab - lo));
   griddep_launch_dependents();
   if (ctas > 1) kv4::cluster_arrive();             // met below, before remote stores
-  if (tid == 0) {
-    for (int i = 0; i < kLpChunks; ++i) mbar_init(&bar[i], 1);
-    mbar_fence_init();
-    c_n = 0;
-  }
-  __syncthreads();
+  if (tid == 0) c_n = s_n = 0;
   griddep_wait();
-
-  // ---- the slice into shared memory, entry i at buf[pad + i]; the aligned
-  // middle in bulk copies, the ends with plain loads, -inf around them
   const float* x = a.x + row * a.vocab + lo;
-  const int pad = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-  const int nf = (pad + cnt + 3) >> 2;             // float4s that hold entries
-  const int mid0 = pad ? 1 : 0, mid1 = (pad + cnt) >> 2;   // whole ones
-  const int per = ((nf + kLpChunks - 1) / kLpChunks + kLpThreads - 1) / kLpThreads * kLpThreads;
-  if (tid == 0) {
-    for (int i = 0; i < kLpChunks; ++i) {
-      const int f0 = max(mid0, i * per), f1 = min(mid1, (i + 1) * per);
-      const uint32_t bytes = f1 > f0 ? (uint32_t)(f1 - f0) * 16u : 0u;
-      mbar_arrive_expect_tx(&bar[i], bytes);
-      if (bytes) bulk_g2s(buf + 4 * f0, x + (4 * f0 - pad), bytes, &bar[i]);
-    }
-  }
-  if (tid < 8) {
-    // the first float4 if it is not whole, and the last one
-    const int f = tid < 4 ? 0 : mid1;
-    const bool mine = tid < 4 ? (mid0 == 1 || mid1 == 0) && nf > 0 : mid1 > 0 && mid1 < nf;
-    if (mine) {
-      const int i = 4 * f + (tid & 3) - pad;
-      buf[4 * f + (tid & 3)] = i >= 0 && i < cnt ? x[i] : -INFINITY;
-    }
-  }
+  sl.pad = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
+  sl.x = x - sl.pad;
+  sl.nf = (sl.pad + sl.cnt + 3) >> 2;
+  const int cnt = sl.cnt, pad = sl.pad, nf = sl.nf;
   const int64_t id = a.ids ? (int64_t)a.ids[row] : -1;
   const bool id_ok = id >= 0 && id < a.vocab;
   const float given = id_ok ? a.x[row * a.vocab + id] : INFINITY;
-  __syncthreads();
 
-  // ---- maxima, and the entries above the given one
-  const float4* b4 = reinterpret_cast<const float4*>(buf);
-  float tm = -INFINITY;
-  int above = 0;
-  bool ok = true;
-  for (int i = 0; i < kLpChunks; ++i) {
-    ok = ok && mbar_wait_t<0>(&bar[i], 0);
-    const int f1 = min(nf, (i + 1) * per);
-    for (int f = i * per + tid; f < f1; f += kLpThreads) {
-      const float4 v = b4[f];
-      tm = fmaxf(fmaxf(tm, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
-      above += (v.x > given) + (v.y > given) + (v.z > given) + (v.w > given);
-    }
-  }
-  if (!ok && a.err) atomicExch(a.err, 6);
-  float m = tm;
+  // ---- one pass: maximum, sums, entries above the given one
+  LpPart me = {-INFINITY, 0.f, 0.f, 0.f, 0};
+  float tm = -INFINITY;                            // this thread's largest entry
+  {
+    constexpr int kRound = kLpAhead * kLpThreads;  // float4s of a round of the CTA
+    const int whole = (pad + cnt) >> 2;            // those before are full, but for the first
+    auto fetch = [&](int f0, float4 (&v)[kLpAhead]) {
+      if (f0 + kRound <= whole && (f0 > 0 || pad == 0)) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    above += __shfl_xor_sync(0xffffffffu, above, o);
-  }
-  if (lane == 0) {
-    s_f[warp] = m;
-    s_i[warp] = above;
-  }
-  __syncthreads();
-  m = s_f[0];
-  above = s_i[0];
-  for (int i = 1; i < kLpWarps; ++i) {
-    m = fmaxf(m, s_f[i]);
-    above += s_i[i];
-  }
-  __syncthreads();
-
-  // ---- sums; only a thread that holds the maximum has to look for it
-  float s = 0.f, z = 0.f;
-  int at_max = 0, nan = 0;
-  if (m == -INFINITY) {
-    for (int f = tid; f < nf; f += kLpThreads) {
-      const float4 v = b4[f];
-      nan |= v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
-    }
-  } else if (tm == m) {
-    for (int f = tid; f < nf; f += kLpThreads) {
-      const float4 v = b4[f];
-      const float e4[4] = {v.x, v.y, v.z, v.w};
-      for (int e = 0; e < 4; ++e) {
-        if (e4[e] == m) {
-          ++at_max;
-          if (m == INFINITY) s = __int_as_float(0x7fffffff);
-        } else {
-          float t = e4[e] - m;
-          const float w = exp_term(t);
-          s += w;
-          z = fmaf(t, w, z);
-        }
+        for (int k = 0; k < kLpAhead; ++k) v[k] = sl.load_whole(f0 + tid + k * kLpThreads);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kLpAhead; ++k) v[k] = sl.load(f0 + tid + k * kLpThreads);
+      }
+    };
+    auto take = [&](const float4 (&v)[kLpAhead]) {
+      float e[4 * kLpAhead];
+#pragma unroll
+      for (int k = 0; k < kLpAhead; ++k) {
+        e[4 * k] = v[k].x;
+        e[4 * k + 1] = v[k].y;
+        e[4 * k + 2] = v[k].z;
+        e[4 * k + 3] = v[k].w;
+      }
+      float most = e[0];
+#pragma unroll
+      for (int k = 0; k < 4 * kLpAhead; ++k) {
+        most = fmaxf(most, e[k]);                  // a NaN has no say
+        me.above += e[k] > given;
+      }
+      tm = fmaxf(tm, most);
+      // one reference a warp: no lane leaves the common path
+      float all;
+      asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(most));
+      if (all > me.r) lp_raise(me, all);
+      const float ref = me.r == -INFINITY ? 0.f : me.r;
+      float s1 = 0.f, z1 = 0.f, top1 = 0.f;        // a second chain
+#pragma unroll
+      for (int k = 0; k < 4 * kLpAhead; ++k) {
+        float t = e[k] - ref;
+        const float w = exp_term(t);
+        float& top = k & 1 ? top1 : me.top;
+        (k & 1 ? s1 : me.s) += fminf(top, w);
+        top = fmaxf(top, w);
+        float& z = k & 1 ? z1 : me.z;
+        z = fmaf(t, w, z);
+      }
+      lp_add(me, top1, s1, z1);
+    };
+    // two rounds' registers in turn
+    float4 va[kLpAhead], vb[kLpAhead];
+    fetch(0, va);
+#pragma unroll 1
+    for (int f0 = 0; f0 < nf; f0 += 2 * kRound) {
+      if (f0 + kRound < nf) fetch(f0 + kRound, vb);
+      take(va);
+      if (f0 + kRound < nf) {
+        if (f0 + 2 * kRound < nf) fetch(f0 + 2 * kRound, va);
+        take(vb);
       }
     }
-  } else {
-    float s1 = 0.f, z1 = 0.f;
-    for (int f = tid; f < nf; f += kLpThreads) {
-      const float4 v = b4[f];
-      float t0 = v.x - m, t1 = v.y - m, t2 = v.z - m, t3 = v.w - m;
-      const float w0 = exp_term(t0), w1 = exp_term(t1), w2 = exp_term(t2), w3 = exp_term(t3);
-      s += w0 + w1;
-      s1 += w2 + w3;
-      z = fmaf(t0, w0, fmaf(t1, w1, z));
-      z1 = fmaf(t2, w2, fmaf(t3, w3, z1));
-    }
-    s += s1;
-    z += z1;
   }
+  LpPart mine = me;                                // the lanes have one reference
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    z += __shfl_xor_sync(0xffffffffu, z, o);
-    nan |= __shfl_xor_sync(0xffffffffu, nan, o);
+    lp_add(mine, __shfl_xor_sync(0xffffffffu, mine.top, o), __shfl_xor_sync(0xffffffffu, mine.s, o),
+           __shfl_xor_sync(0xffffffffu, mine.z, o));
+    mine.above += __shfl_xor_sync(0xffffffffu, mine.above, o);
   }
-  // every entry equal to the maximum counts 1, but for the first one
-  const unsigned holders = __ballot_sync(0xffffffffu, at_max > 0);
-  const bool first_holder = holders && lane == __ffs(holders) - 1;
-  if (lane == 0) s_i[warp] = holders != 0;
+  if (lane == 0) s_part[warp] = mine;
   __syncthreads();
-  bool earlier = false;
-  for (int i = 0; i < warp; ++i) earlier |= s_i[i] != 0;
-  s += (float)(at_max - (first_holder && !earlier ? 1 : 0));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) {
-    s_f[warp] = s;
-    s_f[kLpWarps + warp] = z;
-    s_f[2 * kLpWarps + warp] = nan ? 1.f : 0.f;
-  }
-  __syncthreads();
-  LpPart mine = {m, 0.f, 0.f, 0, above};
-  for (int i = 0; i < kLpWarps; ++i) {
-    mine.s += s_f[i];
-    mine.z += s_f[kLpWarps + i];
-    mine.nan |= s_f[2 * kLpWarps + i] != 0.f;
-  }
+  mine = lp_join(s_part, kLpWarps);
 
   // ---- the slice's alternatives
   const int top = a.top;
   if (top > 0) {
     // the top-th largest of the threads' maxima
-    float v = warp_sort(tm);
-    for (int half = kLpWarps / 2; half > 0; half >>= 1) {
-      if (warp >= half && warp < 2 * half) s_sort[warp][lane] = v;
+    float bound;
+    if (top == 1) {
+      bound = mine.r;                              // the slice's maximum
+    } else {
+      float v = warp_sort(tm);
+      for (int half = kLpWarps / 2; half > 0; half >>= 1) {
+        if (warp >= half && warp < 2 * half) s_sort[warp][lane] = v;
+        __syncthreads();
+        if (warp < half) v = warp_merge(v, s_sort[warp + half][31 - lane]);
+      }
+      if (warp == 0) s_sort[0][lane] = v;
       __syncthreads();
-      if (warp < half) v = warp_merge(v, s_sort[warp + half][31 - lane]);
+      bound = s_sort[0][top - 1];
     }
-    if (warp == 0) s_sort[0][lane] = v;
+    // the threads that reach it, and their shares again, a warp a share
+    if (tm >= bound && tm > -INFINITY) s_who[atomicAdd(&s_n, 1)] = tid;
     __syncthreads();
-    const float bound = s_sort[0][top - 1];
-    if (tm >= bound && tm > -INFINITY)
-      for (int f = tid; f < nf; f += kLpThreads) {
-        const float4 v4 = b4[f];
+    for (int k = warp; k < s_n; k += kLpWarps)
+      for (int f = s_who[k] + lane * kLpThreads; f < nf; f += 32 * kLpThreads) {
+        const float4 v4 = sl.load(f);
         const float e4[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
         for (int e = 0; e < 4; ++e)
           if (e4[e] >= bound && e4[e] > -INFINITY) {
-            const int k = atomicAdd(&c_n, 1);
-            if (k < kLpCand) {
-              c_v[k] = e4[e];
-              c_i[k] = 4 * f + e - pad;
+            const int at = atomicAdd(&c_n, 1);
+            if (at < kLpCand) {
+              c_v[at] = e4[e];
+              c_i[at] = 4 * f + e - pad;
             }
           }
       }
@@ -298,7 +320,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
       if (n < want && warp == 0) {
         for (int i0 = 0; n < want && i0 < cnt; i0 += 32) {
           const int i = i0 + lane;
-          const bool rest = i < cnt && !(buf[pad + i] > -INFINITY);
+          const bool rest = i < cnt && !(x[i] > -INFINITY);
           const unsigned who = __ballot_sync(0xffffffffu, rest);
           const int r = n + __popc(who & ((1u << lane) - 1u));
           if (rest && r < want) {
@@ -317,7 +339,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
         float bv = -INFINITY;
         int bi = INT32_MAX;
         for (int f = tid; f < nf; f += kLpThreads) {
-          const float4 v4 = b4[f];
+          const float4 v4 = sl.load(f);
           const float e4[4] = {v4.x, v4.y, v4.z, v4.w};
           for (int e = 0; e < 4; ++e) {
             const int i = 4 * f + e - pad;
@@ -364,8 +386,8 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   if (ctas > 1) {
     kv4::cluster_wait();
     if (tid < 5) {
-      const uint32_t w[5] = {__float_as_uint(mine.m), __float_as_uint(mine.s), __float_as_uint(mine.z),
-                             (uint32_t)mine.nan, (uint32_t)mine.above};
+      const uint32_t w[5] = {__float_as_uint(mine.r), __float_as_uint(mine.top), __float_as_uint(mine.s),
+                             __float_as_uint(mine.z), (uint32_t)mine.above};
       st_remote(remote_smem(&part[rank], 0) + tid * 4, w[tid]);
     }
     if (tid < top) {
@@ -378,26 +400,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
     kv4::cluster_wait();
     if (rank != 0) return;
     // sums over the slices, in their order
-    float M = -INFINITY;
-    int who = -1;
-    for (unsigned i = 0; i < ctas; ++i) {
-      if (part[i].m > M) {
-        M = part[i].m;
-        who = (int)i;
-      }
-    }
-    LpPart all = {M, 0.f, 0.f, 0, 0};
-    for (unsigned i = 0; i < ctas; ++i) {
-      all.nan |= part[i].nan;
-      all.above += part[i].above;
-      if (part[i].m == -INFINITY) continue;
-      float d = part[i].m - M;
-      const float d0 = d, f = (int)i == who ? 1.f : exp_term(d);
-      const float tot = 1.f + part[i].s;
-      all.s += (int)i == who ? part[i].s : f * tot;
-      all.z += (int)i == who ? part[i].z : f * fmaf(max_nan(d0, -128.f), tot, part[i].z);
-    }
-    mine = all;
+    mine = lp_join(part, (int)ctas);
     const int n = (int)ctas * top;
     for (int i = tid; i < n; i += kLpThreads) {
       const float w = list_v[i];
@@ -414,19 +417,16 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   }
 
   const float nanf_ = __int_as_float(0x7fffffff);
-  const bool empty = mine.m == -INFINITY;          // nothing is possible
+  const bool bad = mine.z != mine.z, empty = mine.r == -INFINITY;  // NaN or +inf; nothing is possible
   const float log_s = log1pf(mine.s);
-  auto lp = [&](float w) -> float {
-    if (mine.nan) return nanf_;
-    return empty ? -INFINITY : (w - mine.m) - log_s;
-  };
+  auto lp = [&](float w) -> float { return bad ? nanf_ : empty ? -INFINITY : (w - mine.r) - log_s; };
   if (tid < top) {
     a.top_ids[row * top + tid] = t_i[tid];
     a.top_lp[row * top + tid] = lp(t_v[tid]);
   }
   if (tid == 0) {
-    if (a.logprob) a.logprob[row] = id_ok ? lp(given) : mine.nan || mine.s != mine.s ? nanf_ : -INFINITY;
-    if (a.entropy) a.entropy[row] = mine.nan ? nanf_ : empty ? 0.f : log_s - mine.z / (1.f + mine.s);
+    if (a.logprob) a.logprob[row] = id_ok ? lp(given) : bad ? nanf_ : -INFINITY;
+    if (a.entropy) a.entropy[row] = bad ? nanf_ : empty ? 0.f : log_s - mine.z / (1.f + mine.s);
     if (a.rank) a.rank[row] = id_ok ? mine.above + 1 : 0;
   }
 }
@@ -450,12 +450,11 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   if (!logits || ((logprob || rank) && !ids) || (n_top > 0 && (!top_ids || !top_logprobs)))
     return set_error(NIMF_ERR_ARG, "logprobs: NULL buffer");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  // As many CTAs a row as bring its slice to 16,384 entries (three CTAs to an
-  // SM then), more where few rows would leave SMs without work.
+  // A CTA a row; several where the rows do not fill the SMs twice over, as long
+  // as a thread keeps four float4s, and for rows that a CTA would stream alone
+  // for long after the others.
   unsigned ctas = 1;
-  while (ctas < (unsigned)kLpMaxCluster &&
-         ((vocab + ctas - 1) / ctas > 16384 ||
-          (rows * ctas < ctx()->num_sms && vocab / ctas > 4 * kLpThreads)))
+  while (ctas < (unsigned)kLpMaxCluster && rows * ctas < 2 * ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
     ctas *= 2;
   LpArgs a = {};
   a.x = logits;
@@ -469,7 +468,5 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   a.vocab = vocab;
   a.slice = (int)(((vocab + ctas - 1) / ctas + 3) & ~(int64_t)3);
   a.top = (int)n_top;
-  const size_t smem = (size_t)(a.slice + 8) * 4;
-  NIMF_TRY(kv4::allow_smem((const void*)logprobs_kernel, 160 * 1024));
-  return kv4::launch(logprobs_kernel, dim3((unsigned)(rows * ctas)), kLpThreads, smem, st, ctas, a);
+  return kv4::launch(logprobs_kernel, dim3((unsigned)(rows * ctas)), kLpThreads, 0, st, ctas, a);
 }
