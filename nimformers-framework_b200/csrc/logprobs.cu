@@ -161,18 +161,30 @@ struct LpSlice {
   }
 };
 
+// How many of n entries (rounded up to four; what is there counts) come before (w, wi).
+__device__ __forceinline__ int rank_of(const float* v, const int* i, int n, float w, int wi) {
+  int r = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 4) {
+    const float4 a = *reinterpret_cast<const float4*>(v + j);
+    const int4 b = *reinterpret_cast<const int4*>(i + j);
+    r += before(a.x, b.x, w, wi) + before(a.y, b.y, w, wi) + before(a.z, b.z, w, wi) + before(a.w, b.w, w, wi);
+  }
+  return r;
+}
+
 __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a) {
   __shared__ LpPart s_part[kLpWarps];
   __shared__ float s_f[kLpWarps];
   __shared__ int s_i[kLpWarps];
   __shared__ float s_sort[kLpWarps][32];
-  __shared__ float c_v[kLpCand];
-  __shared__ int c_i[kLpCand];
+  __shared__ __align__(16) float c_v[kLpCand];
+  __shared__ __align__(16) int c_i[kLpCand];
   __shared__ int c_n, s_n;
   __shared__ int s_who[kLpThreads];                // threads whose share holds candidates
   __shared__ LpPart part[kLpMaxCluster];           // in the first CTA
-  __shared__ float list_v[kLpMaxCluster * kLpMaxTop];
-  __shared__ int list_i[kLpMaxCluster * kLpMaxTop];
+  __shared__ __align__(16) float list_v[kLpMaxCluster * kLpMaxTop];
+  __shared__ __align__(16) int list_i[kLpMaxCluster * kLpMaxTop];
   __shared__ float t_v[kLpMaxTop];                 // this CTA's alternatives
   __shared__ int t_i[kLpMaxTop];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -288,20 +300,34 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a)
     // the threads that reach it, and their shares again, a warp a share
     if (tm >= bound && tm > -INFINITY) s_who[atomicAdd(&s_n, 1)] = tid;
     __syncthreads();
-    for (int k = warp; k < s_n; k += kLpWarps)
-      for (int f = s_who[k] + lane * kLpThreads; f < nf; f += 32 * kLpThreads) {
-        const float4 v4 = sl.load(f);
-        const float e4[4] = {v4.x, v4.y, v4.z, v4.w};
+    for (int k = warp; k < s_n; k += 4 * kLpWarps)
+      for (int f0 = lane * kLpThreads; f0 - lane * kLpThreads < nf; f0 += 32 * kLpThreads) {
+        float4 v[4];                               // of four shares
+        int f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e4[e] >= bound && e4[e] > -INFINITY) {
-            const int at = atomicAdd(&c_n, 1);
-            if (at < kLpCand) {
-              c_v[at] = e4[e];
-              c_i[at] = 4 * f + e - pad;
+        for (int q = 0; q < 4; ++q) {
+          f[q] = k + q * kLpWarps < s_n ? f0 + s_who[k + q * kLpWarps] : nf;
+          v[q] = sl.load(f[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float e4[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e4[e] >= bound && e4[e] > -INFINITY) {
+              const int at = atomicAdd(&c_n, 1);
+              if (at < kLpCand) {
+                c_v[at] = e4[e];
+                c_i[at] = 4 * f[q] + e - pad;
+              }
             }
-          }
+        }
       }
+    __syncthreads();
+    if (tid < 4 && c_n + tid < kLpCand) {          // whole fours for the comparisons
+      c_v[c_n + tid] = -INFINITY;
+      c_i[c_n + tid] = INT32_MAX;
+    }
     __syncthreads();
     int n = c_n;
     const int want = min(top, cnt);
@@ -309,8 +335,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a)
       for (int i = tid; i < n; i += kLpThreads) {
         const float w = c_v[i];
         const int wi = c_i[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += before(c_v[j], c_i[j], w, wi);
+        const int r = rank_of(c_v, c_i, n, w, wi);
         if (r < want) {
           t_v[r] = w;
           t_i[r] = wi;
@@ -399,6 +424,11 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a)
     kv4::cluster_arrive();
     kv4::cluster_wait();
     if (rank != 0) return;
+    if (tid < 4 && (int)ctas * top + tid < kLpMaxCluster * kLpMaxTop) {
+      list_v[ctas * top + tid] = -INFINITY;
+      list_i[ctas * top + tid] = INT32_MAX;
+    }
+    __syncthreads();
     // sums over the slices, in their order
     mine = lp_join(part, (int)ctas);
     const int n = (int)ctas * top;
@@ -406,8 +436,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a)
       const float w = list_v[i];
       const int wi = list_i[i];
       if (wi == INT32_MAX) continue;
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += before(list_v[j], list_i[j], w, wi);
+      const int r = rank_of(list_v, list_i, n, w, wi);
       if (r < top) {
         t_v[r] = w;
         t_i[r] = wi;
@@ -454,7 +483,7 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   // as a thread keeps four float4s, and for rows that a CTA would stream alone
   // for long after the others.
   unsigned ctas = 1;
-  while (ctas < (unsigned)kLpMaxCluster && rows * ctas < 2 * ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
+  while (ctas < (unsigned)kLpMaxCluster && 2 * rows * ctas <= 3 * ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
     ctas *= 2;
   LpArgs a = {};
   a.x = logits;
