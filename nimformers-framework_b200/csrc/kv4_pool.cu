@@ -111,32 +111,43 @@ __global__ void __launch_bounds__(kPoolThreads)
       cu_rows[b] = (int32_t)min(cu_end - nw, (int64_t)INT32_MAX);
       if (b == n_seqs - 1) cu_rows[n_seqs] = (int32_t)min(cu_end, (int64_t)INT32_MAX);
     }
+    // Rows: a warp takes 128 in a row, four a lane, so that the search for a
+    // row's request starts where the one before ended.
     const int cnt = (int)min((int64_t)kPoolThreads, n_seqs - b0);
     const int64_t row_end = min(cu_base + rows_total, max_rows);
-    for (int64_t t = cu_base + (int64_t)rank * kPoolThreads + tid; t < row_end;
-         t += (int64_t)ctas * kPoolThreads) {
-      int lo = 0, hi = cnt - 1;  // the last request whose first row is <= t
+    const int lane = tid & 31;
+    for (int64_t t0 = cu_base + ((int64_t)rank * (kPoolThreads / 32) + (tid >> 5)) * 128; t0 < row_end;
+         t0 += (int64_t)ctas * kPoolThreads * 4) {
+      int lo = 0, hi = cnt - 1;  // the last request whose first row is <= t0
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (s_cu[mid] <= t) lo = mid; else hi = mid - 1;
+        if (s_cu[mid] <= t0) lo = mid; else hi = mid - 1;
       }
-      int32_t slot = -1, pos = 0;
-      if (s_off[lo] >= 0) {
-        const int64_t p = s_len[lo] + (t - s_cu[lo]);
-        const int64_t page = p / bs, old = (s_len[lo] + bs - 1) / bs;
+      int32_t slot[4], pos[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t t = t0 + lane + 32 * k;
+        slot[k] = -1;
+        pos[k] = 0;
+        if (t >= row_end) continue;
+        while (lo + 1 < cnt && s_cu[lo + 1] <= t) ++lo;
+        if (s_off[lo] < 0) continue;
+        const uint32_t old_len = (uint32_t)s_len[lo], p = old_len + (uint32_t)(t - s_cu[lo]);
+        const uint32_t page = p / (uint32_t)bs, old = (old_len + (uint32_t)bs - 1) / (uint32_t)bs, in = p - page * (uint32_t)bs;
         int32_t* entry = table + (b0 + lo) * width + page;
-        int32_t blk;
-        if (page < old) {
-          blk = *entry;
-        } else {
-          blk = free_blocks[nf - 1 - s_off[lo] - (page - old)];
-          if (p % bs == 0) *entry = blk;
-        }
-        pos = (int32_t)p;
-        slot = blk >= 0 && blk < n_blocks ? (int32_t)(blk * (int64_t)bs + p % bs) : -1;
+        const int32_t blk = page < old ? *entry : free_blocks[nf - 1 - s_off[lo] - (page - old)];
+        if (page >= old && in == 0) *entry = blk;
+        pos[k] = (int32_t)p;
+        slot[k] = blk >= 0 && blk < n_blocks ? blk * bs + (int32_t)in : -1;
       }
-      slots[t] = slot;
-      positions[t] = pos;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t t = t0 + lane + 32 * k;
+        if (t < row_end) {
+          slots[t] = slot[k];
+          positions[t] = pos[k];
+        }
+      }
     }
     cu_base += rows_total;
     need_base += need_total;
@@ -235,32 +246,31 @@ __device__ __forceinline__ void store_row(float* p, const float (&x)[VPL]) {
   }
 }
 
-// Rotate-half with the row's table entries, each product and sum rounded (as
-// nimf_rope_dev).  Lane l holds channels l*VPL ..; the other half of a pair is
-// in lane l ^ 16.
+// Rotate-half with the row's table entries c and s, each product and sum rounded
+// (as nimf_rope_dev).  Lane l holds channels l*VPL ..; the other half of a pair
+// is in lane l ^ 16.
 template <int VPL>
-__device__ __forceinline__ void rotate(float (&x)[VPL], const float* cos_row, const float* sin_row,
-                                       int lane) {
-  const int at = (lane & 15) * VPL;
-  const bool upper = lane >= 16;
-  float c[VPL], s[VPL];
-  load_row<VPL>(cos_row + at, c);
-  load_row<VPL>(sin_row + at, s);
+__device__ __forceinline__ void rotate(float (&x)[VPL], const float (&c)[VPL], const float (&s)[VPL], int lane) {
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const float o = __shfl_xor_sync(0xffffffffu, x[i], 16);
-    x[i] = upper ? __fadd_rn(__fmul_rn(o, s[i]), __fmul_rn(x[i], c[i]))
-                 : __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o, s[i]));
+    x[i] = lane >= 16 ? __fadd_rn(__fmul_rn(o, s[i]), __fmul_rn(x[i], c[i]))
+                      : __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o, s[i]));
   }
 }
 
-// One warp per row and head: the query heads are rotated, the key heads
+// A warp takes four heads of a row: the query heads are rotated, the key heads
 // rotated and coded, the value heads coded.  A lane holds D/32 neighbouring
 // channels, a group lies within G / (D/32) lanes.
 //   scale = (max - min) / 15, code = min(15, round((x - min) / scale)),
 // rounded to float at each step, so the codes do not depend on the order of
 // anything.  A group with a NaN, an infinity or a range above the largest
 // float gets NaN as scale and minimum: all it stands for is NaN.
+//
+// Bounded by HBM (the queries alone are read and written in float32): the four
+// heads' loads go out together, and slot, position and table entries are
+// loaded once for them.
+constexpr int kHeads = 4;
 template <int VPL>
 __global__ void __launch_bounds__(256)
     append_kernel(const float* q, float* q_out, int h, const float* __restrict__ k,
@@ -273,81 +283,96 @@ __global__ void __launch_bounds__(256)
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const int ng = D / group, gl = group / VPL;
-  const int per = h + 2 * hkv;
+  const int heads = h + 2 * hkv, per = (heads + kHeads - 1) / kHeads;
   const int64_t items = rows * per;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
        it += (int64_t)gridDim.x * 8) {
-    const int64_t t = it / per;
-    const int hh = (int)(it - t * per);
-    const bool is_q = hh < h, is_k = !is_q && hh < h + hkv;
-    const int64_t slot = slots[t];
-    if (!is_q && (slot < 0 || slot >= n_slots)) {
-      if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
-      continue;
+    const int64_t t = quot(it, per);
+    const int h0 = (int)(it - t * per) * kHeads;
+    float x[kHeads][VPL];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int hh = h0 + i;
+      if (hh >= heads) break;
+      const float* src = hh < h ? q + (t * h + hh) * D
+                                : hh < h + hkv ? k + (t * hkv + hh - h) * D : v + (t * hkv + hh - h - hkv) * D;
+      load_row<VPL>(src + lane * VPL, x[i]);
     }
-    const int head = is_q ? hh : is_k ? hh - h : hh - h - hkv;
-    const float* src = is_q ? q + (t * h + head) * D
-                            : (is_k ? k : v) + (t * hkv + head) * D;
-    float x[VPL];
-    load_row<VPL>(src + lane * VPL, x);
+    const int64_t slot = slots[t];
+    bool keep = slot >= 0 && slot < n_slots;    // the keys and values are appended
+    if (slot >= n_slots && lane == 0 && err && h0 + kHeads > h) atomicExch(err, 4);
+    float c[VPL], s[VPL];
+    bool turn = false;
     if (cos_t) {
       const int64_t pos = positions[t];
-      if (pos < 0 || pos >= max_seq) {  // neither the key nor the value is appended
-        if (lane == 0 && err) atomicExch(err, 4);
+      turn = pos >= 0 && pos < max_seq;
+      if (turn) {
+        load_row<VPL>(cos_t + pos * (D / 2) + (lane & 15) * VPL, c);
+        load_row<VPL>(sin_t + pos * (D / 2) + (lane & 15) * VPL, s);
+      } else if (lane == 0 && err) {
+        atomicExch(err, 4);
+      }
+      keep = keep && turn;
+    }
+    const uint32_t ublk = keep ? (uint32_t)slot / (uint32_t)bs : 0;
+    const int in_blk = keep ? (int)((uint32_t)slot - ublk * (uint32_t)bs) : 0, row = in_blk % kTile;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int hh = h0 + i;
+      if (hh >= heads) break;
+      const bool is_q = hh < h, is_k = !is_q && hh < h + hkv;
+      if (turn && (is_q || is_k)) rotate<VPL>(x[i], c, s, lane);
+      if (is_q) {
+        if (turn || !cos_t) store_row<VPL>(q_out + (t * h + hh) * D + lane * VPL, x[i]);
         continue;
       }
-      if (is_q || is_k) rotate<VPL>(x, cos_t + pos * (D / 2), sin_t + pos * (D / 2), lane);
-    }
-    if (is_q) {
-      store_row<VPL>(q_out + (t * h + head) * D + lane * VPL, x);
-      continue;
-    }
-    float mn = x[0], mx = x[0];
-    bool bad = false;
+      if (!keep) continue;
+      const int head = is_k ? hh - h : hh - h - hkv;
+      float mn = x[i][0], mx = x[i][0];
+      bool bad = false;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      mn = fminf(mn, x[i]);
-      mx = fmaxf(mx, x[i]);
-      bad |= !(fabsf(x[i]) <= FLT_MAX);
-    }
-    mn = __fadd_rn(group_min(mn, gl), 0.f);  // -0 and 0 are one minimum, kept as 0
-    mx = __fadd_rn(group_max(mx, gl), 0.f);
-    const unsigned in_group = (gl == 32 ? 0xffffffffu : ((1u << gl) - 1u)) << (lane / gl * gl);
-    bad = (__ballot_sync(0xffffffffu, bad) & in_group) != 0;
-    float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
-    bad |= !(scale <= FLT_MAX);
-    if (bad) scale = mn = __int_as_float(0x7fffffff);
-    uint32_t code = 0;
-    if (scale > 0.f) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const float c = rintf(__fdiv_rn(__fsub_rn(x[i], mn), scale));
-        code |= (uint32_t)fminf(c, 15.0f) << (4 * i);
+      for (int e = 0; e < VPL; ++e) {
+        mn = fminf(mn, x[i][e]);
+        mx = fmaxf(mx, x[i][e]);
+        bad |= !(fabsf(x[i][e]) <= FLT_MAX);
       }
+      mn = __fadd_rn(group_min(mn, gl), 0.f);  // -0 and 0 are one minimum, kept as 0
+      mx = __fadd_rn(group_max(mx, gl), 0.f);
+      const unsigned in_group = (gl == 32 ? 0xffffffffu : ((1u << gl) - 1u)) << (lane / gl * gl);
+      bad = (__ballot_sync(0xffffffffu, bad) & in_group) != 0;
+      float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
+      bad |= !(scale <= FLT_MAX);
+      if (bad) scale = mn = __int_as_float(0x7fffffff);
+      uint32_t code = 0;
+      if (scale > 0.f) {
+#pragma unroll
+        for (int e = 0; e < VPL; ++e) {
+          const float r = rintf(__fdiv_rn(__fsub_rn(x[i][e], mn), scale));
+          code |= (uint32_t)fminf(r, 15.0f) << (4 * e);
+        }
+      }
+      uint8_t* tile = cache + (((int64_t)ublk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
+      uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
+      const int ch = lane * VPL;
+      if constexpr (VPL == 2) {
+        codes[is_k ? k_byte(ch, D) : v_byte(ch, D)] = (uint8_t)code;
+      } else if constexpr (VPL == 4) {
+        *reinterpret_cast<uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D))) = (uint16_t)code;
+      } else if (is_k) {
+        *reinterpret_cast<uint32_t*>(codes + k_byte(ch, D)) = code;
+      } else {
+        *reinterpret_cast<uint16_t*>(codes + v_byte(ch, D)) = (uint16_t)code;
+        *reinterpret_cast<uint16_t*>(codes + v_byte(ch + 4, D)) = (uint16_t)(code >> 16);
+      }
+      if (lane % gl == 0)
+        *reinterpret_cast<float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
+                                   ((lane / gl) * kTile + row) * 8) = make_float2(scale, mn);
     }
-    const int64_t blk = slot / bs;
-    const int in_blk = (int)(slot - blk * bs), row = in_blk % kTile;
-    uint8_t* tile = cache + ((blk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
-    uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
-    const int ch = lane * VPL;
-    if constexpr (VPL == 2) {
-      codes[is_k ? k_byte(ch, D) : v_byte(ch, D)] = (uint8_t)code;
-    } else if constexpr (VPL == 4) {
-      *reinterpret_cast<uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D))) = (uint16_t)code;
-    } else if (is_k) {
-      *reinterpret_cast<uint32_t*>(codes + k_byte(ch, D)) = code;
-    } else {
-      *reinterpret_cast<uint16_t*>(codes + v_byte(ch, D)) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(codes + v_byte(ch + 4, D)) = (uint16_t)(code >> 16);
-    }
-    if (lane % gl == 0)
-      *reinterpret_cast<float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
-                                 ((lane / gl) * kTile + row) * 8) = make_float2(scale, mn);
   }
 }
 
 // Rows read back: code * scale + min, rounded after the product and after the
-// sum; a slot below zero gives zeros.  One warp per row and head of K and V.
+// sum; a slot below zero gives zeros.  A warp takes four of a row's K and V heads.
 template <int VPL>
 __global__ void __launch_bounds__(256)
     read_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__ slots, int64_t rows,
@@ -358,43 +383,50 @@ __global__ void __launch_bounds__(256)
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const int ng = D / group, gl = group / VPL;
-  const int64_t items = rows * hkv * 2;
+  const int per = (2 * hkv + kHeads - 1) / kHeads;
+  const int64_t items = rows * per;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
        it += (int64_t)gridDim.x * 8) {
-    const int64_t t = it / (2 * hkv);
-    const int hh = (int)(it - t * 2 * hkv);
-    const bool is_k = hh < hkv;
-    const int head = is_k ? hh : hh - hkv;
+    const int64_t t = quot(it, per);
+    const int h0 = (int)(it - t * per) * kHeads;
     const int64_t slot = slots[t];
-    float x[VPL];
-    if (slot < 0 || slot >= n_slots) {
-      if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
+    const bool there = slot >= 0 && slot < n_slots;
+    if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
+    const uint32_t blk = there ? (uint32_t)slot / (uint32_t)bs : 0;
+    const int in_blk = there ? (int)((uint32_t)slot - blk * (uint32_t)bs) : 0, row = in_blk % kTile;
+    uint32_t code[kHeads] = {};
+    float2 p[kHeads] = {};
+    const int ch = lane * VPL;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) x[i] = 0.f;
-    } else {
-      const int64_t blk = slot / bs;
-      const int in_blk = (int)(slot - blk * bs), row = in_blk % kTile;
-      const uint8_t* tile = cache + ((blk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
+    for (int i = 0; i < kHeads; ++i) {
+      const int hh = h0 + i;
+      if (!there || hh >= 2 * hkv) break;
+      const bool is_k = hh < hkv;
+      const uint8_t* tile = cache + (((int64_t)blk * hkv + (is_k ? hh : hh - hkv)) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
       const uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
-      const int ch = lane * VPL;
-      uint32_t code;
       if constexpr (VPL == 2) {
-        code = codes[is_k ? k_byte(ch, D) : v_byte(ch, D)];
+        code[i] = codes[is_k ? k_byte(ch, D) : v_byte(ch, D)];
       } else if constexpr (VPL == 4) {
-        code = *reinterpret_cast<const uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D)));
+        code[i] = *reinterpret_cast<const uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D)));
       } else if (is_k) {
-        code = *reinterpret_cast<const uint32_t*>(codes + k_byte(ch, D));
+        code[i] = *reinterpret_cast<const uint32_t*>(codes + k_byte(ch, D));
       } else {
-        code = *reinterpret_cast<const uint16_t*>(codes + v_byte(ch, D)) |
-               (uint32_t)*reinterpret_cast<const uint16_t*>(codes + v_byte(ch + 4, D)) << 16;
+        code[i] = *reinterpret_cast<const uint16_t*>(codes + v_byte(ch, D)) |
+                  (uint32_t)*reinterpret_cast<const uint16_t*>(codes + v_byte(ch + 4, D)) << 16;
       }
-      const float2 p = *reinterpret_cast<const float2*>(
-          tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) + ((lane / gl) * kTile + row) * 8);
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        x[i] = __fadd_rn(__fmul_rn((float)((code >> (4 * i)) & 15u), p.x), p.y);
+      p[i] = *reinterpret_cast<const float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
+                                              ((lane / gl) * kTile + row) * 8);
     }
-    store_row<VPL>((is_k ? k : v) + (t * hkv + head) * D + lane * VPL, x);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int hh = h0 + i;
+      if (hh >= 2 * hkv) break;
+      const bool is_k = hh < hkv;
+      float x[VPL];
+#pragma unroll
+      for (int e = 0; e < VPL; ++e) x[e] = __fadd_rn(__fmul_rn((float)((code[i] >> (4 * e)) & 15u), p[i].x), p[i].y);
+      store_row<VPL>((is_k ? k : v) + (t * hkv + (is_k ? hh : hh - hkv)) * D + ch, x);
+    }
   }
 }
 
@@ -488,7 +520,7 @@ int nimf_kv4_append_dev(const nimf_kv4_desc* desc, void* cache, const float* k, 
   NIMF_TRY(kv4::stream_of(stream, &st));
   const int h = q ? (int)n_heads : 0;
   auto kern = s.d == 64 ? kv4::append_kernel<2> : s.d == 128 ? kv4::append_kernel<4> : kv4::append_kernel<8>;
-  return kv4::launch(kern, dim3(kv4::warp_grid(rows * (h + 2 * s.hkv))), 256, 0, st, 1, q, q_out, h, k, v,
+  return kv4::launch(kern, dim3(kv4::warp_grid(rows * ((h + 2 * s.hkv + kv4::kHeads - 1) / kv4::kHeads))), 256, 0, st, 1, q, q_out, h, k, v,
                      rows, slots, positions, cos_t, sin_t, max_seq, (uint8_t*)cache, s.hkv, s.bs,
                      s.group, s.n_blocks * s.bs, ctx()->dev_err);
 }
@@ -506,7 +538,7 @@ int nimf_kv4_read_dev(const nimf_kv4_desc* desc, const void* cache, const int32_
     return set_error(NIMF_ERR_ARG, "kv4_read: buffers must be 16-byte aligned");
   NIMF_TRY(kv4::stream_of(stream, &st));
   auto kern = s.d == 64 ? kv4::read_kernel<2> : s.d == 128 ? kv4::read_kernel<4> : kv4::read_kernel<8>;
-  return kv4::launch(kern, dim3(kv4::warp_grid(rows * 2 * s.hkv)), 256, 0, st, 1, (const uint8_t*)cache,
+  return kv4::launch(kern, dim3(kv4::warp_grid(rows * ((2 * s.hkv + kv4::kHeads - 1) / kv4::kHeads))), 256, 0, st, 1, (const uint8_t*)cache,
                      slots, rows, s.hkv, s.bs, s.group, s.n_blocks * s.bs, k, v, ctx()->dev_err);
 }
 
