@@ -111,31 +111,29 @@ __global__ void __launch_bounds__(kPoolThreads)
       cu_rows[b] = (int32_t)min(cu_end - nw, (int64_t)INT32_MAX);
       if (b == n_seqs - 1) cu_rows[n_seqs] = (int32_t)min(cu_end, (int64_t)INT32_MAX);
     }
-    // Rows: a warp takes 128 in a row, four a lane, so that the search for a
-    // row's request starts where the one before ended.
+    // Rows: a warp takes 128 in a row, four a lane, whose searches and loads go
+    // side by side.
     const int cnt = (int)min((int64_t)kPoolThreads, n_seqs - b0);
     const int64_t row_end = min(cu_base + rows_total, max_rows);
     const int lane = tid & 31;
     for (int64_t t0 = cu_base + ((int64_t)rank * (kPoolThreads / 32) + (tid >> 5)) * 128; t0 < row_end;
          t0 += (int64_t)ctas * kPoolThreads * 4) {
-      int lo = 0, hi = cnt - 1;  // the last request whose first row is <= t0
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_cu[mid] <= t0) lo = mid; else hi = mid - 1;
-      }
+      int lo[4] = {};              // the last request whose first row is <= the row
+      for (int step = 1 << (31 - __clz(cnt)); step > 0; step >>= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (lo[k] + step < cnt && s_cu[lo[k] + step] <= t0 + lane + 32 * k) lo[k] += step;
       int32_t slot[4], pos[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int64_t t = t0 + lane + 32 * k;
         slot[k] = -1;
         pos[k] = 0;
-        if (t >= row_end) continue;
-        while (lo + 1 < cnt && s_cu[lo + 1] <= t) ++lo;
-        if (s_off[lo] < 0) continue;
-        const uint32_t old_len = (uint32_t)s_len[lo], p = old_len + (uint32_t)(t - s_cu[lo]);
+        if (t >= row_end || s_off[lo[k]] < 0) continue;
+        const uint32_t old_len = (uint32_t)s_len[lo[k]], p = old_len + (uint32_t)(t - s_cu[lo[k]]);
         const uint32_t page = p / (uint32_t)bs, old = (old_len + (uint32_t)bs - 1) / (uint32_t)bs, in = p - page * (uint32_t)bs;
-        int32_t* entry = table + (b0 + lo) * width + page;
-        const int32_t blk = page < old ? *entry : free_blocks[nf - 1 - s_off[lo] - (page - old)];
+        int32_t* entry = table + (b0 + lo[k]) * width + page;
+        const int32_t blk = page < old ? *entry : free_blocks[nf - 1 - s_off[lo[k]] - (page - old)];
         if (page >= old && in == 0) *entry = blk;
         pos[k] = (int32_t)p;
         slot[k] = blk >= 0 && blk < n_blocks ? blk * bs + (int32_t)in : -1;
@@ -208,12 +206,16 @@ __global__ void __launch_bounds__(kPoolThreads)
   if (tid == 0) n_free[0] = (int32_t)top;
 }
 
-__device__ __forceinline__ float group_min(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
+template <int LANES>
+__device__ __forceinline__ float group_min(float v) {
+#pragma unroll
+  for (int o = LANES >> 1; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ float group_max(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+template <int LANES>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = LANES >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -259,99 +261,123 @@ __device__ __forceinline__ void rotate(float (&x)[VPL], const float (&c)[VPL], c
   }
 }
 
-// A warp takes four heads of a row: the query heads are rotated, the key heads
-// rotated and coded, the value heads coded.  A lane holds D/32 neighbouring
-// channels, a group lies within G / (D/32) lanes.
+// One group's codes, four bits each, of this lane's VPL channels.
 //   scale = (max - min) / 15, code = min(15, round((x - min) / scale)),
 // rounded to float at each step, so the codes do not depend on the order of
 // anything.  A group with a NaN, an infinity or a range above the largest
 // float gets NaN as scale and minimum: all it stands for is NaN.
 //
-// Bounded by HBM (the queries alone are read and written in float32): the four
-// heads' loads go out together, and slot, position and table entries are
-// loaded once for them.
-constexpr int kHeads = 4;
-template <int VPL>
+// The quotients are taken as products with 1 / scale, which are off by 2^-18 at
+// most here (three roundings of 2^-24, quotients up to 15): where one lies
+// within 2^-16 of the middle between two codes, and for scales whose
+// reciprocal may overflow, the division decides.
+template <int VPL, int LANES>
+__device__ __forceinline__ uint32_t code_group(const float (&x)[VPL], int lane, float& scale, float& mn) {
+  float mx = x[0];
+  mn = x[0];
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < VPL; ++e) {
+    mn = fminf(mn, x[e]);
+    mx = fmaxf(mx, x[e]);
+    bad |= !(fabsf(x[e]) <= FLT_MAX);
+  }
+  mn = __fadd_rn(group_min<LANES>(mn), 0.f);    // -0 and 0 are one minimum, kept as 0
+  mx = __fadd_rn(group_max<LANES>(mx), 0.f);
+  const unsigned in_group = (LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u)) << (lane / LANES * LANES);
+  bad = (__ballot_sync(0xffffffffu, bad) & in_group) != 0;
+  scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
+  bad |= !(scale <= FLT_MAX);
+  uint32_t code = 0;
+  if (!bad && scale > 0.f) {
+    bool near = scale < 0x1p-100f;
+    const float inv = __frcp_rn(scale);
+#pragma unroll
+    for (int e = 0; e < VPL; ++e) {
+      const float q = __fmul_rn(__fsub_rn(x[e], mn), inv);
+      const float r = __fadd_rn(q, 12582912.f);  // its last bits are the nearest integer
+      near |= !(fabsf(__fsub_rn(q, __fsub_rn(r, 12582912.f))) < 0.5f - 0x1p-16f);
+      code |= (__float_as_uint(r) & 15u) << (4 * e);
+    }
+    if (near) {
+      code = 0;
+#pragma unroll 1
+      for (int e = 0; e < VPL; ++e) {
+        float d = x[0];
+#pragma unroll
+        for (int i = 1; i < VPL; ++i) d = i == e ? x[i] : d;
+        const float r = rintf(__fdiv_rn(__fsub_rn(d, mn), scale));
+        code |= (uint32_t)fminf(r, 15.0f) << (4 * e);
+      }
+    }
+  }
+  if (bad) scale = mn = __int_as_float(0x7fffffff);
+  return code;
+}
+
+// A warp takes HB heads of one kind of a row: query heads are rotated, key
+// heads rotated and coded, value heads coded.  A lane holds VPL = D/32
+// neighbouring channels, a group lies within LANES = G / VPL lanes.
+//
+// Long batches are bounded by HBM (the queries alone are read and written in
+// float32) with HB = 4: four loads go out together, and slot, position and table
+// entries are loaded once for them.  With fewer heads than warps HB = 1 has the
+// shorter way.
+template <int VPL, int LANES, int HB>
 __global__ void __launch_bounds__(256)
     append_kernel(const float* q, float* q_out, int h, const float* __restrict__ k,
                   const float* __restrict__ v, int64_t rows, const int32_t* __restrict__ slots,
                   const int32_t* __restrict__ positions, const float* __restrict__ cos_t,
                   const float* __restrict__ sin_t, int64_t max_seq, uint8_t* __restrict__ cache,
-                  int hkv, int bs, int group, int64_t n_slots, int* err) {
-  constexpr int D = VPL * 32;
+                  int hkv, int bs, int64_t n_slots, int* err) {
+  constexpr int D = VPL * 32, NG = 32 / LANES, TB = tile_bytes(D, NG);
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
-  const int ng = D / group, gl = group / VPL;
-  const int heads = h + 2 * hkv, per = (heads + kHeads - 1) / kHeads;
+  const int nq = (h + HB - 1) / HB, nk = (hkv + HB - 1) / HB, per = nq + 2 * nk;
   const int64_t items = rows * per;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
        it += (int64_t)gridDim.x * 8) {
     const int64_t t = quot(it, per);
-    const int h0 = (int)(it - t * per) * kHeads;
-    float x[kHeads][VPL];
+    const int w = (int)(it - t * per);
+    const bool is_q = w < nq, is_k = !is_q && w < nq + nk;
+    const int h0 = (is_q ? w : is_k ? w - nq : w - nq - nk) * HB, heads = is_q ? h : hkv;
+    const float* src = (is_q ? q : is_k ? k : v) + (t * heads + h0) * D + lane * VPL;
+    float x[HB][VPL];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int hh = h0 + i;
-      if (hh >= heads) break;
-      const float* src = hh < h ? q + (t * h + hh) * D
-                                : hh < h + hkv ? k + (t * hkv + hh - h) * D : v + (t * hkv + hh - h - hkv) * D;
-      load_row<VPL>(src + lane * VPL, x[i]);
-    }
-    const int64_t slot = slots[t];
-    bool keep = slot >= 0 && slot < n_slots;    // the keys and values are appended
-    if (slot >= n_slots && lane == 0 && err && h0 + kHeads > h) atomicExch(err, 4);
-    float c[VPL], s[VPL];
-    bool turn = false;
+    for (int i = 0; i < HB; ++i)
+      if (HB == 1 || h0 + i < heads) load_row<VPL>(src + i * D, x[i]);
+    bool turn = true;
     if (cos_t) {
       const int64_t pos = positions[t];
-      turn = pos >= 0 && pos < max_seq;
-      if (turn) {
+      turn = pos >= 0 && pos < max_seq;           // otherwise nothing of the row is done
+      if (!turn && lane == 0 && err) atomicExch(err, 4);
+      if (turn && (is_q || is_k)) {
+        float c[VPL], s[VPL];
         load_row<VPL>(cos_t + pos * (D / 2) + (lane & 15) * VPL, c);
         load_row<VPL>(sin_t + pos * (D / 2) + (lane & 15) * VPL, s);
-      } else if (lane == 0 && err) {
-        atomicExch(err, 4);
+#pragma unroll
+        for (int i = 0; i < HB; ++i) rotate<VPL>(x[i], c, s, lane);
       }
-      keep = keep && turn;
     }
-    const uint32_t ublk = keep ? (uint32_t)slot / (uint32_t)bs : 0;
-    const int in_blk = keep ? (int)((uint32_t)slot - ublk * (uint32_t)bs) : 0, row = in_blk % kTile;
+    if (is_q) {
+      if (turn)
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int hh = h0 + i;
-      if (hh >= heads) break;
-      const bool is_q = hh < h, is_k = !is_q && hh < h + hkv;
-      if (turn && (is_q || is_k)) rotate<VPL>(x[i], c, s, lane);
-      if (is_q) {
-        if (turn || !cos_t) store_row<VPL>(q_out + (t * h + hh) * D + lane * VPL, x[i]);
-        continue;
-      }
-      if (!keep) continue;
-      const int head = is_k ? hh - h : hh - h - hkv;
-      float mn = x[i][0], mx = x[i][0];
-      bool bad = false;
+        for (int i = 0; i < HB; ++i)
+          if (HB == 1 || h0 + i < heads) store_row<VPL>(q_out + (t * h + h0 + i) * D + lane * VPL, x[i]);
+      continue;
+    }
+    const int64_t slot = slots[t];
+    if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
+    if (!turn || slot < 0 || slot >= n_slots) continue;
+    const uint32_t blk = (uint32_t)slot / (uint32_t)bs, in_blk = (uint32_t)slot - blk * (uint32_t)bs;
+    const int row = in_blk % kTile, tiles = bs / kTile;
+    uint8_t* tile = cache + (((int64_t)blk * hkv + h0) * tiles + in_blk / kTile) * TB;
 #pragma unroll
-      for (int e = 0; e < VPL; ++e) {
-        mn = fminf(mn, x[i][e]);
-        mx = fmaxf(mx, x[i][e]);
-        bad |= !(fabsf(x[i][e]) <= FLT_MAX);
-      }
-      mn = __fadd_rn(group_min(mn, gl), 0.f);  // -0 and 0 are one minimum, kept as 0
-      mx = __fadd_rn(group_max(mx, gl), 0.f);
-      const unsigned in_group = (gl == 32 ? 0xffffffffu : ((1u << gl) - 1u)) << (lane / gl * gl);
-      bad = (__ballot_sync(0xffffffffu, bad) & in_group) != 0;
-      float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
-      bad |= !(scale <= FLT_MAX);
-      if (bad) scale = mn = __int_as_float(0x7fffffff);
-      uint32_t code = 0;
-      if (scale > 0.f) {
-#pragma unroll
-        for (int e = 0; e < VPL; ++e) {
-          const float r = rintf(__fdiv_rn(__fsub_rn(x[i][e], mn), scale));
-          code |= (uint32_t)fminf(r, 15.0f) << (4 * e);
-        }
-      }
-      uint8_t* tile = cache + (((int64_t)ublk * hkv + head) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
+    for (int i = 0; i < HB; ++i, tile += (int64_t)tiles * TB) {
+      if (HB > 1 && h0 + i >= heads) break;
+      float scale, mn;
+      const uint32_t code = code_group<VPL, LANES>(x[i], lane, scale, mn);
       uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
       const int ch = lane * VPL;
       if constexpr (VPL == 2) {
@@ -364,68 +390,66 @@ __global__ void __launch_bounds__(256)
         *reinterpret_cast<uint16_t*>(codes + v_byte(ch, D)) = (uint16_t)code;
         *reinterpret_cast<uint16_t*>(codes + v_byte(ch + 4, D)) = (uint16_t)(code >> 16);
       }
-      if (lane % gl == 0)
-        *reinterpret_cast<float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
-                                   ((lane / gl) * kTile + row) * 8) = make_float2(scale, mn);
+      if (lane % LANES == 0)
+        *reinterpret_cast<float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, NG)) +
+                                   ((lane / LANES) * kTile + row) * 8) = make_float2(scale, mn);
     }
   }
 }
 
 // Rows read back: code * scale + min, rounded after the product and after the
-// sum; a slot below zero gives zeros.  A warp takes four of a row's K and V heads.
-template <int VPL>
+// sum; a slot below zero gives zeros.  A warp takes HB of a row's K and V heads.
+template <int VPL, int LANES, int HB>
 __global__ void __launch_bounds__(256)
     read_kernel(const uint8_t* __restrict__ cache, const int32_t* __restrict__ slots, int64_t rows,
-                int hkv, int bs, int group, int64_t n_slots, float* __restrict__ k,
-                float* __restrict__ v, int* err) {
-  constexpr int D = VPL * 32;
+                int hkv, int bs, int64_t n_slots, float* __restrict__ k, float* __restrict__ v, int* err) {
+  constexpr int D = VPL * 32, NG = 32 / LANES, TB = tile_bytes(D, NG);
   griddep_launch_dependents();
   griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const int ng = D / group, gl = group / VPL;
-  const int per = (2 * hkv + kHeads - 1) / kHeads;
+  const int lane = threadIdx.x & 31, ch = lane * VPL;
+  const int nk = (hkv + HB - 1) / HB, per = 2 * nk;
   const int64_t items = rows * per;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items;
        it += (int64_t)gridDim.x * 8) {
     const int64_t t = quot(it, per);
-    const int h0 = (int)(it - t * per) * kHeads;
+    const int w = (int)(it - t * per);
+    const bool is_k = w < nk;
+    const int h0 = (is_k ? w : w - nk) * HB;
     const int64_t slot = slots[t];
     const bool there = slot >= 0 && slot < n_slots;
     if (slot >= n_slots && lane == 0 && err) atomicExch(err, 4);
-    const uint32_t blk = there ? (uint32_t)slot / (uint32_t)bs : 0;
-    const int in_blk = there ? (int)((uint32_t)slot - blk * (uint32_t)bs) : 0, row = in_blk % kTile;
-    uint32_t code[kHeads] = {};
-    float2 p[kHeads] = {};
-    const int ch = lane * VPL;
+    uint32_t code[HB] = {};
+    float2 p[HB] = {};
+    if (there) {
+      const uint32_t blk = (uint32_t)slot / (uint32_t)bs, in_blk = (uint32_t)slot - blk * (uint32_t)bs;
+      const int row = in_blk % kTile, tiles = bs / kTile;
+      const uint8_t* tile = cache + (((int64_t)blk * hkv + h0) * tiles + in_blk / kTile) * TB;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int hh = h0 + i;
-      if (!there || hh >= 2 * hkv) break;
-      const bool is_k = hh < hkv;
-      const uint8_t* tile = cache + (((int64_t)blk * hkv + (is_k ? hh : hh - hkv)) * (bs / kTile) + in_blk / kTile) * tile_bytes(D, ng);
-      const uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
-      if constexpr (VPL == 2) {
-        code[i] = codes[is_k ? k_byte(ch, D) : v_byte(ch, D)];
-      } else if constexpr (VPL == 4) {
-        code[i] = *reinterpret_cast<const uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D)));
-      } else if (is_k) {
-        code[i] = *reinterpret_cast<const uint32_t*>(codes + k_byte(ch, D));
-      } else {
-        code[i] = *reinterpret_cast<const uint16_t*>(codes + v_byte(ch, D)) |
-                  (uint32_t)*reinterpret_cast<const uint16_t*>(codes + v_byte(ch + 4, D)) << 16;
+      for (int i = 0; i < HB; ++i, tile += (int64_t)tiles * TB) {
+        if (HB > 1 && h0 + i >= hkv) break;
+        const uint8_t* codes = tile + (is_k ? 0 : v_codes_at(D)) + row * (D / 2);
+        if constexpr (VPL == 2) {
+          code[i] = codes[is_k ? k_byte(ch, D) : v_byte(ch, D)];
+        } else if constexpr (VPL == 4) {
+          code[i] = *reinterpret_cast<const uint16_t*>(codes + (is_k ? k_byte(ch, D) : v_byte(ch, D)));
+        } else if (is_k) {
+          code[i] = *reinterpret_cast<const uint32_t*>(codes + k_byte(ch, D));
+        } else {
+          code[i] = *reinterpret_cast<const uint16_t*>(codes + v_byte(ch, D)) |
+                    (uint32_t)*reinterpret_cast<const uint16_t*>(codes + v_byte(ch + 4, D)) << 16;
+        }
+        p[i] = *reinterpret_cast<const float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, NG)) +
+                                                ((lane / LANES) * kTile + row) * 8);
       }
-      p[i] = *reinterpret_cast<const float2*>(tile + (is_k ? k_params_at(D) : v_params_at(D, ng)) +
-                                              ((lane / gl) * kTile + row) * 8);
     }
+    float* dst = (is_k ? k : v) + (t * hkv + h0) * D + ch;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int hh = h0 + i;
-      if (hh >= 2 * hkv) break;
-      const bool is_k = hh < hkv;
+    for (int i = 0; i < HB; ++i) {
+      if (HB > 1 && h0 + i >= hkv) break;
       float x[VPL];
 #pragma unroll
       for (int e = 0; e < VPL; ++e) x[e] = __fadd_rn(__fmul_rn((float)((code[i] >> (4 * e)) & 15u), p[i].x), p[i].y);
-      store_row<VPL>((is_k ? k : v) + (t * hkv + (is_k ? hh : hh - hkv)) * D + ch, x);
+      store_row<VPL>(dst + i * D, x);
     }
   }
 }
@@ -435,6 +459,62 @@ unsigned warp_grid(int64_t items) {
   const int64_t most = (int64_t)(c ? c->num_sms : 148) * 8;
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, (items + 7) / 8));
 }
+
+// Warps that are resident at once; with fewer items a warp takes one head.
+int64_t all_warps() { return (int64_t)ctx()->num_sms * 64; }
+
+struct AppendArgs {
+  const float *q;
+  float* q_out;
+  int h;
+  const float *k, *v;
+  int64_t rows;
+  const int32_t *slots, *positions;
+  const float *cos_t, *sin_t;
+  int64_t max_seq;
+  uint8_t* cache;
+  Shape s;
+};
+
+template <int VPL, int LANES>
+int run_append(const AppendArgs& a, cudaStream_t st) {
+  const bool few = a.rows * (a.h + 2 * a.s.hkv) <= all_warps();
+  const int hb = few ? 1 : 4;
+  const int64_t items = a.rows * ((a.h + hb - 1) / hb + 2 * ((a.s.hkv + hb - 1) / hb));
+  auto kern = few ? append_kernel<VPL, LANES, 1> : append_kernel<VPL, LANES, 4>;
+  return launch(kern, dim3(warp_grid(items)), 256, 0, st, 1, a.q, a.q_out, a.h, a.k, a.v, a.rows, a.slots,
+                a.positions, a.cos_t, a.sin_t, a.max_seq, a.cache, a.s.hkv, a.s.bs, a.s.n_blocks * a.s.bs,
+                ctx()->dev_err);
+}
+
+template <int VPL, int LANES>
+int run_read(const Shape& s, const uint8_t* cache, const int32_t* slots, int64_t rows, float* k, float* v,
+             cudaStream_t st) {
+  const bool few = rows * 2 * s.hkv <= all_warps();
+  const int hb = few ? 1 : 4;
+  auto kern = few ? read_kernel<VPL, LANES, 1> : read_kernel<VPL, LANES, 4>;
+  return launch(kern, dim3(warp_grid(rows * 2 * ((s.hkv + hb - 1) / hb))), 256, 0, st, 1, cache, slots, rows,
+                s.hkv, s.bs, s.n_blocks * s.bs, k, v, ctx()->dev_err);
+}
+
+// f<VPL, LANES>(...) of a cache's head dim and group.
+#define NIMF_KV4_BY_SHAPE(f, s, ...)                                          \
+  switch ((s).d * 16 + (s).d / (s).group) {                                   \
+    case 64 * 16 + 1: return f<2, 32>(__VA_ARGS__);                           \
+    case 64 * 16 + 2: return f<2, 16>(__VA_ARGS__);                           \
+    case 128 * 16 + 1: return f<4, 32>(__VA_ARGS__);                          \
+    case 128 * 16 + 2: return f<4, 16>(__VA_ARGS__);                          \
+    case 128 * 16 + 4: return f<4, 8>(__VA_ARGS__);                           \
+    case 256 * 16 + 2: return f<8, 16>(__VA_ARGS__);                          \
+    case 256 * 16 + 4: return f<8, 8>(__VA_ARGS__);                           \
+    default: return f<8, 4>(__VA_ARGS__);                                     \
+  }
+int append_by_shape(const AppendArgs& a, cudaStream_t st) { NIMF_KV4_BY_SHAPE(run_append, a.s, a, st) }
+int read_by_shape(const Shape& s, const uint8_t* cache, const int32_t* slots, int64_t rows, float* k,
+                  float* v, cudaStream_t st) {
+  NIMF_KV4_BY_SHAPE(run_read, s, s, cache, slots, rows, k, v, st)
+}
+#undef NIMF_KV4_BY_SHAPE
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -518,11 +598,8 @@ int nimf_kv4_append_dev(const nimf_kv4_desc* desc, void* cache, const float* k, 
     if (!kv4::aligned(p, 16))
       return set_error(NIMF_ERR_ARG, "kv4_append: buffers must be 16-byte aligned");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  const int h = q ? (int)n_heads : 0;
-  auto kern = s.d == 64 ? kv4::append_kernel<2> : s.d == 128 ? kv4::append_kernel<4> : kv4::append_kernel<8>;
-  return kv4::launch(kern, dim3(kv4::warp_grid(rows * ((h + 2 * s.hkv + kv4::kHeads - 1) / kv4::kHeads))), 256, 0, st, 1, q, q_out, h, k, v,
-                     rows, slots, positions, cos_t, sin_t, max_seq, (uint8_t*)cache, s.hkv, s.bs,
-                     s.group, s.n_blocks * s.bs, ctx()->dev_err);
+  return kv4::append_by_shape({q, q_out, q ? (int)n_heads : 0, k, v, rows, slots, positions, cos_t, sin_t,
+                               max_seq, (uint8_t*)cache, s}, st);
 }
 
 int nimf_kv4_read_dev(const nimf_kv4_desc* desc, const void* cache, const int32_t* slots,
@@ -537,9 +614,7 @@ int nimf_kv4_read_dev(const nimf_kv4_desc* desc, const void* cache, const int32_
   if (!kv4::aligned(cache, 16) || !kv4::aligned(k, 16) || !kv4::aligned(v, 16))
     return set_error(NIMF_ERR_ARG, "kv4_read: buffers must be 16-byte aligned");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  auto kern = s.d == 64 ? kv4::read_kernel<2> : s.d == 128 ? kv4::read_kernel<4> : kv4::read_kernel<8>;
-  return kv4::launch(kern, dim3(kv4::warp_grid(rows * ((2 * s.hkv + kv4::kHeads - 1) / kv4::kHeads))), 256, 0, st, 1, (const uint8_t*)cache,
-                     slots, rows, s.hkv, s.bs, s.group, s.n_blocks * s.bs, k, v, ctx()->dev_err);
+  return kv4::read_by_shape(s, (const uint8_t*)cache, slots, rows, k, v, st);
 }
 
 }  // extern "C"
