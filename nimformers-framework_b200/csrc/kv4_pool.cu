@@ -59,110 +59,162 @@ constexpr int kPoolThreads = 1024;
 //   rows(b) = [cu(b), cu(b) + new(b))              prefix sum of the new tokens
 //   need(b) = ceil((len + new) / bs) - ceil(len / bs)   where the request fits
 //   granted = fits and (need == 0 or its inclusive sum of needs <= n_free)
-// The sum never falls, so the granted needs are the first ones and the j-th
-// fresh block of request b is free[n_free - 1 - (sum before b) - j].  A new
-// row's block is either an old entry of the table or one of those, so no row
-// waits for a table entry to be written; the row that opens a block writes it.
+// The sum never falls, so the granted needs are the first ones, and the i-th
+// fresh block of the step is free[n_free - 1 - i].
 //
-// The cost is latency (a few dependent loads, two scans of 1,024 requests and
-// a search), not bytes.  Every CTA of the one cluster scans all requests and
-// they share the rows; lens may be its own output, so the CTAs meet between
-// reading a chunk of requests and CTA 0 writing it.
+// The cost is latency (dependent loads, two scans, a search for each row's
+// request), not bytes.  One CTA scans the requests and writes the tables; up to
+// kOwnRows rows it also writes the slots (64 requests with one row each: 5 us
+// with launch), more are left to a second kernel on all SMs (130,000 rows: 30 us
+// where a cluster of 8 CTAs did everything).
+constexpr int kOwnRows = 4096;
+
+// x / bs for x < 2^31: bs = 16 d, and 2^36 / d rounded up is exact enough.
+struct Blocks {
+  uint64_t magic;
+  uint32_t bs;
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)((uint64_t)(x >> 4) * magic >> 36); }
+};
+
+// The slots and positions of rows [t0, t0 + 128), a warp; the requests' tables
+// and lengths are already the new ones.
+__device__ __forceinline__ void write_rows(int64_t t0, int n_seqs, int64_t width, Blocks blocks,
+                                           int64_t n_blocks, const int32_t* lens_out,
+                                           const int32_t* table, int64_t max_rows,
+                                           const int32_t* cu_rows, const int32_t* granted,
+                                           int32_t* slots, int32_t* positions) {
+  const int lane = threadIdx.x & 31;
+  // the last request whose first row is <= t0, the same for the warp's last row,
+  // then each lane's between them
+  int lo = 0, last = 0;
+  const int64_t t_end = min(t0 + 127, max_rows - 1);
+  for (int step = 1 << (31 - __clz(n_seqs)); step > 0; step >>= 1) {
+    const int a = lo + step, b = last + step;
+    const int ca = a < n_seqs ? cu_rows[a] : INT32_MAX, cb = b < n_seqs ? cu_rows[b] : INT32_MAX;
+    if (ca <= t0) lo = a;
+    if (cb <= t_end) last = b;
+  }
+  int req[4] = {lo, lo, lo, lo};
+  if (last > lo)
+    for (int step = 1 << (31 - __clz(last - lo)); step > 0; step >>= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int a = min(req[k] + step, last);
+        if (cu_rows[a] <= t0 + lane + 32 * k) req[k] = a;
+      }
+  const int32_t* entry[4];
+  int32_t pos[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t t = t0 + lane + 32 * k;
+    const int b = req[k];
+    const int32_t end = cu_rows[b + 1];
+    const bool ok = t < end && granted[b] != 0;
+    pos[k] = ok ? lens_out[b] - (end - (int32_t)t) : 0;
+    entry[k] = ok ? table + b * width + blocks.of((uint32_t)pos[k]) : nullptr;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t t = t0 + lane + 32 * k;
+    const int32_t blk = entry[k] ? *entry[k] : -1;
+    const int32_t in = pos[k] - (int32_t)(blocks.of((uint32_t)pos[k]) * blocks.bs);
+    if (t < max_rows) {
+      slots[t] = blk >= 0 && blk < n_blocks ? blk * (int32_t)blocks.bs + in : -1;
+      positions[t] = pos[k];
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kPoolThreads)
-    reserve_kernel(int64_t n_seqs, int64_t width, int bs, int64_t n_blocks,
+    reserve_kernel(int n_seqs, int64_t width, Blocks blocks, int64_t n_blocks,
                    const int32_t* __restrict__ n_new, const int32_t* lens, int32_t* lens_out,
                    int32_t* table, const int32_t* __restrict__ free_blocks, const int32_t* n_free_in,
-                   int32_t* n_free_out, int64_t max_rows, int32_t* __restrict__ cu_rows,
-                   int32_t* __restrict__ slots, int32_t* __restrict__ positions,
-                   int32_t* __restrict__ granted) {
+                   int32_t* n_free_out, int64_t max_rows, int32_t* cu_rows, int32_t* slots,
+                   int32_t* positions, int32_t* granted, int own_rows) {
   __shared__ int64_t sh[33];
-  __shared__ int64_t s_cu[kPoolThreads];    // first row of each request of the chunk
-  __shared__ int64_t s_off[kPoolThreads];   // fresh blocks before it; -1: not granted
-  __shared__ int32_t s_len[kPoolThreads];
+  __shared__ int64_t s_off[kPoolThreads];   // fresh blocks before each request of the chunk
+  __shared__ int32_t s_have[kPoolThreads];
+  __shared__ unsigned long long s_taken;
   griddep_launch_dependents();
   griddep_wait();
-  const unsigned rank = cluster_rank(), ctas = cluster_size();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const uint32_t bs = blocks.bs;
   const int64_t nf = min((int64_t)max(n_free_in[0], 0), n_blocks);
-  int64_t cu_base = 0, need_base = 0, taken = 0;
-  for (int64_t b0 = 0; b0 < n_seqs; b0 += kPoolThreads) {
-    const int64_t b = b0 + tid;
+  if (tid == 0) s_taken = 0;
+  int64_t cu_base = 0, need_base = 0;
+  for (int b0 = 0; b0 < n_seqs; b0 += threads) {
+    const int b = b0 + tid;
     const bool live = b < n_seqs;
     const int64_t len = live ? max(lens[b], 0) : 0;
     const int64_t nw = live ? max(n_new[b], 0) : 0;
     int64_t rows_total, need_total;
     const int64_t cu_end = cu_base + block_scan<int64_t>(nw, sh, &rows_total);
-    const int64_t have = (len + bs - 1) / bs, total = (len + nw + bs - 1) / bs;
-    const bool fits = live && total <= width && cu_end <= max_rows;
+    const bool short_enough = len + nw <= (int64_t)INT32_MAX - bs;
+    const uint32_t have = blocks.of((uint32_t)min(len, (int64_t)INT32_MAX - bs) + bs - 1);
+    const uint32_t total = short_enough ? blocks.of((uint32_t)(len + nw) + bs - 1) : 0;
+    const bool fits = live && short_enough && total <= width && cu_end <= max_rows;
     const int64_t need = fits ? total - have : 0;
     const int64_t upto = need_base + block_scan<int64_t>(need, sh, &need_total);
     const bool ok = fits && (need == 0 || upto <= nf);
+    const int64_t taken_before = (int64_t)s_taken;
     __syncthreads();
-    s_cu[tid] = cu_end - nw;
-    s_off[tid] = ok ? upto - need : -1;
-    s_len[tid] = (int32_t)len;
-    int64_t chunk_taken;
-    block_scan<int64_t>(ok ? need : 0, sh, &chunk_taken);
-    cluster_arrive();
-    cluster_wait();  // every CTA has read this chunk's lens
-    if (rank == 0 && live) {
+    s_off[tid] = upto - need;
+    s_have[tid] = (int32_t)have;
+    if (ok && need > 0) atomicMax(&s_taken, (unsigned long long)upto);
+    if (live) {
       lens_out[b] = (int32_t)(ok ? len + nw : len);
       granted[b] = ok ? 1 : 0;
       cu_rows[b] = (int32_t)min(cu_end - nw, (int64_t)INT32_MAX);
       if (b == n_seqs - 1) cu_rows[n_seqs] = (int32_t)min(cu_end, (int64_t)INT32_MAX);
     }
-    // Rows: a warp takes 128 in a row, four a lane, whose searches and loads go
-    // side by side.
-    const int cnt = (int)min((int64_t)kPoolThreads, n_seqs - b0);
-    const int64_t row_end = min(cu_base + rows_total, max_rows);
-    const int lane = tid & 31;
-    for (int64_t t0 = cu_base + ((int64_t)rank * (kPoolThreads / 32) + (tid >> 5)) * 128; t0 < row_end;
-         t0 += (int64_t)ctas * kPoolThreads * 4) {
-      int lo[4] = {};              // the last request whose first row is <= the row
+    __syncthreads();
+    // the chunk's fresh blocks into the tables
+    const int cnt = min(threads, n_seqs - b0);
+    const int64_t taken = (int64_t)s_taken;
+    for (int64_t i0 = max(taken_before, need_base) + tid; i0 < taken; i0 += 4 * threads) {
+      int lo[4] = {}, blk[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) blk[k] = i0 + k * threads < taken ? free_blocks[nf - 1 - i0 - k * threads] : 0;
       for (int step = 1 << (31 - __clz(cnt)); step > 0; step >>= 1)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (lo[k] + step < cnt && s_cu[lo[k] + step] <= t0 + lane + 32 * k) lo[k] += step;
-      int32_t slot[4], pos[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t t = t0 + lane + 32 * k;
-        slot[k] = -1;
-        pos[k] = 0;
-        if (t >= row_end || s_off[lo[k]] < 0) continue;
-        const uint32_t old_len = (uint32_t)s_len[lo[k]], p = old_len + (uint32_t)(t - s_cu[lo[k]]);
-        const uint32_t page = p / (uint32_t)bs, old = (old_len + (uint32_t)bs - 1) / (uint32_t)bs, in = p - page * (uint32_t)bs;
-        int32_t* entry = table + (b0 + lo[k]) * width + page;
-        const int32_t blk = page < old ? *entry : free_blocks[nf - 1 - s_off[lo[k]] - (page - old)];
-        if (page >= old && in == 0) *entry = blk;
-        pos[k] = (int32_t)p;
-        slot[k] = blk >= 0 && blk < n_blocks ? blk * bs + (int32_t)in : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t t = t0 + lane + 32 * k;
-        if (t < row_end) {
-          slots[t] = slot[k];
-          positions[t] = pos[k];
+        for (int k = 0; k < 4; ++k) {
+          const int a = min(lo[k] + step, cnt - 1);
+          if (s_off[a] <= i0 + k * threads) lo[k] = a;
         }
-      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k * threads < taken)
+          table[(int64_t)(b0 + lo[k]) * width + s_have[lo[k]] + (i0 + k * threads - s_off[lo[k]])] = blk[k];
     }
     cu_base += rows_total;
     need_base += need_total;
-    taken += chunk_taken;
     __syncthreads();
   }
-  for (int64_t t = cu_base + (int64_t)rank * kPoolThreads + tid; t < max_rows;
-       t += (int64_t)ctas * kPoolThreads) {
-    slots[t] = -1;
-    positions[t] = 0;
-  }
-  cluster_arrive();
-  cluster_wait();  // every CTA has read n_free
-  if (rank == 0 && tid == 0) {
-    n_free_out[0] = (int32_t)(nf - taken);
+  if (tid == 0) {
+    n_free_out[0] = (int32_t)(nf - (int64_t)s_taken);
     if (n_seqs == 0) cu_rows[0] = 0;
   }
+  if (own_rows)
+    for (int64_t t0 = (tid >> 5) * 128; t0 < max_rows; t0 += (threads >> 5) * 128) {
+      if (n_seqs > 0) {
+        write_rows(t0, n_seqs, width, blocks, n_blocks, lens_out, table, max_rows, cu_rows, granted, slots, positions);
+      } else {
+        for (int64_t t = t0 + (tid & 31); t < min(t0 + 128, max_rows); t += 32) {
+          slots[t] = -1;
+          positions[t] = 0;
+        }
+      }
+    }
+}
+
+__global__ void __launch_bounds__(256)
+    rows_kernel(int n_seqs, int64_t width, Blocks blocks, int64_t n_blocks, const int32_t* __restrict__ lens_out,
+                const int32_t* __restrict__ table, int64_t max_rows, const int32_t* __restrict__ cu_rows,
+                const int32_t* __restrict__ granted, int32_t* __restrict__ slots, int32_t* __restrict__ positions) {
+  griddep_launch_dependents();
+  griddep_wait();
+  for (int64_t t0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * 128; t0 < max_rows; t0 += (int64_t)gridDim.x * 8 * 128)
+    write_rows(t0, n_seqs, width, blocks, n_blocks, lens_out, table, max_rows, cu_rows, granted, slots, positions);
 }
 
 // Returns the blocks of the finished requests to the free list, in the order
@@ -551,12 +603,20 @@ int nimf_kv4_reserve_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_
       (max_rows > 0 && (!slots || !positions)))
     return set_error(NIMF_ERR_ARG, "kv4_reserve: NULL buffer");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  // One CTA writes about 10,000 rows in the time that a cluster's two barriers
-  // and eight launches cost.
-  const unsigned ctas = max_rows > 8192 ? 8 : 1;
-  return kv4::launch(kv4::reserve_kernel, dim3(ctas), kv4::kPoolThreads, 0, st, ctas, n_seqs,
-                     max_blocks, s.bs, s.n_blocks, n_new, lens, lens_out, block_table, free_blocks,
-                     n_free, n_free_out, max_rows, cu_rows, slots, positions, granted);
+  kv4::Blocks blocks;
+  blocks.bs = (uint32_t)s.bs;
+  blocks.magic = (((uint64_t)1 << 36) + s.bs / 16 - 1) / (s.bs / 16);
+  const bool own = max_rows <= kv4::kOwnRows || n_seqs == 0;
+  // as many threads as requests or warps' rows ask for: scans of few warps are short
+  const int64_t want = own ? std::max<int64_t>(n_seqs, max_rows / 4) : kv4::kPoolThreads;
+  const unsigned threads = want <= 128 ? 128 : want <= 256 ? 256 : want <= 512 ? 512 : kv4::kPoolThreads;
+  NIMF_TRY(kv4::launch(kv4::reserve_kernel, dim3(1), threads, 0, st, 1, (int)n_seqs, max_blocks, blocks, s.n_blocks,
+                       n_new, lens, lens_out, block_table, free_blocks, n_free, n_free_out, max_rows, cu_rows,
+                       slots, positions, granted, own ? 1 : 0));
+  if (own) return NIMF_OK;
+  return kv4::launch(kv4::rows_kernel, dim3(kv4::warp_grid((max_rows + 127) / 128)), 256, 0, st, 1, (int)n_seqs,
+                     max_blocks, blocks, s.n_blocks, (const int32_t*)lens_out, (const int32_t*)block_table, max_rows,
+                     (const int32_t*)cu_rows, (const int32_t*)granted, slots, positions);
 }
 
 int nimf_kv4_release_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
