@@ -141,6 +141,7 @@ struct Args {
   int64_t n_seqs, rows, width, n_blocks;
   int h, hkv, r, bs;
   float scale2;               // softmax scale * log2(e)
+  int uncut, wide;            // no segment is shared by CTAs; 64-bit sums of units
   int big;                    // sequences with more rows a KV head than this go to kv4_tc.cu
 };
 

@@ -141,92 +141,129 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
   }
   griddep_wait();
 
-  // ---- the line of units, and where this warp begins on it.  Every warp sums
-  // all sequences for itself: no barrier, one latency for 256 of them.
+  // ---- the line of units, and where this warp begins on it
   auto tiles_of = [&](int n) { return n * a.r > a.big ? 0 : seq_tiles<ROWS>(n, a.r); };
-  auto line_units = [&](int64_t b) -> int64_t {
-    if (b >= a.n_seqs) return 0;
-    const Seq s = seq_of(a, b);
-    return (int64_t)seq_units(s.len) * tiles_of(s.n) * a.hkv;
-  };
-  auto scan = [&](int64_t v) -> int64_t {   // inclusive, over the lanes
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, v, x);
-      if (lane >= x) v += u;
-    }
-    return v;
-  };
   const int64_t cta = blockIdx.x;
   SegInfo* info = reinterpret_cast<SegInfo*>(a.ws);
   float* parts = reinterpret_cast<float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
-  int64_t total = 0, mine = 0, upto = 0;    // of the last 32 sequences scanned
-#pragma unroll 1
-  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
-    mine = line_units(b0 + lane);
-    if (b0 + 32 < a.n_seqs) {               // only sums are needed of all but the last ones
-      int64_t more = 0;
+  int64_t total, ctas, each, more, cta_a, cta_b, w_a, w_b, b, off;
+  // Every warp sums all sequences for itself: no barrier, one latency for 256 of
+  // them.  T is 32 bits wide unless the host's bound of the line is wider: all
+  // warps of an SM do this at once, and the 64-bit sums and divisions took twice
+  // the time (2.6 us of a 20 us call).
+  auto plan = [&](auto zero) -> bool {
+    using T = decltype(zero);
+    auto line_units = [&](int64_t b) -> T {
+      if (b >= a.n_seqs) return 0;
+      const Seq s = seq_of(a, b);
+      return (T)seq_units(s.len) * (T)tiles_of(s.n) * (T)a.hkv;
+    };
+    auto scan = [&](T v) -> T {             // inclusive, over the lanes
 #pragma unroll
-      for (int i = 1; i < 8; ++i)
-        if (b0 + 32 * i < a.n_seqs) more += line_units(b0 + 32 * i + lane);
-      mine += more;
-      b0 += 32 * 7;
-    }
-    upto = scan(mine) + total;
-    total = __shfl_sync(0xffffffffu, upto, 31);
-  }
-  const int64_t ctas = max((int64_t)1, min((int64_t)gridDim.x, quot(total + W - 1, W)));
-  if (cta >= ctas || total == 0) {
-    if (tid == 0) info[cta].u0 = -1;
-    return;
-  }
-  const int64_t each = quot(total, ctas), more = total - each * ctas;
-  const int64_t cta_a = cut(cta, each, more), cta_b = cut(cta + 1, each, more);
-  const int64_t w_each = quot(cta_b - cta_a, W), w_more = cta_b - cta_a - w_each * W;
-  const int64_t w_a = cta_a + cut(warp, w_each, w_more), w_b = cta_a + cut(warp + 1, w_each, w_more);
-  if (lane < 2) s_seg[warp][lane].u0 = -1;
-  int64_t b = 0, off = 0;                   // the sequence of unit w_a, and the unit within it
-  if (a.n_seqs > 1) {
-#pragma unroll 1
-    for (int64_t b0 = 0, base = 0; b0 < a.n_seqs; b0 += 32) {
-      if (a.n_seqs > 32) {                  // otherwise they are still there
-        mine = line_units(b0 + lane);
-        upto = scan(mine) + base;
-        base = __shfl_sync(0xffffffffu, upto, 31);
+      for (int x = 1; x < 32; x <<= 1) {
+        const T u = __shfl_up_sync(0xffffffffu, v, x);
+        if (lane >= x) v += u;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, upto > w_a);
-      if (past) {
+      return v;
+    };
+    auto div = [](T x, T y) -> T { return (T)((sizeof(T) == 4) ? (uint32_t)x / (uint32_t)y : quot(x, y)); };
+    // Up to 256 sequences stay in registers, a lane each of eight chunks; more are
+    // summed 256 at a time, eight to a lane, and again where they are looked for.
+    const bool few = a.n_seqs <= 256;
+    auto eight = [&](int64_t b0) -> T {
+      T v = 0;
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) v += line_units(b0 + lane * 8 + i);
+      return v;
+    };
+    T units[8], upto[8], all = 0;
+    if (few) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        units[i] = 0;
+        if (32 * i < a.n_seqs) units[i] = line_units(32 * i + lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (32 * i < a.n_seqs) {
+          upto[i] = a.n_seqs == 1 ? units[i] : scan(units[i]) + all;
+          all = __shfl_sync(0xffffffffu, upto[i], a.n_seqs == 1 ? 0 : 31);
+        }
+    } else {
+#pragma unroll 1
+      for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) all += __shfl_sync(0xffffffffu, scan(eight(b0)), 31);
+    }
+    const T n_ctas = max((T)1, min((T)gridDim.x, div(all + W - 1, W)));
+    total = all;
+    ctas = n_ctas;
+    if (cta >= ctas || all == 0) return false;
+    // the sequence of a unit, and the unit within it
+    auto find = [&](T unit, int64_t& b, T& off) {
+      b = 0;
+      off = unit;
+      if (a.n_seqs == 1) return;
+      if (few) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (32 * i < a.n_seqs) {
+            const unsigned past = __ballot_sync(0xffffffffu, upto[i] > unit);
+            if (past) {
+              const int who = __ffs(past) - 1;
+              b = 32 * i + who;
+              off = unit - __shfl_sync(0xffffffffu, upto[i] - units[i], who);
+              return;
+            }
+          }
+        return;
+      }
+      T base = 0;
+#pragma unroll 1
+      for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) {
+        const T v = eight(b0), end = scan(v) + base;
+        base = __shfl_sync(0xffffffffu, end, 31);
+        const unsigned past = __ballot_sync(0xffffffffu, end > unit);
+        if (!past) continue;
         const int who = __ffs(past) - 1;
-        b = b0 + who;
-        off = w_a - __shfl_sync(0xffffffffu, upto - mine, who);
+        b = b0 + who * 8;
+        off = unit - __shfl_sync(0xffffffffu, end - v, who);
+        const T u = lane < 8 ? line_units(b + lane) : 0, sum = scan(u);
+        const int at = __ffs(__ballot_sync(0xffffffffu, sum > off)) - 1;  // which of that lane's eight
+        b += at;
+        off -= __shfl_sync(0xffffffffu, sum - u, at);
         break;
       }
+    };
+    const T t_each = div(all, n_ctas), t_more = all - t_each * n_ctas, me = (T)cta;
+    T first = me * t_each + min(me, t_more), last = first + t_each + (me < t_more ? 1 : 0), o;
+    if (a.uncut) {                          // the segments that begin in this CTA's part
+      auto next_segment = [&](T unit) -> T {
+        if (unit >= all) return all;
+        find(unit, b, o);
+        const T nu = (T)seq_units(seq_of(a, b).len), rem = o - div(o, nu) * nu;
+        return rem ? unit + nu - rem : unit;
+      };
+      first = next_segment(first);
+      last = next_segment(last);
+      if (first >= last) return false;
     }
-  } else {
-    off = w_a;
+    const T w_each = div(last - first, W), w_more = last - first - w_each * W, w = (T)warp;
+    const T mine = first + w * w_each + min(w, w_more);
+    find(mine, b, o);
+    off = o;
+    each = t_each;
+    more = t_more;
+    cta_a = first;
+    cta_b = last;
+    w_a = mine;
+    w_b = mine + w_each + (w < w_more ? 1 : 0);
+    return true;
+  };
+  if (!(a.wide ? plan((int64_t)0) : plan((int32_t)0))) {
+    if (tid == 0 && !a.uncut) info[cta].u0 = -1;
+    return;
   }
-  if (tid == 0) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
-    const Seq s = seq_of(a, b);
-    const int tiles = tiles_of(s.n), nu = seq_units(s.len);
-    const int64_t seg = quot(off, nu);
-    SegInfo si;
-    si.u0 = cta_a - (off - seg * nu);
-    si.u1 = si.u0 + nu;
-    si.row0 = s.row0;
-    si.n = s.n;
-    si.kvh = (int32_t)quot(seg, tiles);
-    si.tile = (int32_t)(seg - (int64_t)si.kvh * tiles);
-    const int64_t before = cut(cta - 1, each, more);
-    int64_t last = cta;                     // the CTA that holds its last unit
-    if (each > 0) last = max(cta, quot(si.u1 - 1, each + 1));
-    while (last + 1 < ctas && cut(last + 1, each, more) < si.u1) ++last;
-    si.parts = (int32_t)(last - (cta - 1) + 1);
-    si.second = si.u0 > before;
-    si.pad = 0;
-    if (si.u0 == cta_a || si.u0 < before) si.u0 = -1;
-    info[cta] = si;
-  }
-
+  if (lane < 2) s_seg[warp][lane].u0 = -1;
+  const int64_t b_first = b, off_first = off;
   uint8_t* ring = smem + (size_t)warp * kStages * 2 * TB;
   float* kept = reinterpret_cast<float*>(smem + (size_t)W * kStages * 2 * TB) + warp * PF;
   uint32_t phase = 0;                       // parity of each stage's next use
@@ -241,19 +278,19 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
     const int64_t seg = quot(off, nu);
     const int u_first = (int)(off - seg * nu);
     const int u_count = (int)min((int64_t)(nu - u_first), w_b - at);
-    const int kvh = (int)quot(seg, tiles), tile = (int)(seg - (int64_t)kvh * tiles);
+    const int kvh = tiles == 1 ? (int)seg : (int)quot(seg, tiles), tile = (int)(seg - (int64_t)kvh * tiles);
 
     // Rows of the tile: lane column g of B is row g / 2 (integer part, then
     // rest); scores, softmax and outputs of row c are with the lanes c.
     auto row_at = [&](int i, int& tok, int& hq) -> bool {
       const int rr = tile * ROWS + i;
-      tok = a.r == 1 ? rr : (int)((uint32_t)rr / (uint32_t)a.r);
+      tok = s.n == 1 ? (rr >= a.r) : a.r == 1 ? rr : (int)((uint32_t)rr / (uint32_t)a.r);
       hq = kvh * a.r + rr - tok * a.r;
       return rr < s.n * a.r;
     };
-    const int last_tok = min(s.n - 1, (tile * ROWS + ROWS - 1) / a.r);
+    const int last_tok = s.n == 1 ? 0 : min(s.n - 1, (int)((uint32_t)(tile * ROWS + ROWS - 1) / (uint32_t)a.r));
     const int seg_len = max(0, min(s.len, s.len - s.n + last_tok + 1));  // no row sees further
-    const int all_see = s.len - s.n + tile * ROWS / a.r + 1;             // every row sees these
+    const int all_see = s.len - s.n + (s.n == 1 ? 0 : (int)((uint32_t)(tile * ROWS) / (uint32_t)a.r)) + 1;             // every row sees these
     const int u_live = min(u_first + u_count, (seg_len + kUnit - 1) / kUnit);
 
     // this lane's part of the query rows, on its way while the tiles are found
@@ -612,7 +649,28 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
     off += u_count;
   }
 
-  // ---- pieces of one segment in neighbouring warps, a row a warp
+  // ---- for the join, and pieces of one segment in neighbouring warps, a row a warp
+  if (tid == 0 && !a.uncut) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
+    const Seq s = seq_of(a, b_first);
+    const int tiles = tiles_of(s.n), nu = seq_units(s.len);
+    const int64_t seg = quot(off_first, nu);
+    SegInfo si;
+    si.u0 = cta_a - (off_first - seg * nu);
+    si.u1 = si.u0 + nu;
+    si.row0 = s.row0;
+    si.n = s.n;
+    si.kvh = (int32_t)quot(seg, tiles);
+    si.tile = (int32_t)(seg - (int64_t)si.kvh * tiles);
+    const int64_t before = cut(cta - 1, each, more);
+    int64_t last = cta;                     // the CTA that holds its last unit
+    if (each > 0) last = max(cta, quot(si.u1 - 1, each + 1));
+    while (last + 1 < ctas && cut(last + 1, each, more) < si.u1) ++last;
+    si.parts = (int32_t)(last - (cta - 1) + 1);
+    si.second = si.u0 > before;
+    si.pad = 0;
+    if (si.u0 == cta_a || si.u0 < before) si.u0 = -1;
+    info[cta] = si;
+  }
   __syncthreads();
   constexpr int V = D / 32;
   auto piece_at = [&](int i) -> const float* {
@@ -742,6 +800,7 @@ int run_nb(const Args& a, cudaStream_t st) {
   NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
   const int ctas = grid_of(D, NB);
   NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
+  if (a.uncut) return NIMF_OK;
   return launch(join_kernel<D, NB>, dim3(ctas), kJoinWarps * 32, 0, st, 1, a);
 }
 
@@ -831,6 +890,12 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   a.r = (int)(n_heads / s.hkv);
   a.bs = s.bs;
   a.scale2 = (float)((double)scale * 1.4426950408889634);
+  // Short contexts: a CTA takes whole segments, so nothing is left to join.  A
+  // segment of 24 units costs a CTA two units more a warp (2 us) than a cut one,
+  // the join's launch and latency 3 us.
+  a.uncut = max_blocks * s.bs <= 24 * kv4::kUnit;
+  // an upper bound of the line of units: every row tile over a whole table row
+  a.wide = ((double)rows * a.r / 4 + (double)n_seqs) * s.hkv * ((double)max_blocks * s.bs / kv4::kUnit + 1) > 1e9;
   a.big = INT32_MAX;
   if (kv4::tc_serves(s.d) && max_new * a.r > kv4::kBigRows) {
     a.big = kv4::kBigRows;

@@ -597,19 +597,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int j = 0; j < OP; ++j) o[j][i] = mul2(o[j][i], c2);
         }
+      float acc[NS][32];
 #pragma unroll
-      for (int k = 0; k < NS; ++k) {
-        float acc[32];
-        tmem_ld_frag(my_at + 256 + x * D + 64 * k, acc);
-        tmem_wait_ld();
+      for (int k = 0; k < NS; ++k) tmem_ld_frag(my_at + 256 + x * D + 64 * k, acc[k]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < NS; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float f1 = fac[(64 * k + 8 * j) / G];
           const f2 f = pk(f1, f1);
-          o[8 * k + j][0] = fma2(pk(acc[4 * j], acc[4 * j + 1]), f, o[8 * k + j][0]);
-          o[8 * k + j][1] = fma2(pk(acc[4 * j + 2], acc[4 * j + 3]), f, o[8 * k + j][1]);
+          o[8 * k + j][0] = fma2(pk(acc[k][4 * j], acc[k][4 * j + 1]), f, o[8 * k + j][0]);
+          o[8 * k + j][1] = fma2(pk(acc[k][4 * j + 2], acc[k][4 * j + 3]), f, o[8 * k + j][1]);
         }
-      }
       tc_fence_before();
     };
     constexpr int CH = N < 64 ? N : 64, CP = CH / 8;  // columns, pairs of a lane, of a TMEM access
@@ -623,12 +623,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // x of 2 rows x NP pairs of tokens
       f2 x[NP][2];
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < NG; ++n) {
+        float sc[N / CH][CP * 4];
 #pragma unroll
-        for (int k = 0; k < N / CH; ++k) {
-          float sc[CP * 4];
-          tmem_ld_frag(s_at + n * N + k * CH, sc);
-          tmem_wait_ld();
+        for (int k = 0; k < N / CH; ++k) tmem_ld_frag(s_at + n * N + k * CH, sc[k]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < N / CH; ++k)
 #pragma unroll
           for (int j = 0; j < CP; ++j) {
             const float4 p = prm[n * (N / 2) + 4 * (k * CP + j)];
@@ -637,10 +638,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int i = 0; i < 2; ++i) {
               f2& v = x[k * CP + j][i];
               const f2 b = n ? fma2(qs[n][i], km, v) : mul2(qs[n][i], km);
-              v = fma2(pk(sc[4 * j + 2 * i], sc[4 * j + 2 * i + 1]), ks, b);
+              v = fma2(pk(sc[k][4 * j + 2 * i], sc[k][4 * j + 2 * i + 1]), ks, b);
             }
           }
-        }
+      }
       const bool cut = (t_first + t + 1) * N > all_see;  // some row does not see all of the tile
       if (cut)
 #pragma unroll
