@@ -32,8 +32,14 @@ namespace {
 
 constexpr int kUnit = 32;        // tokens a warp takes at a time (two tiles)
 constexpr int kStages = 2;       // units in flight per warp
-// Warps of a CTA: with the ring of a 256-channel tile, six fill the shared memory.
-__host__ __device__ constexpr int warps_of(int d) { return d <= 128 ? 8 : 6; }
+// Warps of a CTA, CTAs of an SM.  16 warps with 128 registers a thread fill an
+// SM: in one CTA where their rings fit its shared memory, so that more of a
+// segment is joined there, else in two.  More rows a segment need twice the
+// registers; with the ring of a 256-channel tile six warps fill the shared memory.
+__host__ __device__ constexpr int warps_of(int d, int ng, int nb) {
+  return d > 128 ? 6 : nb == 1 && ng <= 2 ? 16 : 8;
+}
+__host__ __device__ constexpr int ctas_per_sm(int d, int ng, int nb) { return d <= 128 && nb == 1 && ng > 2 ? 2 : 1; }
 
 // A kept piece of a segment, and (in the workspace) the segment that a CTA's
 // beginning cuts first: u0 its first unit on the line, -1 for none.
@@ -52,11 +58,9 @@ __host__ __device__ constexpr int rows_of(int nb) { return 4 * nb; }
 constexpr int kMaxNB = 4;
 __host__ __device__ constexpr int part_floats(int d, int nb) { return rows_of(nb) * (d + 2); }
 
-// CTAs of an SM: two where 128 registers a thread hold a segment's state.
-__host__ __device__ constexpr int ctas_per_sm(int d, int nb) { return d <= 128 && nb == 1 ? 2 : 1; }
 // Rings, then one kept piece per warp.
 constexpr int attn_smem(int d, int ng, int nb) {
-  return warps_of(d) * (kStages * 2 * tile_bytes(d, ng) + part_floats(d, nb) * 4);
+  return warps_of(d, ng, nb) * (kStages * 2 * tile_bytes(d, ng) + part_floats(d, nb) * 4);
 }
 
 size_t ws_bytes(int ctas, int d) {
@@ -125,8 +129,8 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
 //
 // Each warp streams its tiles with bulk copies into its own two-stage ring.
 template <int D, int NG, int NB>
-__global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_kernel(const Args a) {
-  constexpr int NC = D / 32, NS = D / 64, G = D / NG, W = warps_of(D);
+__global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, NB)) attn_kernel(const Args a) {
+  constexpr int NC = D / 32, NS = D / 64, G = D / NG, W = warps_of(D, NG, NB);
   constexpr int TB = tile_bytes(D, NG), PF = part_floats(D, NB), ROWS = rows_of(NB);
   constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // codes, and 16 times them
   extern __shared__ __align__(128) uint8_t smem[];
@@ -701,14 +705,13 @@ __global__ void __launch_bounds__(warps_of(D) * 32, ctas_per_sm(D, NB)) attn_ker
       const float pm = in ? mine_p[ROWS * D + row] : -INFINITY;
       float top = pm;
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      top = __shfl_sync(0xffffffffu, top, 0);
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float f = ex2(pm - (top == -INFINITY ? 0.f : top));
       float pl = in ? mine_p[ROWS * D + ROWS + row] * f : 0.f;
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, x);
+      for (int x = 16; x > 0; x >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, x);
       all.m = top;
-      all.l = __shfl_sync(0xffffffffu, pl, 0);
+      all.l = pl;
 #pragma unroll 1
       for (unsigned rest = members; rest; rest &= rest - 1) {
         const int who = __ffs(rest) - 1;
@@ -789,17 +792,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
   store_v<V>(a.out + ((si.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
 }
 
-int grid_of(int d, int nb) {
+int grid_of(int d, int ng, int nb) {
   Context* c = ctx();
-  return (c ? c->num_sms : 148) * ctas_per_sm(d, nb);
+  return (c ? c->num_sms : 148) * ctas_per_sm(d, ng, nb);
 }
 
 template <int D, int NG, int NB>
 int run_nb(const Args& a, cudaStream_t st) {
   const int smem = attn_smem(D, NG, NB);
   NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
-  const int ctas = grid_of(D, NB);
-  NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D) * 32, smem, st, 1, a));
+  const int ctas = grid_of(D, NG, NB);
+  NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D, NG, NB) * 32, smem, st, 1, a));
   if (a.uncut) return NIMF_OK;
   return launch(join_kernel<D, NB>, dim3(ctas), kJoinWarps * 32, 0, st, 1, a);
 }
@@ -817,7 +820,7 @@ int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
   return run_nb<D, NG, 2>(a, st);
 }
 
-size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 1), d) + 255) / 256 * 256; }
+size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 4, 1), d) + 255) / 256 * 256; }
 size_t all_ws_bytes(int d) { return few_ws_bytes(d) + (tc_serves(d) ? tc_ws_bytes(d) : 0); }
 
 // Rows a KV head from which a sequence is worth the tensor-core kernel's tiles
