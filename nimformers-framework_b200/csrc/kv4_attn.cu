@@ -681,23 +681,33 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     return i & 1 ? reinterpret_cast<const float*>(smem + (size_t)(i >> 1) * kStages * 2 * TB)
                  : reinterpret_cast<const float*>(smem + (size_t)W * kStages * 2 * TB) + (i >> 1) * PF;
   };
-  // which of the 2 W places hold a piece, and which begin another segment
+  // which of the 2 W places hold a piece and which begin another segment, a lane
+  // each, and the tasks (rows of segments) up to there
   const int64_t my_u0 = lane < 2 * W ? s_seg[lane >> 1][lane & 1].u0 : -1;
   const unsigned used = __ballot_sync(0xffffffffu, my_u0 >= 0);
   const int prev = 31 - __clz(used & ((1u << lane) - 1u));
   const int64_t prev_u0 = __shfl_sync(0xffffffffu, my_u0, max(prev, 0));
-  const unsigned first = __ballot_sync(0xffffffffu, my_u0 >= 0 && (prev < 0 || prev_u0 != my_u0));
-  int task = 0;
-  for (unsigned todo = first; todo; todo &= todo - 1) {
-    const int i0 = __ffs(todo) - 1;
-    const unsigned later = todo & (todo - 1);
+  const bool is_first = my_u0 >= 0 && (prev < 0 || prev_u0 != my_u0);
+  const unsigned first = __ballot_sync(0xffffffffu, is_first);
+  int my_rows = 0;
+  if (is_first) my_rows = min(ROWS, s_seg[lane >> 1][lane & 1].n * a.r - s_seg[lane >> 1][lane & 1].tile * ROWS);
+  int tasks = my_rows;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, tasks, x);
+    if (lane >= x) tasks += v;
+  }
+  const int all_tasks = __shfl_sync(0xffffffffu, tasks, 31);
+#pragma unroll 1
+  for (int task = warp; task < all_tasks; task += W) {
+    const int i0 = __ffs(__ballot_sync(0xffffffffu, tasks > task)) - 1;
+    const int row = task - __shfl_sync(0xffffffffu, tasks - my_rows, i0);
+    const unsigned later = i0 == 31 ? 0u : first & ~((2u << i0) - 1u);
     const unsigned members = used & ~((1u << i0) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : ~0u);
-    const SegInfo si = s_seg[i0 >> 1][i0 & 1];
+    const SegInfo& si = s_seg[i0 >> 1][i0 & 1];
     const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
     float* slot = parts + (size_t)(2 * cta + (si.u0 <= cta_a ? 0 : 1)) * PF;
-    const int rows = min(ROWS, si.n * a.r - si.tile * ROWS);
-    for (int row = 0; row < rows; ++row, ++task) {
-      if (task % W != warp) continue;
+    {
       // the members' maxima and sums, a lane each; then their outputs
       Merged<V> all;
       const bool in = members >> lane & 1u;
