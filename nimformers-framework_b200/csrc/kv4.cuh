@@ -142,7 +142,8 @@ struct Args {
   int h, hkv, r, bs;
   float scale2;               // softmax scale * log2(e)
   int uncut, wide;            // no segment is shared by CTAs; 64-bit sums of units
-  int big;                    // sequences with more rows a KV head than this go to kv4_tc.cu
+  int big;                    // sequences with more rows a KV head than this go to kv4_tc.cu (INT32_MAX: none)
+  int sms;                    // CTAs of kv4_tc.cu that run at once
 };
 
 // Sequence b as the kernels see it: its rows [row0, row0 + n) and its cached
@@ -226,10 +227,61 @@ __device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) 
 }
 
 // Attention of sequences with more than a.big rows a KV head, on tcgen05
-// (kv4_tc.cu): head dims and groups served, workspace, launch.
+// (kv4_tc.cu): 128 rows of one KV head an item, items of few tokens parts where
+// the items would leave SMs idle.  A part is the rows' outputs, maxima and sums.
+constexpr int kTcRows = 128;
+__device__ __forceinline__ int big_tiles(const Args& a, int n) {
+  return n * a.r > a.big ? (n * a.r + kTcRows - 1) / kTcRows : 0;
+}
+// Parts of an item: as many as run at once, each of four tiles of tokens or more.
+__device__ __forceinline__ int item_splits(const Args& a, int items, int token_tiles) {
+  return max(1, min(a.sms / max(items, 1), token_tiles / 4));
+}
+__host__ __device__ constexpr size_t tc_part_floats(int d) { return (size_t)kTcRows * (d + 2); }
+// The sequence and its tile of rows of index i, counted from the end (the last
+// rows see most tokens: the longest go first), and the number of all tiles.
+// Every lane of a warp gets them.
+__device__ __forceinline__ bool find_tile(const Args& a, int index, int& b, int& tile, int& total) {
+  const int lane = threadIdx.x & 31;
+  total = 0;
+  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
+    const int64_t x = b0 + lane;
+    total += __reduce_add_sync(0xffffffffu, x < a.n_seqs ? big_tiles(a, seq_of(a, x).n) : 0);
+  }
+  if (index >= total) return false;
+  int want = total - 1 - index, base = 0;
+  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
+    const int64_t x = b0 + lane;
+    const int t = x < a.n_seqs ? big_tiles(a, seq_of(a, x).n) : 0;
+    int upto = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base + upto > want);
+    if (past) {
+      const int who = __ffs(past) - 1;
+      tile = want - base - __shfl_sync(0xffffffffu, upto - t, who);
+      b = (int)b0 + who;
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+// Tokens that some row of the tile sees.
+__device__ __forceinline__ int tile_len(const Args& a, const Seq& s, int tile) {
+  const int rows = min(kTcRows, s.n * a.r - tile * kTcRows);
+  const int last_tok = (int)((uint32_t)(tile * kTcRows + rows - 1) / (uint32_t)a.r);
+  return max(0, min(s.len, s.len - s.n + last_tok + 1));
+}
+
+// Head dims served, workspace, items that a call may have at most, launch.
 bool tc_serves(int d);
 size_t tc_ws_bytes(int d);
-int run_tc(const Args& a, int d, int ng, int64_t max_blocks, unsigned char* ws, cudaStream_t st);
+int64_t tc_items(const Args& a);
+int run_tc(const Args& a, int d, int ng, unsigned char* ws, cudaStream_t st);
 
 }  // namespace kv4
 }  // namespace nimf

@@ -21,6 +21,7 @@
 // out; sums of the integer columns stay below 2^24 and are exact, the rests
 // are small, and so products and sums have float32's accuracy.  w's integers
 // count from the largest w of the 32 tokens of a unit.
+#include <algorithm>
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -51,6 +52,13 @@ struct SegInfo {
   int32_t parts;    // join: CTAs that hold a part, counted from the one before
   int32_t second;   // join: the first of them holds it as its last segment
   int32_t pad;
+};
+
+// What a CTA's end needs to know of its part of the line: how CTAs' parts are
+// cut, its own [begin, end), where it begins (unit off of sequence b), CTAs in
+// use.  It lies in shared memory: in registers it cost spills in the main loop.
+struct Line {
+  int64_t each, more, begin, end, off, b, ctas;
 };
 
 // A segment's query rows: 4 per column tile of the MMA's B operand.
@@ -120,6 +128,24 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// The SMs that tc_kernel leaves idle, or 0 if taking all SMs later is as fast:
+// its tiles take about as long for 32 tokens as a unit here, its longest sequence
+// thus as long as the wait for its SMs.  units: of a warp on all SMs.
+__device__ __forceinline__ int idle_sms(const Args& a, float units) {
+  const int lane = threadIdx.x & 31;
+  int items = 0, longest = 0;
+#pragma unroll 1
+  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
+    const Seq s = b0 + lane < a.n_seqs ? seq_of(a, b0 + lane) : Seq{};
+    const int t = big_tiles(a, s.n);
+    items += __reduce_add_sync(0xffffffffu, t);
+    longest = max(longest, __reduce_max_sync(0xffffffffu, t ? s.len : 0));
+  }
+  items *= a.hkv;
+  const int idle = a.sms - items * max(1, a.sms / max(items, 1));
+  return idle > 0 && units * (float)(a.sms - idle) * kUnit <= (float)longest * (float)idle ? idle : 0;
+}
+
 // Work: a segment is 4 NB query rows (tokens x heads of one KV head) of one
 // sequence over all its tokens; its units are 32 tokens.  All units of all
 // segments lie on one line that is cut evenly among the warps of a grid that
@@ -128,13 +154,18 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
 // that other CTAs continue go to the workspace for join_kernel.
 //
 // Each warp streams its tiles with bulk copies into its own two-stage ring.
-template <int D, int NG, int NB>
+//
+// BESIDE: launched behind tc_kernel, which has waited for what came before when
+// this kernel starts; the two run side by side on different SMs, and this grid
+// ends (its first CTA does) after that one.
+template <int D, int NG, int NB, bool BESIDE>
 __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, NB)) attn_kernel(const Args a) {
   constexpr int NC = D / 32, NS = D / 64, G = D / NG, W = warps_of(D, NG, NB);
   constexpr int TB = tile_bytes(D, NG), PF = part_floats(D, NB), ROWS = rows_of(NB);
   constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // codes, and 16 times them
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[W][kStages];
+  __shared__ Line s_line;
   __shared__ SegInfo s_seg[W][2];           // kept pieces: at the warp's first unit, at its last
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -143,14 +174,15 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     for (int i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1);
     mbar_fence_init();
   }
-  griddep_wait();
+  if constexpr (BESIDE) __syncwarp();
+  else griddep_wait();
 
   // ---- the line of units, and where this warp begins on it
   auto tiles_of = [&](int n) { return n * a.r > a.big ? 0 : seq_tiles<ROWS>(n, a.r); };
   const int64_t cta = blockIdx.x;
   SegInfo* info = reinterpret_cast<SegInfo*>(a.ws);
   float* parts = reinterpret_cast<float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
-  int64_t total, ctas, each, more, cta_a, cta_b, w_a, w_b, b, off;
+  int64_t w_a, w_b, b, off;
   // Every warp sums all sequences for itself: no barrier, one latency for 256 of
   // them.  T is 32 bits wide unless the host's bound of the line is wider: all
   // warps of an SM do this at once, and the 64-bit sums and divisions took twice
@@ -197,10 +229,13 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
 #pragma unroll 1
       for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) all += __shfl_sync(0xffffffffu, scan(eight(b0)), 31);
     }
-    const T n_ctas = max((T)1, min((T)gridDim.x, div(all + W - 1, W)));
-    total = all;
-    ctas = n_ctas;
-    if (cta >= ctas || all == 0) return false;
+    T grid = (T)gridDim.x;
+    if constexpr (BESIDE) {
+      const int idle = idle_sms(a, (float)all / W / (float)gridDim.x);
+      if (idle > 0) grid = (T)(gridDim.x / a.sms * idle);
+    }
+    const T n_ctas = max((T)1, min(grid, div(all + W - 1, W)));
+    if (cta >= n_ctas || all == 0) return false;
     // the sequence of a unit, and the unit within it
     auto find = [&](T unit, int64_t& b, T& off) {
       b = 0;
@@ -254,20 +289,17 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     const T mine = first + w * w_each + min(w, w_more);
     find(mine, b, o);
     off = o;
-    each = t_each;
-    more = t_more;
-    cta_a = first;
-    cta_b = last;
+    if (tid == 0) s_line = {t_each, t_more, first, last, o, b, n_ctas};
     w_a = mine;
     w_b = mine + w_each + (w < w_more ? 1 : 0);
     return true;
   };
   if (!(a.wide ? plan((int64_t)0) : plan((int32_t)0))) {
     if (tid == 0 && !a.uncut) info[cta].u0 = -1;
+    if (BESIDE && cta == 0) griddep_wait();
     return;
   }
   if (lane < 2) s_seg[warp][lane].u0 = -1;
-  const int64_t b_first = b, off_first = off;
   uint8_t* ring = smem + (size_t)warp * kStages * 2 * TB;
   float* kept = reinterpret_cast<float*>(smem + (size_t)W * kStages * 2 * TB) + warp * PF;
   uint32_t phase = 0;                       // parity of each stage's next use
@@ -655,24 +687,25 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
 
   // ---- for the join, and pieces of one segment in neighbouring warps, a row a warp
   if (tid == 0 && !a.uncut) {  // the segment cut by this CTA's beginning, joined in its name if that is its first cut
-    const Seq s = seq_of(a, b_first);
+    const Seq s = seq_of(a, s_line.b);
     const int tiles = tiles_of(s.n), nu = seq_units(s.len);
-    const int64_t seg = quot(off_first, nu);
+    const Line l = s_line;
+    const int64_t seg = quot(l.off, nu);
     SegInfo si;
-    si.u0 = cta_a - (off_first - seg * nu);
+    si.u0 = l.begin - (l.off - seg * nu);
     si.u1 = si.u0 + nu;
     si.row0 = s.row0;
     si.n = s.n;
     si.kvh = (int32_t)quot(seg, tiles);
     si.tile = (int32_t)(seg - (int64_t)si.kvh * tiles);
-    const int64_t before = cut(cta - 1, each, more);
+    const int64_t before = cut(cta - 1, l.each, l.more);
     int64_t last = cta;                     // the CTA that holds its last unit
-    if (each > 0) last = max(cta, quot(si.u1 - 1, each + 1));
-    while (last + 1 < ctas && cut(last + 1, each, more) < si.u1) ++last;
+    if (l.each > 0) last = max(cta, quot(si.u1 - 1, l.each + 1));
+    while (last + 1 < l.ctas && cut(last + 1, l.each, l.more) < si.u1) ++last;
     si.parts = (int32_t)(last - (cta - 1) + 1);
     si.second = si.u0 > before;
     si.pad = 0;
-    if (si.u0 == cta_a || si.u0 < before) si.u0 = -1;
+    if (si.u0 == l.begin || si.u0 < before) si.u0 = -1;
     info[cta] = si;
   }
   __syncthreads();
@@ -681,6 +714,7 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     return i & 1 ? reinterpret_cast<const float*>(smem + (size_t)(i >> 1) * kStages * 2 * TB)
                  : reinterpret_cast<const float*>(smem + (size_t)W * kStages * 2 * TB) + (i >> 1) * PF;
   };
+  const int64_t begin = s_line.begin, end = s_line.end;
   // which of the 2 W places hold a piece and which begin another segment, a lane
   // each, and the tasks (rows of segments) up to there
   const int64_t my_u0 = lane < 2 * W ? s_seg[lane >> 1][lane & 1].u0 : -1;
@@ -705,8 +739,8 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     const unsigned later = i0 == 31 ? 0u : first & ~((2u << i0) - 1u);
     const unsigned members = used & ~((1u << i0) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : ~0u);
     const SegInfo& si = s_seg[i0 >> 1][i0 & 1];
-    const bool whole = si.u0 >= cta_a && si.u1 <= cta_b;
-    float* slot = parts + (size_t)(2 * cta + (si.u0 <= cta_a ? 0 : 1)) * PF;
+    const bool whole = si.u0 >= begin && si.u1 <= end;
+    float* slot = parts + (size_t)(2 * cta + (si.u0 <= begin ? 0 : 1)) * PF;
     {
       // the members' maxima and sums, a lane each; then their outputs
       Merged<V> all;
@@ -744,24 +778,48 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
       }
     }
   }
+  if (BESIDE && cta == 0) griddep_wait();
 }
 
 // Joins the segments that several CTAs share.  Block i: the segment that CTA
 // i's beginning cuts, if that is the segment's first cut.  Its rows are shared
 // by the warps, several warps a row where there are few; every result is taken
-// in a fixed order, so it does not depend on timing.
+// in a fixed order, so it does not depend on timing.  The blocks behind them
+// join the parts of tc_kernel's items, four blocks an item and a warp a row.
 constexpr int kJoinWarps = 16;
-template <int D, int NB>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
+template <int D, int NB, bool BESIDE>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a, int ctas, const float* tc_parts, int tc_tokens) {
   constexpr int PF = part_floats(D, NB), ROWS = rows_of(NB), V = D / 32;
   __shared__ __align__(16) float s_o[kJoinWarps][D];
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t cta = blockIdx.x;
+  const int64_t cta = BESIDE && a.uncut ? blockIdx.x + ctas : blockIdx.x;
+  if (BESIDE && cta >= ctas) {
+    int b = 0, tile = 0, total = 0;
+    const int item = (int)(cta - ctas) / 4, kvh = item % a.hkv;
+    if (!find_tile(a, item / a.hkv, b, tile, total)) return;
+    const int items = total * a.hkv, cut = max(1, a.sms / items);
+    const Seq s = seq_of(a, b);
+    const int splits = item_splits(a, items, (tile_len(a, s, tile) + tc_tokens - 1) / tc_tokens);
+    if (splits == 1) return;
+    const int row0 = tile * kTcRows, rows = min(kTcRows, s.n * a.r - row0);
+    for (int row = (int)(cta - ctas) % 4 * kJoinWarps + warp; row < rows; row += 4 * kJoinWarps) {
+      Merged<V> all;
+      for (int j = 0; j < splits; ++j) {
+        const float* p = tc_parts + (size_t)(item * cut + j) * tc_part_floats(D);
+        float po[V];
+        load_v<V>(p + row * D + lane * V, po);
+        all.take(p[kTcRows * D + row], p[kTcRows * (D + 1) + row], po);
+      }
+      const int rr = row0 + row, tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
+      store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
+    }
+    return;
+  }
   const SegInfo si = reinterpret_cast<const SegInfo*>(a.ws)[cta];
-  const float* parts = reinterpret_cast<const float*>(a.ws + (size_t)gridDim.x * sizeof(SegInfo));
+  const float* parts = reinterpret_cast<const float*>(a.ws + (size_t)ctas * sizeof(SegInfo));
   if (si.u0 < 0) return;
   const int rows = min(ROWS, si.n * a.r - si.tile * ROWS);
   const int groups = rows == 1 ? kJoinWarps : rows == 2 ? kJoinWarps / 2 : kJoinWarps / (rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
@@ -807,31 +865,40 @@ int grid_of(int d, int ng, int nb) {
   return (c ? c->num_sms : 148) * ctas_per_sm(d, ng, nb);
 }
 
-template <int D, int NG, int NB>
+size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 4, 1), d) + 255) / 256 * 256; }
+size_t all_ws_bytes(int d) { return few_ws_bytes(d) + (tc_serves(d) ? tc_ws_bytes(d) : 0); }
+
+template <int D, int NG, int NB, bool BESIDE>
 int run_nb(const Args& a, cudaStream_t st) {
   const int smem = attn_smem(D, NG, NB);
-  NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB>, smem));
+  NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB, BESIDE>, smem));
   const int ctas = grid_of(D, NG, NB);
-  NIMF_TRY(launch(attn_kernel<D, NG, NB>, dim3(ctas), warps_of(D, NG, NB) * 32, smem, st, 1, a));
-  if (a.uncut) return NIMF_OK;
-  return launch(join_kernel<D, NB>, dim3(ctas), kJoinWarps * 32, 0, st, 1, a);
+  NIMF_TRY(launch(attn_kernel<D, NG, NB, BESIDE>, dim3(ctas), warps_of(D, NG, NB) * 32, smem, st, 1, a));
+  // tc_kernel's items have parts where they fill half the SMs or less
+  const int64_t tc_blocks = BESIDE ? 4 * std::min<int64_t>(tc_items(a), a.sms / 2) : 0;
+  const int64_t blocks = (a.uncut ? 0 : ctas) + tc_blocks;
+  if (blocks == 0) return NIMF_OK;
+  return launch(join_kernel<D, NB, BESIDE>, dim3((unsigned)blocks), kJoinWarps * 32, 0, st, 1, a, ctas,
+                (const float*)(a.ws + few_ws_bytes(D)), 128 / NG);
 }
 
 // 4 rows a segment where no sequence should have more of them for a KV head,
 // 8 or 16 where one may: each pass over a sequence's tiles serves more rows,
 // at more registers and partial results.  Beside sequences of many rows, which
 // go elsewhere, the others are taken for decoding ones with one row a head.
+template <int D, int NG, bool BESIDE>
+int run_rows(const Args& a, int64_t rows, cudaStream_t st) {
+  if (rows <= 4) return run_nb<D, NG, 1, BESIDE>(a, st);
+  if constexpr (D <= 128)
+    if (rows > 8) return run_nb<D, NG, 4, BESIDE>(a, st);
+  return run_nb<D, NG, 2, BESIDE>(a, st);
+}
 template <int D, int NG>
 int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
-  const int64_t rows = a.big < INT32_MAX ? a.r : max_new * a.r;
-  if (rows <= 4) return run_nb<D, NG, 1>(a, st);
   if constexpr (D <= 128)
-    if (rows > 8) return run_nb<D, NG, 4>(a, st);
-  return run_nb<D, NG, 2>(a, st);
+    if (a.big < INT32_MAX) return run_rows<D, NG, true>(a, a.r, st);
+  return run_rows<D, NG, false>(a, max_new * a.r, st);
 }
-
-size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 4, 1), d) + 255) / 256 * 256; }
-size_t all_ws_bytes(int d) { return few_ws_bytes(d) + (tc_serves(d) ? tc_ws_bytes(d) : 0); }
 
 // Rows a KV head from which a sequence is worth the tensor-core kernel's tiles
 // of 128: such a tile costs about what 16 rows cost here (1.1 against 1.2 us
@@ -910,9 +977,10 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   // an upper bound of the line of units: every row tile over a whole table row
   a.wide = ((double)rows * a.r / 4 + (double)n_seqs) * s.hkv * ((double)max_blocks * s.bs / kv4::kUnit + 1) > 1e9;
   a.big = INT32_MAX;
+  a.sms = ctx()->num_sms;
   if (kv4::tc_serves(s.d) && max_new * a.r > kv4::kBigRows) {
     a.big = kv4::kBigRows;
-    NIMF_TRY(kv4::run_tc(a, s.d, s.d / s.group, max_blocks, a.ws + kv4::few_ws_bytes(s.d), st));
+    NIMF_TRY(kv4::run_tc(a, s.d, s.d / s.group, a.ws + kv4::few_ws_bytes(s.d), st));
   }
   switch (s.d * 16 + s.d / s.group) {
     case 64 * 16 + 1: return kv4::run_attn<64, 1>(a, max_new, st);

@@ -41,10 +41,11 @@ int allow_smem(const void* kern, int bytes) {
     const void* kern;
     int device, bytes;
   };
-  static Done done[32];                      // zero: a free place
+  constexpr int kKernels = 64;
+  static Done done[kKernels];                // zero: a free place
   const int device = ctx()->device;
   Done* d = done;
-  while (d < done + 31 && d->kern && d->kern != kern) ++d;
+  while (d < done + kKernels - 1 && d->kern && d->kern != kern) ++d;
   if (d->kern == kern && d->device == device && d->bytes >= bytes) return NIMF_OK;
   NIMF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   *d = {kern, device, bytes};

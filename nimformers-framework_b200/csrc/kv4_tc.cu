@@ -32,7 +32,6 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kTcRows = 128;
 constexpr int kTcThreads = 512;     // 8 softmax warps, 4 of unpack, 1 of MMA issue
 constexpr int kUnpack0 = 256;       // first unpack thread
 constexpr int kPrmSlots = 4;        // tiles whose scales and minima are held
@@ -52,8 +51,6 @@ struct TcLayout {
   static constexpr int BAR = ROW + (1 + NG) * 128 * 4;                 // barriers
   static constexpr int SIZE = BAR + 256;
 };
-
-size_t part_bytes(int d) { return (size_t)kTcRows * (d + 2) * 4; }
 
 // ------------------------------------------------------------ PTX
 // Descriptors (smem_desc's) as their two halves: the upper one is a constant of
@@ -153,63 +150,21 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Tiles of 128 rows of a sequence here, and the sequence and tile of index i
-// counted from the end (the last rows see most tokens: the longest go first).
-__device__ __forceinline__ int big_tiles(const Args& a, int n) {
-  return n * a.r > a.big ? (n * a.r + kTcRows - 1) / kTcRows : 0;
-}
-__device__ __forceinline__ bool find_tile(const Args& a, int index, int& b, int& tile) {
-  const int lane = threadIdx.x & 31;
-  int total = 0;
-  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
-    const int64_t x = b0 + lane;
-    int t = x < a.n_seqs ? big_tiles(a, seq_of(a, x).n) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    total += t;
-  }
-  if (index >= total) return false;
-  int want = total - 1 - index, base = 0;
-  for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 32) {
-    const int64_t x = b0 + lane;
-    const int t = x < a.n_seqs ? big_tiles(a, seq_of(a, x).n) : 0;
-    int upto = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, base + upto > want);
-    if (past) {
-      const int who = __ffs(past) - 1;
-      tile = want - base - __shfl_sync(0xffffffffu, upto - t, who);
-      b = (int)b0 + who;
-      return true;
-    }
-    base += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return false;
-}
-
 template <int D, int NG>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    tc_kernel(const Args a, int splits, unsigned char* parts) {
+    tc_kernel(const Args a, unsigned char* parts) {
   using L = TcLayout<D, NG>;
   constexpr int N = L::N, G = D / NG, NC = D / 32, NS = D / 64, TB = tile_bytes(D, NG);
   constexpr int SB_D = D * 16, SB_N = N * 16;   // 8-row groups of operands with D, N columns of K
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_where[3];
+  __shared__ int s_where[4];
   __shared__ int s_stop;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6;
   uint64_t *s_full = bar + 8, *p_full = bar + 10, *o_full = bar + 12, *prm_full = bar + 14;
   uint64_t *q_full = bar + 18, *all_done = bar + 19;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
-  const int kvh = item % a.hkv;
-
-  griddep_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 128);
@@ -227,26 +182,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_fence_init();
   }
   griddep_wait();
+  griddep_launch_dependents();                  // attn_kernel: what came before is complete
   if (warp == 0) {
-    int b = 0, tile = 0;
-    const bool ok = find_tile(a, item / a.hkv, b, tile);
+    // the items' number gives their parts, so the item of a CTA is known after it
+    int b = 0, tile = 0, total = 0;
+    find_tile(a, INT32_MAX, b, tile, total);
+    const int items = total * a.hkv, cut = max(1, a.sms / max(items, 1));
+    const int item = blockIdx.x / cut;
+    const bool ok = find_tile(a, item / a.hkv, b, tile, total);
     if (lane == 0) {
-      s_where[0] = ok;
+      s_where[0] = ok ? cut : 0;
       s_where[1] = b;
       s_where[2] = tile;
+      s_where[3] = items;
     }
   }
   __syncthreads();
   if (!s_where[0]) return;                      // more CTAs than tiles: the host knows a bound
+  const int split = blockIdx.x % s_where[0], item = blockIdx.x / s_where[0];
+  const int kvh = item % a.hkv;
   const int b = s_where[1], tile = s_where[2];
   const Seq s = seq_of(a, b);
   const int rows = min(kTcRows, s.n * a.r - tile * kTcRows);
   const int first_tok = (int)((uint32_t)(tile * kTcRows) / (uint32_t)a.r);
-  const int last_tok = (int)((uint32_t)(tile * kTcRows + rows - 1) / (uint32_t)a.r);
-  const int seg_len = max(0, min(s.len, s.len - s.n + last_tok + 1));
+  const int seg_len = tile_len(a, s, tile);
   const int all_see = s.len - s.n + first_tok + 1;
   // this split's tiles of tokens
   const int nt_all = (seg_len + N - 1) / N;
+  const int splits = item_splits(a, s_where[3], nt_all);
+  if (split >= splits) return;
   const int t_first = (int)((int64_t)nt_all * split / splits);
   const int nt = (int)((int64_t)nt_all * (split + 1) / splits) - t_first;
 
@@ -740,7 +704,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (nt > 0) flush(nt - 1);
     // ---- sums over the quad's lanes, and out
     const bool whole = splits == 1;
-    float* part = reinterpret_cast<float*>(parts + (size_t)blockIdx.x * kTcRows * (D + 2) * 4);
+    float* part = reinterpret_cast<float*>(parts + blockIdx.x * tc_part_floats(D) * 4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = row0 + 8 * i;
@@ -782,75 +746,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the splits of each tile of rows, in their order; a warp a row.
-template <int D>
-__global__ void __launch_bounds__(512) tc_join_kernel(const Args a, int splits, const unsigned char* parts) {
-  constexpr int V = D / 32;
-  __shared__ int s_where[3];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int item = blockIdx.x, kvh = item % a.hkv;
-  if (warp == 0) {
-    int b = 0, tile = 0;
-    const bool ok = find_tile(a, item / a.hkv, b, tile);
-    if (lane == 0) {
-      s_where[0] = ok;
-      s_where[1] = b;
-      s_where[2] = tile;
-    }
-  }
-  __syncthreads();
-  if (!s_where[0]) return;
-  const Seq s = seq_of(a, s_where[1]);
-  const int row0 = s_where[2] * kTcRows, rows = min(kTcRows, s.n * a.r - row0);
-  for (int row = blockIdx.y * 16 + warp; row < rows; row += gridDim.y * 16) {
-    Merged<V> all;
-    for (int j = 0; j < splits; ++j) {
-      const float* p = reinterpret_cast<const float*>(parts + (size_t)(item * splits + j) * kTcRows * (D + 2) * 4);
-      float po[V];
-      load_v<V>(p + row * D + lane * V, po);
-      all.take(p[kTcRows * D + row], p[kTcRows * (D + 1) + row], po);
-    }
-    const int rr = row0 + row, tok = (int)((uint32_t)rr / (uint32_t)a.r), hq = kvh * a.r + rr - tok * a.r;
-    store_v<V>(a.out + ((s.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
-  }
-}
-
 int sms() {
   Context* c = ctx();
   return c ? c->num_sms : 148;
 }
 
 template <int D, int NG>
-int run(const Args& a, int64_t max_blocks, unsigned char* ws, cudaStream_t st) {
+int run(const Args& a, unsigned char* ws, cudaStream_t st) {
   using L = TcLayout<D, NG>;
-  const int64_t rows = a.rows * a.r;
-  const int64_t tiles = rows / kTcRows + std::min<int64_t>(a.n_seqs, rows / (a.big + 1));
-  const int64_t items = tiles * a.hkv;
-  if (items == 0) return NIMF_OK;
-  // With fewer tiles of rows than SMs the tokens are split too, down to four
-  // tiles of them a CTA.
-  const int64_t deep = std::max<int64_t>(1, max_blocks * a.bs / (4 * L::N));
-  const int splits = items >= sms() ? 1 : (int)std::min<int64_t>(deep, 2 * sms() / items);
+  // Items that fill half the SMs or less are cut into parts, a.sms of them at most.
+  const int64_t items = tc_items(a), ctas = std::max<int64_t>(items, a.sms);
   NIMF_TRY(allow_smem((const void*)tc_kernel<D, NG>, L::SIZE));
-  NIMF_TRY(launch(tc_kernel<D, NG>, dim3((unsigned)(items * splits)), kTcThreads, L::SIZE, st, 1, a, splits, ws));
-  if (splits == 1) return NIMF_OK;
-  return launch(tc_join_kernel<D>, dim3((unsigned)items, 4), 512, 0, st, 1, a, splits, (const unsigned char*)ws);
+  return launch(tc_kernel<D, NG>, dim3((unsigned)ctas), kTcThreads, L::SIZE, st, 1, a, ws);
 }
 
 }  // namespace
 
 bool tc_serves(int d) { return d <= 128; }
-size_t tc_ws_bytes(int d) { return 2 * (size_t)sms() * part_bytes(d); }
+size_t tc_ws_bytes(int d) { return sms() * tc_part_floats(d) * 4; }
+int64_t tc_items(const Args& a) {
+  const int64_t rows = a.rows * a.r;
+  return (rows / kTcRows + std::min<int64_t>(a.n_seqs, rows / (a.big + 1))) * a.hkv;
+}
 
-int run_tc(const Args& a, int d, int ng, int64_t max_blocks, unsigned char* ws, cudaStream_t st) {
+int run_tc(const Args& a, int d, int ng, unsigned char* ws, cudaStream_t st) {
   switch (d * 16 + ng) {
-    case 64 * 16 + 1: return run<64, 1>(a, max_blocks, ws, st);
-    case 64 * 16 + 2: return run<64, 2>(a, max_blocks, ws, st);
-    case 128 * 16 + 1: return run<128, 1>(a, max_blocks, ws, st);
-    case 128 * 16 + 2: return run<128, 2>(a, max_blocks, ws, st);
-    default: return run<128, 4>(a, max_blocks, ws, st);
+    case 64 * 16 + 1: return run<64, 1>(a, ws, st);
+    case 64 * 16 + 2: return run<64, 2>(a, ws, st);
+    case 128 * 16 + 1: return run<128, 1>(a, ws, st);
+    case 128 * 16 + 2: return run<128, 2>(a, ws, st);
+    default: return run<128, 4>(a, ws, st);
   }
 }
 
