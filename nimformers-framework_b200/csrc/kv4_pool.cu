@@ -42,7 +42,7 @@ int allow_smem(const void* kern, int bytes) {
     int device, bytes;
   };
   constexpr int kKernels = 64;
-  static Done done[kKernels];                // zero: a free place
+  static thread_local Done done[kKernels];   // zero: a free place
   const int device = ctx()->device;
   Done* d = done;
   while (d < done + kKernels - 1 && d->kern && d->kern != kern) ++d;

@@ -455,6 +455,169 @@ def test_attention_in_graphs_on_two_streams(nimf_gpu, torch_dev):
             check(d["out"].cpu().numpy(), pool, tab, lens, new, q, 0.1)
 
 
+@pytest.mark.parametrize("dim,group,rows,hkv,r", [(64, 32, 1301, 3, 3), (128, 128, 997, 5, 2), (256, 64, 1603, 2, 2)])
+def test_append_long_batches(nimf_gpu, torch_dev, dim, group, rows, hkv, r):
+    """More rows than a warp each has heads for, head counts that no four heads
+    a warp divide: every row's values, and some rows' bytes."""
+    torch = torch_dev
+    rng = np.random.default_rng(rows)
+    bs, h = 16, hkv * r
+    blocks = -(-rows // bs) + 3
+    q, k, v = (rng.standard_normal((rows, x, dim)).astype(F) for x in (h, hkv, hkv))
+    slots = rng.permutation(blocks * bs)[:rows].astype(np.int32)
+    slots[::50] = -1
+    pos = rng.integers(0, 500, rows).astype(np.int32)
+    ct, st = tables(dim, 500)
+    qr, kr = R.rope(q, pos, ct, st), R.rope(k, pos, ct, st)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=hkv, head_dim=dim, block_size=bs, group=group)
+    cache = torch.zeros(kv4.nbytes, dtype=torch.uint8, device="cuda")
+    dq, dk, dv, ds, dp, dc, dn = (up(torch, a) for a in (q, k, v, slots, pos, ct, st))
+    kv4.append(cache.data_ptr(), dk.data_ptr(), dv.data_ptr(), rows, ds.data_ptr(), q=dq.data_ptr(), q_out=dq.data_ptr(), n_heads=h,
+               positions=dp.data_ptr(), cos=dc.data_ptr(), sin=dn.data_ptr(), max_seq=500, stream=1)
+    ko, vo = (torch.full((rows, hkv, dim), 7.0, device="cuda") for _ in range(2))
+    kv4.read(cache.data_ptr(), ds.data_ptr(), rows, ko.data_ptr(), vo.data_ptr(), stream=1)
+    sync(torch, nimf_gpu)
+    assert np.array_equal(dq.cpu().numpy(), qr)
+    for out, x in ((ko, kr), (vo, v)):
+        want = R.decode(*R.encode(x, group))
+        want[slots < 0] = 0
+        assert np.array_equal(out.cpu().numpy(), want)
+    pool = R.Pool(blocks, hkv, dim, bs, group)
+    pool.buf[:] = cache.cpu().numpy().reshape(pool.buf.shape)
+    before = pool.buf.copy()
+    for t in [t for t in range(0, rows, 41) if slots[t] >= 0]:
+        pool.write(slots[t], True, kr[t])
+        pool.write(slots[t], False, v[t])
+    assert np.array_equal(before, pool.buf)
+
+
+@pytest.mark.parametrize("lens,new", [
+    ([5000], [70]),                              # few rows of a long context: its tokens in parts
+    ([3000, 700, 1, 40, 2049], [150, 1, 1, 1, 3]),
+    ([60, 9000, 33], [60, 1, 1]),                # a short prompt beside a long context
+    ([1500, 1200], [700, 600]),
+    ([130, 0, 500], [200, 0, 90]),               # rows before the first token
+])
+@pytest.mark.parametrize("dim,group,hkv,r,bs", [(64, 32, 2, 2, 48), (64, 64, 1, 3, 16), (128, 32, 1, 4, 16), (128, 64, 2, 2, 16), (128, 128, 1, 2, 80)])
+def test_attention_prompts_in_parts(nimf_gpu, torch_dev, dim, group, hkv, r, bs, lens, new):
+    """Prompts whose tokens are shared by CTAs, in tables of any width, beside
+    single tokens; NaN behind the ends; the same bits every time."""
+    rng = np.random.default_rng(dim + group + sum(lens))
+    blocks, tab = layout(rng, lens, bs)
+    pool = R.Pool(blocks, hkv, dim, bs, group, rng)
+    fill(pool, rng)
+    for b, n in enumerate(lens):
+        poison(pool, tab[b], n)
+    q = rng.standard_normal((sum(new), hkv * r, dim)).astype(F)
+    scale = 1 / np.sqrt(dim)
+    first = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale)
+    check(first, pool, tab, lens, new, q, scale)
+    for _ in range(2):
+        assert np.array_equal(first, attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale))
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("width", [47, 48, 49, 60])
+def test_attention_short_tables(nimf_gpu, torch_dev, dim, group, width):
+    """Tables around the longest context that is not shared by CTAs, for single
+    tokens, short chunks and prompts beside them."""
+    rng = np.random.default_rng(dim + group + width)
+    full = 16 * width
+    lens = [full, full - 1, 1, 0, 100, full - 16, 31, 32] + [int(n) for n in rng.integers(1, full, 20)]
+    blocks, tab = layout(rng, lens, 16)
+    tab = tab[:, :width]
+    pool = R.Pool(blocks, 2, dim, 16, group, rng)
+    fill(pool, rng)
+    for new in ([1] * 28, [3] + [1] * 26 + [4], [40] + [1] * 26 + [25]):
+        q = rng.standard_normal((sum(new), 4, dim)).astype(F)
+        got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.1)
+        check(got, pool, tab, lens, new, q, 0.1)
+
+
+def test_attention_rows_of_a_huge_table(nimf_gpu, torch_dev):
+    """A table so wide that units are counted in 64 bits and entries lie behind
+    2^26 others."""
+    torch = torch_dev
+    rng = np.random.default_rng(31)
+    width, lens, new = 2 ** 27 - 1, [100, 700], [1, 1]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, 8, 64, 16, 32, rng)
+    fill(pool, rng)
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=8, head_dim=64, block_size=16, group=32)
+    big = torch.empty(2, width, dtype=torch.int32, device="cuda")
+    big[:, :tab.shape[1]] = up(torch, tab)
+    for new, hint in (([1, 1], 1), ([30, 2], 30)):
+        q = rng.standard_normal((sum(new), 8, 64)).astype(F)
+        d = [up(torch, a) for a in (pool.buf, q, np.array(lens, np.int32), np.array([0, new[0], sum(new)], np.int32))]
+        out = torch.empty(sum(new), 8, 64, device="cuda")
+        work = torch.empty(kv4.attention_workspace(8), dtype=torch.uint8, device="cuda")
+        kv4.attention(d[0].data_ptr(), d[1].data_ptr(), sum(new), 8, 2, d[3].data_ptr(), d[2].data_ptr(), big.data_ptr(), width, 0.125,
+                      out.data_ptr(), work.data_ptr(), work.numel(), max_new=hint, stream=1)
+        sync(torch, nimf_gpu)
+        check(out.cpu().numpy(), pool, tab, lens, new, q, 0.125)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [60, 1, 25, 1]])
+def test_steps_in_a_graph_and_on_the_library_stream(nimf_gpu, torch_dev, new):
+    """Reserve, append and attention of several layers captured once and replayed
+    step after step, and the same calls on the library's stream: the same bits as
+    call by call."""
+    torch = torch_dev
+    rng = np.random.default_rng(17)
+    bs, hkv, r, dim, group, width, blocks, layers, steps = 16, 2, 3, 128, 64, 20, 90, 3, 3
+    n, h, rows, max_seq = len(new), hkv * r, sum(new), 400
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=hkv, head_dim=dim, block_size=bs, group=group)
+    ct, st = (up(torch, t) for t in tables(dim, max_seq))
+    xs = [[rng.standard_normal((rows, x, dim)).astype(F) for x in (h, hkv, hkv)] for _ in range(steps)]
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    class State:
+        def __init__(self):
+            self.cache = [torch.zeros(kv4.nbytes, dtype=torch.uint8, device="cuda") for _ in range(layers)]
+            self.free, self.nf = torch.arange(blocks, dtype=torch.int32, device="cuda"), i32(1) + blocks
+            self.lens, self.tab, self.cu, self.granted = i32(n), i32(n, width) - 1, i32(n + 1), i32(n)
+            self.slots, self.pos, self.new = i32(rows), i32(rows), up(torch, np.array(new, np.int32))
+            self.x = [torch.zeros(rows, y, dim, device="cuda") for y in (h, hkv, hkv)]
+            self.q, self.out = (torch.zeros(layers, rows, h, dim, device="cuda") for _ in range(2))
+            self.work = torch.empty(kv4.attention_workspace(h), dtype=torch.uint8, device="cuda")
+
+        def step(self, stream):
+            p = lambda t: t.data_ptr()  # noqa: E731
+            kv4.reserve(n, width, p(self.new), p(self.lens), p(self.lens), p(self.tab), p(self.free), p(self.nf), p(self.nf), rows,
+                        p(self.cu), p(self.slots), p(self.pos), p(self.granted), stream=stream)
+            for i in range(layers):
+                kv4.append(p(self.cache[i]), p(self.x[1]), p(self.x[2]), rows, p(self.slots), q=p(self.x[0]) if i == 0 else p(self.out[i - 1]),
+                           q_out=p(self.q[i]), n_heads=h, positions=p(self.pos), cos=p(ct), sin=p(st), max_seq=max_seq, stream=stream)
+                kv4.attention(p(self.cache[i]), p(self.q[i]), rows, h, n, p(self.cu), p(self.lens), p(self.tab), width, 0.09, p(self.out[i]),
+                              p(self.work), self.work.numel(), max_new=max(new), stream=stream)
+
+    def run(how):
+        s, outs = State(), []
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        if how == "graph":
+            with torch.cuda.graph(graph, stream=side):
+                s.step(side.cuda_stream)
+        for x in xs:
+            for t, y in zip(s.x, x):
+                t.copy_(up(torch, y))
+            torch.cuda.synchronize()
+            if how == "graph":
+                graph.replay()
+            else:
+                s.step(1 if how == "calls" else None)
+            sync(torch, nimf_gpu)
+            outs += [s.out.cpu().numpy(), s.lens.cpu().numpy(), s.tab.cpu().numpy()]
+        assert int(s.granted.sum()) == n
+        return outs + [c.cpu().numpy() for c in s.cache]
+
+    first = run("calls")
+    assert np.isfinite(first[0]).all() and first[0].any()
+    for how in ("graph", "library"):
+        for a, b in zip(first, run(how)):
+            assert np.array_equal(a, b), how
+
+
 # ------------------------------------------------------------------ together
 def test_serving_steps(nimf_gpu, torch_dev):
     """Prompts admitted, tokens decoded, a request finished and its blocks used
