@@ -347,8 +347,8 @@ int nimf_greedy_sample_dev(const float* logits, int64_t rows, int64_t vocab, con
  * logprob, entropy and rank are nullable (logprob and rank need ids, ids may
  * be NULL without them); n_top 0 .. 32, at most vocab (0: no alternatives).
  * A row with a NaN or +inf gives NaN log-probabilities and entropy; a row of
- * -inf only gives log-probabilities -inf and entropy 0.  The logits are read
- * once and not modified; vocab <= 262144.  No workspace, nothing allocated. */
+ * -inf only gives log-probabilities -inf and entropy 0.  The logits are not
+ * modified; vocab <= 262144.  No workspace, nothing allocated. */
 int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t vocab, const int32_t* ids,
                       int64_t n_top, float* logprob, float* entropy, int32_t* rank,
                       int32_t* top_ids, float* top_logprobs, void* stream);
@@ -372,11 +372,11 @@ int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t vocab, const in
  * a token is coded with its own scale and minimum (float32):
  *   scale = (max - min) / 15, code = min(15, round((x - min) / scale)),
  * every step rounded to float32, halves to even; a code stands for
- * code * scale + min (a minimum of -0 is kept as 0).  A group holding a NaN, an infinity or a range above the
- * largest float stands for NaN.  head_dim 64, 128 or 256; group 32, 64 or 128,
- * at most head_dim; block_size a multiple of 16 up to 4096;
- * n_blocks * block_size below 2^31.  Slot s is token s % block_size of block
- * s / block_size. */
+ * code * scale + min (a minimum of -0 is kept as 0).  A group holding a NaN,
+ * an infinity or a range above the largest float stands for NaN.  head_dim 64,
+ * 128 or 256; group 32, 64 or 128, at most head_dim; block_size a multiple of
+ * 16 up to 4096; n_blocks * block_size below 2^31; up to 2^30 requests a call.
+ * Slot s is token s % block_size of block s / block_size. */
 typedef struct nimf_kv4_desc {
   int64_t n_blocks, n_kv_heads, head_dim, block_size, group;
 } nimf_kv4_desc;
@@ -446,9 +446,9 @@ int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int
  * NULL: row b alone), which are its last lens[b] tokens: row i of n sees the
  * tokens 0 .. lens[b] - n + i, the cache holding them all (append first).  A
  * row that sees nothing gives zeros; rows of no sequence are left as they
- * were.  max_new is the largest number of rows of a sequence as the host knows
- * it (a hint that chooses kernels, 1 for a decode step; results do not depend
- * on its being right).  A block id outside the cache leaves its tokens out and
+ * were.  cu_rows never falls.  max_new is the largest number of rows of a
+ * sequence as the host knows it, 1 for a decode step: a hint that chooses
+ * kernels; whatever it is, every row is computed.  A block id outside the cache leaves its tokens out and
  * makes nimf_sync report device error 4.  Scores, softmax and sums are float32;
  * q and the probabilities enter the tensor cores as two fp16 terms each, the
  * codes exactly.  Results do not depend on timing.  Buffers 16-byte aligned. */

@@ -26,6 +26,7 @@ namespace nimf {
 namespace kv4 {
 
 constexpr int kTile = 16;  // tokens of a tile
+constexpr int kMaxSeqs = 1 << 30;  // requests of a call: searches add two indexes in 32 bits
 
 // Sizes of a cache as the kernels take them.
 struct Shape {

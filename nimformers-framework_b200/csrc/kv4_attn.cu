@@ -937,7 +937,7 @@ int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const f
   kv4::Shape s;
   NIMF_TRY(kv4::check_desc(desc, "kv4_attention", &s));
   if (rows < 0 || rows > INT32_MAX || n_heads < 1 || n_heads % s.hkv || n_heads > 65535 ||
-      n_seqs < 0 || n_seqs > INT32_MAX || max_blocks < 1 || max_blocks > INT32_MAX / s.bs || max_new < 0)
+      n_seqs < 0 || n_seqs > kv4::kMaxSeqs || max_blocks < 1 || max_blocks > INT32_MAX / s.bs || max_new < 0)
     return set_error(NIMF_ERR_SHAPE,
                      "kv4_attention: rows %lld n_heads %lld (a multiple of n_kv_heads %d) n_seqs "
                      "%lld max_blocks %lld max_new %lld",

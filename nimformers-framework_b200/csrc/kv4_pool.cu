@@ -120,8 +120,9 @@ __device__ __forceinline__ void write_rows(int64_t t0, int n_seqs, int64_t width
     const int32_t blk = entry[k] ? *entry[k] : -1;
     const int32_t in = pos[k] - (int32_t)(blocks.of((uint32_t)pos[k]) * blocks.bs);
     if (t < max_rows) {
-      slots[t] = blk >= 0 && blk < n_blocks ? blk * (int32_t)blocks.bs + in : -1;
-      positions[t] = pos[k];
+      const bool there = blk >= 0 && blk < n_blocks;
+      slots[t] = there ? blk * (int32_t)blocks.bs + in : -1;
+      positions[t] = there ? pos[k] : 0;
     }
   }
 }
@@ -595,7 +596,7 @@ int nimf_kv4_reserve_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_
   cudaStream_t st;
   kv4::Shape s;
   NIMF_TRY(kv4::check_desc(desc, "kv4_reserve", &s));
-  if (n_seqs < 0 || n_seqs > INT32_MAX || max_blocks < 1 || max_blocks > INT32_MAX / s.bs ||
+  if (n_seqs < 0 || n_seqs > kv4::kMaxSeqs || max_blocks < 1 || max_blocks > INT32_MAX / s.bs ||
       max_rows < 0 || max_rows > INT32_MAX)
     return set_error(NIMF_ERR_SHAPE, "kv4_reserve: n_seqs %lld max_blocks %lld max_rows %lld",
                      (long long)n_seqs, (long long)max_blocks, (long long)max_rows);
@@ -626,7 +627,7 @@ int nimf_kv4_release_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_
   cudaStream_t st;
   kv4::Shape s;
   NIMF_TRY(kv4::check_desc(desc, "kv4_release", &s));
-  if (n_seqs < 0 || n_seqs > INT32_MAX || max_blocks < 1 || max_blocks > INT32_MAX / s.bs)
+  if (n_seqs < 0 || n_seqs > kv4::kMaxSeqs || max_blocks < 1 || max_blocks > INT32_MAX / s.bs)
     return set_error(NIMF_ERR_SHAPE, "kv4_release: n_seqs %lld max_blocks %lld", (long long)n_seqs,
                      (long long)max_blocks);
   if (n_seqs == 0) return NIMF_OK;

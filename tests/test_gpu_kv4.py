@@ -92,6 +92,19 @@ def test_reserve_odd_inputs(nimf_gpu, torch_dev):
         assert np.array_equal(got[k].cpu().numpy(), np.reshape(want[k], got[k].shape)), k
 
 
+def test_reserve_over_a_missing_block(nimf_gpu, torch_dev):
+    """A request whose last block is not in its table: no slot and position 0
+    for the rows that would lie there, the others as ever."""
+    kv4 = nimf_gpu.KV4Cache(n_blocks=4, n_kv_heads=1, head_dim=64, block_size=16, group=32)
+    new, lens = np.array([10, 1], np.int32), np.array([20, 3], np.int32)
+    table = np.array([[3, -1, -1], [2, -1, -1]], np.int32)
+    got = run_reserve(torch_dev, nimf_gpu, kv4, 2, 3, new, lens, table, np.array([0, 1, 0, 0], np.int32), 2, 12, False)
+    assert got["slots"].tolist() == [-1] * 10 + [35, -1] and got["positions"].tolist() == [0] * 10 + [3, 0]
+    new[0] = 15
+    got = run_reserve(torch_dev, nimf_gpu, kv4, 2, 3, new, lens, table, np.array([0, 1, 0, 0], np.int32), 2, 16, False)
+    assert got["slots"].tolist() == [-1] * 12 + [16, 17, 18, 35] and got["positions"].tolist() == [0] * 12 + [32, 33, 34, 3]
+
+
 def test_release_returns_blocks_in_order(nimf_gpu, torch_dev):
     torch = torch_dev
     rng = np.random.default_rng(8)
@@ -514,6 +527,22 @@ def test_attention_prompts_in_parts(nimf_gpu, torch_dev, dim, group, hkv, r, bs,
     check(first, pool, tab, lens, new, q, scale)
     for _ in range(2):
         assert np.array_equal(first, attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, scale))
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 32), (128, 128), (256, 128)])
+@pytest.mark.parametrize("hkv,r", [(1, 20), (2, 33), (1, 130)])
+def test_attention_many_heads_of_a_kv_head(nimf_gpu, torch_dev, dim, group, hkv, r):
+    """Single tokens with more heads a KV head than a row tile of either kind."""
+    rng = np.random.default_rng(dim + r)
+    lens, new = [300, 1, 0, 2500, 63], [1, 1, 1, 1, 2]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, hkv, dim, 16, group, rng)
+    fill(pool, rng)
+    for b, n in enumerate(lens):
+        poison(pool, tab[b], n)
+    q = rng.standard_normal((sum(new), hkv * r, dim)).astype(F)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.1)
+    check(got, pool, tab, lens, new, q, 0.1)
 
 
 @pytest.mark.parametrize("dim,group", [(64, 32), (128, 32), (128, 128), (256, 64)])

@@ -109,3 +109,11 @@ def test_reference_decodes_what_it_encodes():
         pool.write((2 if t < 16 else 0) * 16 + t, True, x[t:t + 1])
     c2, s2, l2 = pool.tokens([2, 0], 5, True)
     assert np.array_equal(R.decode(c2, s2, l2)[:, 0], y)
+
+
+def test_requests_of_a_call_are_limited():
+    """More than 2^30 requests, which the searches' 32-bit indexes do not reach."""
+    c, n = kv4(), (1 << 30) + 1
+    refused("SHAPE", c.reserve, n, 4, X, X, X, X, X, X, X, 10, X, X, X, X)
+    refused("SHAPE", c.release, n, 4, X, X, X, X, X)
+    refused("SHAPE", c.attention, X, X, 2, 4, n, X, X, X, 4, 1.0, X, X, 1 << 30)
