@@ -228,16 +228,27 @@ __device__ __forceinline__ void store_v(float* p, const float (&x)[V], float f) 
 }
 
 // Attention of sequences with more than a.big rows a KV head, on tcgen05
-// (kv4_tc.cu): 128 rows of one KV head an item, items of few tokens parts where
-// the items would leave SMs idle.  A part is the rows' outputs, maxima and sums.
+// (kv4_tc.cu): an item is 128 rows of one KV head.  Items run in waves of a CTA
+// an SM; those of a last wave that half fills the SMs or less are cut into parts
+// of their tokens, as many as run at once.  A part is the rows' outputs, maxima
+// and sums.
 constexpr int kTcRows = 128;
 __device__ __forceinline__ int big_tiles(const Args& a, int n) {
   return n * a.r > a.big ? (n * a.r + kTcRows - 1) / kTcRows : 0;
 }
-// Parts of an item: as many as run at once, each of four tiles of tokens or more.
-__device__ __forceinline__ int item_splits(const Args& a, int items, int token_tiles) {
-  return max(1, min(a.sms / max(items, 1), token_tiles / 4));
-}
+struct Waves {
+  int items, whole, cut;        // items; those of full waves; parts of each of the others
+  __device__ __forceinline__ Waves(const Args& a, int n) {
+    items = n;
+    whole = n / a.sms * a.sms;
+    cut = a.sms / max(n - whole, 1);
+    if (cut < 1 || n == whole) cut = 1;
+  }
+  // Parts of an item, each of four tiles of tokens or more.
+  __device__ __forceinline__ int parts(int item, int token_tiles) const {
+    return item < whole ? 1 : max(1, min(cut, token_tiles / 4));
+  }
+};
 __host__ __device__ constexpr size_t tc_part_floats(int d) { return (size_t)kTcRows * (d + 2); }
 // The sequence and its tile of rows of index i, counted from the end (the last
 // rows see most tokens: the longest go first), and the number of all tiles.

@@ -141,8 +141,9 @@ __device__ __forceinline__ int idle_sms(const Args& a, float units) {
     items += __reduce_add_sync(0xffffffffu, t);
     longest = max(longest, __reduce_max_sync(0xffffffffu, t ? s.len : 0));
   }
-  items *= a.hkv;
-  const int idle = a.sms - items * max(1, a.sms / max(items, 1));
+  const Waves waves(a, items * a.hkv);
+  const int idle = waves.items == waves.whole ? 0 : a.sms - (waves.items - waves.whole) * waves.cut;
+  longest /= waves.cut;
   return idle > 0 && units * (float)(a.sms - idle) * kUnit <= (float)longest * (float)idle ? idle : 0;
 }
 
@@ -798,17 +799,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a, int
   const int64_t cta = BESIDE && a.uncut ? blockIdx.x + ctas : blockIdx.x;
   if (BESIDE && cta >= ctas) {
     int b = 0, tile = 0, total = 0;
-    const int item = (int)(cta - ctas) / 4, kvh = item % a.hkv;
-    if (!find_tile(a, item / a.hkv, b, tile, total)) return;
-    const int items = total * a.hkv, cut = max(1, a.sms / items);
+    find_tile(a, INT32_MAX, b, tile, total);
+    const Waves waves(a, total * a.hkv);
+    const int last = (int)(cta - ctas) / 4, item = waves.whole + last, kvh = item % a.hkv;  // of the last wave
+    if (waves.cut == 1 || !find_tile(a, item / a.hkv, b, tile, total)) return;
     const Seq s = seq_of(a, b);
-    const int splits = item_splits(a, items, (tile_len(a, s, tile) + tc_tokens - 1) / tc_tokens);
+    const int splits = waves.parts(item, (tile_len(a, s, tile) + tc_tokens - 1) / tc_tokens);
     if (splits == 1) return;
     const int row0 = tile * kTcRows, rows = min(kTcRows, s.n * a.r - row0);
     for (int row = (int)(cta - ctas) % 4 * kJoinWarps + warp; row < rows; row += 4 * kJoinWarps) {
       Merged<V> all;
       for (int j = 0; j < splits; ++j) {
-        const float* p = tc_parts + (size_t)(item * cut + j) * tc_part_floats(D);
+        const float* p = tc_parts + (size_t)(last * waves.cut + j) * tc_part_floats(D);
         float po[V];
         load_v<V>(p + row * D + lane * V, po);
         all.take(p[kTcRows * D + row], p[kTcRows * (D + 1) + row], po);
@@ -874,7 +876,7 @@ int run_nb(const Args& a, cudaStream_t st) {
   NIMF_TRY(allow_smem((const void*)attn_kernel<D, NG, NB, BESIDE>, smem));
   const int ctas = grid_of(D, NG, NB);
   NIMF_TRY(launch(attn_kernel<D, NG, NB, BESIDE>, dim3(ctas), warps_of(D, NG, NB) * 32, smem, st, 1, a));
-  // tc_kernel's items have parts where they fill half the SMs or less
+  // items with parts are half a wave or less
   const int64_t tc_blocks = BESIDE ? 4 * std::min<int64_t>(tc_items(a), a.sms / 2) : 0;
   const int64_t blocks = (a.uncut ? 0 : ctas) + tc_blocks;
   if (blocks == 0) return NIMF_OK;

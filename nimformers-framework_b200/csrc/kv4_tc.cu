@@ -187,19 +187,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // the items' number gives their parts, so the item of a CTA is known after it
     int b = 0, tile = 0, total = 0;
     find_tile(a, INT32_MAX, b, tile, total);
-    const int items = total * a.hkv, cut = max(1, a.sms / max(items, 1));
-    const int item = blockIdx.x / cut;
+    const Waves wv(a, total * a.hkv);
+    const int over = (int)blockIdx.x - wv.whole, item = over < 0 ? blockIdx.x : wv.whole + over / wv.cut;
     const bool ok = find_tile(a, item / a.hkv, b, tile, total);
     if (lane == 0) {
-      s_where[0] = ok ? cut : 0;
+      s_where[0] = ok;
       s_where[1] = b;
       s_where[2] = tile;
-      s_where[3] = items;
+      s_where[3] = wv.items;
     }
   }
   __syncthreads();
   if (!s_where[0]) return;                      // more CTAs than tiles: the host knows a bound
-  const int split = blockIdx.x % s_where[0], item = blockIdx.x / s_where[0];
+  const Waves waves(a, s_where[3]);
+  const int over = (int)blockIdx.x - waves.whole;
+  const int item = over < 0 ? blockIdx.x : waves.whole + over / waves.cut, split = over < 0 ? 0 : over % waves.cut;
   const int kvh = item % a.hkv;
   const int b = s_where[1], tile = s_where[2];
   const Seq s = seq_of(a, b);
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int all_see = s.len - s.n + first_tok + 1;
   // this split's tiles of tokens
   const int nt_all = (seg_len + N - 1) / N;
-  const int splits = item_splits(a, s_where[3], nt_all);
+  const int splits = waves.parts(item, nt_all);
   if (split >= splits) return;
   const int t_first = (int)((int64_t)nt_all * split / splits);
   const int nt = (int)((int64_t)nt_all * (split + 1) / splits) - t_first;
@@ -704,7 +706,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (nt > 0) flush(nt - 1);
     // ---- sums over the quad's lanes, and out
     const bool whole = splits == 1;
-    float* part = reinterpret_cast<float*>(parts + blockIdx.x * tc_part_floats(D) * 4);
+    float* part = reinterpret_cast<float*>(parts + (size_t)max(over, 0) * tc_part_floats(D) * 4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = row0 + 8 * i;
@@ -754,8 +756,8 @@ int sms() {
 template <int D, int NG>
 int run(const Args& a, unsigned char* ws, cudaStream_t st) {
   using L = TcLayout<D, NG>;
-  // Items that fill half the SMs or less are cut into parts, a.sms of them at most.
-  const int64_t items = tc_items(a), ctas = std::max<int64_t>(items, a.sms);
+  // a last wave of items or parts, whatever number of items it turns out to be
+  const int64_t ctas = (tc_items(a) / a.sms + 1) * a.sms;
   NIMF_TRY(allow_smem((const void*)tc_kernel<D, NG>, L::SIZE));
   return launch(tc_kernel<D, NG>, dim3((unsigned)ctas), kTcThreads, L::SIZE, st, 1, a, ws);
 }
