@@ -156,9 +156,11 @@ struct Seq {
 __device__ __forceinline__ Seq seq_of(const Args& a, int64_t b) {
   Seq s;
   int64_t e;
-  if (a.cu_rows) {
-    s.row0 = min((int64_t)max(a.cu_rows[b], 0), a.rows);
-    e = min((int64_t)max(a.cu_rows[b + 1], 0), a.rows);
+  const int32_t* cu = a.cu_rows;
+  asm volatile("" : "+l"(cu));  // opaque: loops are not to be copied for either case
+  if (cu) {
+    s.row0 = min((int64_t)max(cu[b], 0), a.rows);
+    e = min((int64_t)max(cu[b + 1], 0), a.rows);
   } else {
     s.row0 = min(b, a.rows);
     e = min(b + 1, a.rows);

@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
   // Every warp sums all sequences for itself: no barrier, one latency for 256 of
   // them.  T is 32 bits wide unless the host's bound of the line is wider: all
   // warps of an SM do this at once, and the 64-bit sums and divisions took twice
-  // the time (2.6 us of a 20 us call).
+  // the time (2.6 us of a 20 us call).  Loops stay rolled and there is one search:
+  // unrolled copies made this 100 KB of code, and fetching instructions took most
+  // of a short call's time.
   auto plan = [&](auto zero) -> bool {
     using T = decltype(zero);
     auto line_units = [&](int64_t b) -> T {
@@ -195,7 +197,9 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
       const Seq s = seq_of(a, b);
       return (T)seq_units(s.len) * (T)tiles_of(s.n) * (T)a.hkv;
     };
+    const bool one = a.n_seqs == 1;
     auto scan = [&](T v) -> T {             // inclusive, over the lanes
+      if (one) return __shfl_sync(0xffffffffu, v, 0);
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const T u = __shfl_up_sync(0xffffffffu, v, x);
@@ -204,32 +208,18 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
       return v;
     };
     auto div = [](T x, T y) -> T { return (T)((sizeof(T) == 4) ? (uint32_t)x / (uint32_t)y : quot(x, y)); };
-    // Up to 256 sequences stay in registers, a lane each of eight chunks; more are
-    // summed 256 at a time, eight to a lane, and again where they are looked for.
-    const bool few = a.n_seqs <= 256;
-    auto eight = [&](int64_t b0) -> T {
+    // A lane has up to eight neighbouring sequences at a time.
+    const int per = a.n_seqs > 224 ? 8 : ((int)a.n_seqs + 31) / 32;
+    auto some = [&](int64_t b0) -> T {
       T v = 0;
 #pragma unroll 1
-      for (int i = 0; i < 8; ++i) v += line_units(b0 + lane * 8 + i);
+      for (int i = 0; i < per; ++i) v += line_units(b0 + lane * per + i);
       return v;
     };
-    T units[8], upto[8], all = 0;
-    if (few) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        units[i] = 0;
-        if (32 * i < a.n_seqs) units[i] = line_units(32 * i + lane);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (32 * i < a.n_seqs) {
-          upto[i] = a.n_seqs == 1 ? units[i] : scan(units[i]) + all;
-          all = __shfl_sync(0xffffffffu, upto[i], a.n_seqs == 1 ? 0 : 31);
-        }
-    } else {
+    const T v_first = some(0), end_first = scan(v_first);
+    T all = __shfl_sync(0xffffffffu, end_first, 31);
 #pragma unroll 1
-      for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) all += __shfl_sync(0xffffffffu, scan(eight(b0)), 31);
-    }
+    for (int64_t b0 = 32 * per; b0 < a.n_seqs; b0 += 32 * per) all += __shfl_sync(0xffffffffu, scan(some(b0)), 31);
     T grid = (T)gridDim.x;
     if constexpr (BESIDE) {
       const int idle = idle_sms(a, (float)all / W / (float)gridDim.x);
@@ -237,62 +227,58 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     }
     const T n_ctas = max((T)1, min(grid, div(all + W - 1, W)));
     if (cta >= n_ctas || all == 0) return false;
-    // the sequence of a unit, and the unit within it
-    auto find = [&](T unit, int64_t& b, T& off) {
-      b = 0;
-      off = unit;
-      if (a.n_seqs == 1) return;
-      if (few) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (32 * i < a.n_seqs) {
-            const unsigned past = __ballot_sync(0xffffffffu, upto[i] > unit);
-            if (past) {
-              const int who = __ffs(past) - 1;
-              b = 32 * i + who;
-              off = unit - __shfl_sync(0xffffffffu, upto[i] - units[i], who);
-              return;
-            }
-          }
-        return;
-      }
-      T base = 0;
-#pragma unroll 1
-      for (int64_t b0 = 0; b0 < a.n_seqs; b0 += 256) {
-        const T v = eight(b0), end = scan(v) + base;
-        base = __shfl_sync(0xffffffffu, end, 31);
-        const unsigned past = __ballot_sync(0xffffffffu, end > unit);
-        if (!past) continue;
-        const int who = __ffs(past) - 1;
-        b = b0 + who * 8;
-        off = unit - __shfl_sync(0xffffffffu, end - v, who);
-        const T u = lane < 8 ? line_units(b + lane) : 0, sum = scan(u);
-        const int at = __ffs(__ballot_sync(0xffffffffu, sum > off)) - 1;  // which of that lane's eight
-        b += at;
-        off -= __shfl_sync(0xffffffffu, sum - u, at);
-        break;
-      }
-    };
     const T t_each = div(all, n_ctas), t_more = all - t_each * n_ctas, me = (T)cta;
-    T first = me * t_each + min(me, t_more), last = first + t_each + (me < t_more ? 1 : 0), o;
-    if (a.uncut) {                          // the segments that begin in this CTA's part
-      auto next_segment = [&](T unit) -> T {
-        if (unit >= all) return all;
-        find(unit, b, o);
-        const T nu = (T)seq_units(seq_of(a, b).len), rem = o - div(o, nu) * nu;
-        return rem ? unit + nu - rem : unit;
-      };
-      first = next_segment(first);
-      last = next_segment(last);
-      if (first >= last) return false;
+    T first = me * t_each + min(me, t_more), last = first + t_each + (me < t_more ? 1 : 0), unit = first, o = 0;
+    // Uncut, a CTA has the segments that begin in its part: steps 0 and 1 move its
+    // ends to where segments begin.  Step 2 looks for this warp's first unit.
+#pragma unroll 1
+    for (int step = a.uncut ? 0 : 2; step < 3; ++step) {
+      if (step == 2) {
+        if (first >= last) return false;
+        const T w_each = div(last - first, W), w_more = last - first - w_each * W, w = (T)warp;
+        unit = first + w * w_each + min(w, w_more);
+        w_a = unit;
+        w_b = unit + w_each + (w < w_more ? 1 : 0);
+      }
+      // the sequence of the unit, and the unit within it
+      b = 0;
+      o = unit;
+      if (!one && unit < all) {
+        T base = 0, v = v_first, end = end_first;
+        unsigned past;
+#pragma unroll 1
+        while (!(past = __ballot_sync(0xffffffffu, base + end > unit)) && b + 32 * per < a.n_seqs) {
+          base += __shfl_sync(0xffffffffu, end, 31);
+          b += 32 * per;
+          v = some(b);
+          end = scan(v);
+        }
+        const int who = past ? __ffs(past) - 1 : 0;
+        o = unit - base - __shfl_sync(0xffffffffu, end - v, who);
+        b += who * per;
+        if (per > 1) {
+          const T u = lane < per ? line_units(b + lane) : 0, sum = scan(u);
+          const unsigned here = __ballot_sync(0xffffffffu, sum > o);
+          const int at = here ? __ffs(here) - 1 : 0;
+          b += at;
+          o -= __shfl_sync(0xffffffffu, sum - u, at);
+        }
+      }
+      if (step < 2) {
+        if (unit < all) {
+          const T nu = (T)seq_units(seq_of(a, b).len), rem = o - div(o, nu) * nu;
+          if (rem) unit += nu - rem;
+        }
+        if (step == 0) {
+          first = unit;
+          unit = last;
+        } else {
+          last = unit;
+        }
+      }
     }
-    const T w_each = div(last - first, W), w_more = last - first - w_each * W, w = (T)warp;
-    const T mine = first + w * w_each + min(w, w_more);
-    find(mine, b, o);
     off = o;
     if (tid == 0) s_line = {t_each, t_more, first, last, o, b, n_ctas};
-    w_a = mine;
-    w_b = mine + w_each + (w < w_more ? 1 : 0);
     return true;
   };
   if (!(a.wide ? plan((int64_t)0) : plan((int32_t)0))) {
