@@ -408,6 +408,30 @@ def test_attention_nan_reaches_only_who_sees_it(nimf_gpu, torch_dev):
     assert np.isnan(got[20:50]).all() and np.isfinite(got[:20]).all() and np.isfinite(got[50]).all()
 
 
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128)])
+@pytest.mark.parametrize("hint", [1, 40])
+def test_attention_nan_in_one_part_of_many(nimf_gpu, torch_dev, dim, group, hint):
+    """A context that many CTAs share: a value's NaN in the last part reaches its
+    group of the rows that see it, a key's NaN in an early part every row."""
+    rng = np.random.default_rng(dim)
+    lens, new = [5000], [40]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, 1, dim, 16, group, rng)
+    fill(pool, rng)
+    x = rng.standard_normal((1, dim)).astype(F)
+    x[0, dim - 1] = np.nan
+    pool.write(tab[0][4985 // 16] * 16 + 4985 % 16, False, x)
+    q = rng.standard_normal((40, 2, dim)).astype(F)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.1, max_new=hint)
+    seen = np.arange(40) >= 25
+    assert np.isnan(got[seen][:, :, dim - group:]).all() and np.isfinite(got[seen][:, :, :dim - group]).all()
+    want, tol = R.attention(pool, tab[0], 4985, q[:25], 0.1)
+    assert (np.abs(got[:25] - want) <= tol).all()
+    pool.write(tab[0][100 // 16] * 16 + 100 % 16, True, x)
+    got = attend(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.1, max_new=hint)
+    assert np.isnan(got).all()
+
+
 def test_attention_leaves_out_blocks_that_are_not_there(nimf_gpu, torch_dev):
     """A table entry outside the cache: its tokens take no part, nimf_sync
     reports it, and lens past the table are cut to it."""
