@@ -15,7 +15,7 @@
 // candidates, for which the threads that reach the bound read their shares again
 // (out of L2).  Bounded by HBM; a slice kept in shared memory instead cost 64 KB
 // a CTA, loads and passes took turns, and 4,096 rows of 32,000 took 230 us; they
-// take 101 us now (5.2 TB/s), 64 rows of 128,001 with 20 alternatives 15 us, one
+// take 92 us now (5.7 TB/s), 64 rows of 128,001 with 20 alternatives 12.5 us, one
 // row of 32,000 6.2 us, both of these latency.
 #include <cfloat>
 
@@ -175,7 +175,12 @@ __device__ __forceinline__ int rank_of(const float* v, const int* i, int n, floa
   return r;
 }
 
-__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(const LpArgs a) {
+// PER_SM CTAs fit an SM.  Two, with all the registers that they want, where all of
+// the grid runs at once (64 rows of 128,001 in clusters of 4: 12.5 us, 15.3 with
+// three, 17.4 with four; 200 rows of 32,000: 9.6, with four 15.9); four where rows
+// queue (4,096 rows of 32,000: 92 us, 102 with three, 98 with five, which spill).
+template <int PER_SM>
+__global__ void __launch_bounds__(kLpThreads, PER_SM) logprobs_kernel(const LpArgs a) {
   __shared__ LpPart s_part[kLpWarps];
   __shared__ float s_f[kLpWarps];
   __shared__ int s_i[kLpWarps];
@@ -481,11 +486,10 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   if (!logits || ((logprob || rank) && !ids) || (n_top > 0 && (!top_ids || !top_logprobs)))
     return set_error(NIMF_ERR_ARG, "logprobs: NULL buffer");
   NIMF_TRY(kv4::stream_of(stream, &st));
-  // A CTA a row; several where the rows do not fill the SMs twice over, as long
-  // as a thread keeps four float4s, and for rows that a CTA would stream alone
-  // for long after the others.
+  // A CTA a row; several where the rows do not fill the SMs, up to two CTAs an SM,
+  // as long as a thread keeps four float4s.
   unsigned ctas = 1;
-  while (ctas < (unsigned)kLpMaxCluster && 2 * rows * ctas <= 3 * ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
+  while (ctas < (unsigned)kLpMaxCluster && rows * ctas <= ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
     ctas *= 2;
   LpArgs a = {};
   a.x = logits;
@@ -499,5 +503,5 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   a.vocab = vocab;
   a.slice = (int)(((vocab + ctas - 1) / ctas + 3) & ~(int64_t)3);
   a.top = (int)n_top;
-  return kv4::launch(logprobs_kernel, dim3((unsigned)(rows * ctas)), kLpThreads, 0, st, ctas, a);
+  return kv4::launch(rows * ctas <= 2 * ctx()->num_sms ? logprobs_kernel<2> : logprobs_kernel<4>, dim3((unsigned)(rows * ctas)), kLpThreads, 0, st, ctas, a);
 }
