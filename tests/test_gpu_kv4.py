@@ -731,3 +731,70 @@ def test_serving_steps(nimf_gpu, torch_dev):
         ref = R.logprobs(logits.cpu().numpy(), ids, 4)
         assert np.array_equal(rank.cpu().numpy(), ref["rank"]) and np.array_equal(top_i.cpu().numpy(), ref["top_ids"])
         assert np.allclose(lp.cpu().numpy(), ref["logprob"], rtol=2e-6, atol=2e-6)
+
+
+# ------------------------------------------------------------------ tables with missing blocks
+def check_rows_over_missing(got, pool, tab, lens, new, q, scale):
+    """Each row for itself: a table without the missing blocks holds what the
+    row sees, since only the last block it sees can be partly filled."""
+    row = 0
+    for b, (n, m) in enumerate(zip(lens, new)):
+        for i in range(m):
+            left, blocks, tokens = max(0, n - m + i + 1), [], 0
+            for blk in tab[b]:
+                here = min(pool.bs, left)
+                if here > 0 and 0 <= blk < pool.blocks:
+                    blocks.append(blk)
+                    tokens += here
+                left -= here
+            want, tol = R.attention(pool, blocks, tokens, q[row:row + 1], scale)
+            assert (np.abs(got[row] - want[0]) <= tol[0]).all(), (b, i)
+            row += 1
+    return row
+
+
+def attend_reported(torch, nimf, *args, **kw):
+    """attend(), which has to report device error 4 (once)."""
+    with pytest.raises(nimf.CatchableError, match="code 4"):
+        attend(torch, nimf, *args, **kw)
+    nimf.check(nimf.lib().nimf_sync())
+    return kw["out"].cpu().numpy()
+
+
+@pytest.mark.parametrize("dim,group", SHAPES)
+@pytest.mark.parametrize("hint", [1, 40])
+@pytest.mark.parametrize("bs,missing", [(16, [0]), (48, [2]), (16, [3, 4, 11]), (16, [17, 18]), (64, [4])])
+def test_prompts_leave_out_blocks_that_are_not_there(nimf_gpu, torch_dev, dim, group, hint, bs, missing):
+    """Chunks and whole prompts over tables whose first, middle or last blocks lie
+    outside the cache, beside single tokens: the same answer whatever max_new
+    says, zeros for a row that sees missing blocks only."""
+    rng = np.random.default_rng(dim + group + bs + missing[0])
+    lens, new = [300, 40, 70, 33], [30, 40, 1, 20]
+    blocks, tab = layout(rng, lens, bs)
+    pool = R.Pool(blocks, 2, dim, bs, group, rng)
+    fill(pool, rng)
+    tab[:, 0] = np.where(missing[0] == 0, [-1, blocks, -(2 ** 31), 2 ** 31 - 1], tab[:, 0])
+    tab[0, missing] = [-1, blocks, 2 ** 30][:len(missing)]
+    q = rng.standard_normal((sum(new) + 2, 4, dim)).astype(F)
+    got = attend_reported(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.2, max_new=hint, out=torch_dev.full(q.shape, 5.0, device="cuda"))
+    end = check_rows_over_missing(got, pool, tab, lens, new, q, 0.2)
+    assert (got[end:] == 5.0).all()
+    if missing[0] == 0:
+        assert not got[30:46].any()     # the second request's first rows see the missing block only
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 128)])
+@pytest.mark.parametrize("missing", [range(0, 100), range(100, 300, 3), range(290, 313), range(0, 313)])
+def test_shared_contexts_leave_out_blocks_that_are_not_there(nimf_gpu, torch_dev, dim, group, missing):
+    """A context whose tokens many CTAs share, with whole parts of it missing: a
+    chunk, and single tokens of many heads a KV head."""
+    rng = np.random.default_rng(dim + group + len(missing))
+    lens = [5000]
+    blocks, tab = layout(rng, lens, 16)
+    pool = R.Pool(blocks, 1, dim, 16, group, rng)
+    fill(pool, rng)
+    tab[0, list(missing)] = -1
+    for new, heads in (([5], 4), ([1], 20)):
+        q = rng.standard_normal((new[0], heads, dim)).astype(F)
+        got = attend_reported(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.2, max_new=new[0], out=torch_dev.full(q.shape, 5.0, device="cuda"))
+        check_rows_over_missing(got, pool, tab, lens, new, q, 0.2)
