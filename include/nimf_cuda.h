@@ -448,10 +448,13 @@ int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int
  * row that sees nothing gives zeros; rows of no sequence are left as they
  * were.  cu_rows never falls.  max_new is the largest number of rows of a
  * sequence as the host knows it, 1 for a decode step: a hint that chooses
- * kernels; whatever it is, every row is computed.  A block id outside the cache leaves its tokens out and
- * makes nimf_sync report device error 4.  Scores, softmax and sums are float32;
- * q and the probabilities enter the tensor cores as two fp16 terms each, the
- * codes exactly.  Results do not depend on timing.  Buffers 16-byte aligned. */
+ * kernels; whatever it is, every row is computed.  A block id outside the cache
+ * leaves its tokens out and makes nimf_sync report device error 4.  Scores,
+ * softmax and sums are float32; q and the probabilities enter the tensor cores as
+ * two fp16 terms each, the codes exactly.  Sequences of few rows take the first
+ * term of q from a grid of their row: a channel is held to 2^-22 of itself, one far
+ * below the row's largest to 2^-27 of that.  Results do not depend on timing.
+ * Buffers 16-byte aligned. */
 int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const float* q,
                            int64_t rows, int64_t n_heads, int64_t n_seqs, const int32_t* cu_rows,
                            const int32_t* lens, const int32_t* block_table, int64_t max_blocks,

@@ -16,11 +16,17 @@
 // accumulators' first value: -8 sum(q), and -8 sum(w) out of one MMA.
 //
 // The codes are the A operand (16 tokens, or 16 channels of the values), q and
-// w the B operand: 4 query rows a tile, each as two columns, an integer of 11
-// bits and the fp16 rest of it.  The tensor core cuts what an addition shifts
+// w the B operand: 4 query rows a tile, each as two columns, an integer that
+// fp16 holds and the fp16 rest of it.  The tensor core cuts what an addition shifts
 // out; sums of the integer columns stay below 2^24 and are exact, the rests
-// are small, and so products and sums have float32's accuracy.  w's integers
-// count from the largest w of the 32 tokens of a unit.
+// are small, and so products and sums have float32's accuracy.
+// q's integers are as large as those sums allow: a row's magnitudes add up to
+// 2^20 at most and none reaches 2^15 (fp16's end, with room for a rounding), so a
+// channel is off by 2^-22 of itself, or by 2^-13 of an integer's step where that is
+// more: 2^-27 of a row's largest channel if that one stands out (with 11 bits for
+// the largest it was 2^-23, and a channel a hundred times the others cost these
+// more than float32's sums do).  w's integers, of 11 bits, count from the largest w
+// of the 32 tokens of a unit, 2^-23 of which is nothing to their sum.
 //
 // Long contexts are bounded by HBM and by the ALU that masks the nibbles: 4
 // requests of 65,537 to 131,000 tokens and 8 KV heads of 128 take 91 us, 5.2 TB/s.
@@ -86,8 +92,10 @@ __device__ __forceinline__ int seq_tiles(int n, int r) {
   return (int)(((int64_t)n * r + ROWS - 1) / ROWS);
 }
 
-// An integer up to 2^11 (nearest, halves to even) and the rest of x.
+// The integer nearest to x (halves to even).
 __device__ __forceinline__ float int_part(float x) { return __fadd_rn(__fadd_rn(x, 12582912.f), -12582912.f); }
+// x's 11 leading bits (nearest): a whole number that fp16 holds, for a whole x below 2^15.
+__device__ __forceinline__ float lead_part(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -374,19 +382,22 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     float qsum[NB][NG], qc[NB][NG][2], row_f[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float amax = 0.f;
+      float amax = 0.f, asum = 0.f;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[nb][j][i] *= a.scale2;
           amax = fmaxf(amax, fabsf(x[nb][j][i]));
+          asum += fabsf(x[nb][j][i]);
         }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // the largest magnitude goes to [2^10, 2^11)
-      const int e = max(14, min(240, exp_field(amax)));
-      const float up = pow2_field(264 - e);
+      asum += __shfl_xor_sync(0xffffffffu, asum, 1);
+      asum += __shfl_xor_sync(0xffffffffu, asum, 2);
+      // the largest magnitude goes below 2^15, the sum of all below 2^20
+      const int e = max(14, min(240, max(exp_field(amax), exp_field(asum) - 5)));
+      const float up = pow2_field(268 - e);
       float sum[NG], grid[NG];              // of q, and of this column's fp16 values
 #pragma unroll
       for (int n = 0; n < NG; ++n) sum[n] = grid[n] = 0.f;
@@ -396,7 +407,7 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           sum[j * 32 / G] += x[nb][j][i];
-          const float v = x[nb][j][i] * up, hi = rintf(v);
+          const float v = x[nb][j][i] * up, hi = lead_part(rintf(v));
           y[i] = g & 1 ? v - hi : hi;
           if (i & 1) y[i] *= 0.0625f;       // odd nibbles count 16 times
         }
@@ -421,7 +432,7 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
         qc[nb][n][0] = __shfl_sync(0xffffffffu, grid[n], 8 * c) * -0x1p-21f;
         qc[nb][n][1] = __shfl_sync(0xffffffffu, grid[n], 8 * c + 4) * -0x1p-21f;
       }
-      row_f[nb] = __shfl_sync(0xffffffffu, pow2_field(e + 14), 8 * c);  // 2^24 / up
+      row_f[nb] = __shfl_sync(0xffffffffu, pow2_field(e + 10), 8 * c);  // 2^24 / up
     }
     int limit[NB];
 #pragma unroll

@@ -798,3 +798,75 @@ def test_shared_contexts_leave_out_blocks_that_are_not_there(nimf_gpu, torch_dev
         q = rng.standard_normal((new[0], heads, dim)).astype(F)
         got = attend_reported(torch_dev, nimf_gpu, pool, tab, lens, new, q, 0.2, max_new=new[0], out=torch_dev.full(q.shape, 5.0, device="cuda"))
         check_rows_over_missing(got, pool, tab, lens, new, q, 0.2)
+
+
+# ------------------------------------------------------------------ queries with one large channel
+def grid_query(dim, group, factor, seed):
+    """A query of one large channel and others of one size, and keys whose codes
+    have the others' signs or the opposite ones while the large channel's key is
+    0: roundings of the others' values that go one way add up.  Returns q [dim]
+    float32 times a softmax scale of 1, keys [2, dim] float32 that are coded
+    exactly ((code - 8) / 8), and the size's rounding in two fp16 terms on a grid
+    of 2^-11 of the large channel's power of two, the worst of 4,000 sizes."""
+    rng = np.random.default_rng(seed)
+    sign = np.where(rng.random(dim) < 0.5, -1.0, 1.0)
+    size = (1.0 + np.arange(4000) / 8000.0) / dim
+    v = (size.astype(F) * F(np.log2(np.e))).astype(F).astype(np.float64)
+    grid = 2.0 ** (np.floor(np.log2(v * factor)) - 10)
+    rest = v / grid - np.rint(v / grid)
+    lost = np.abs(rest - rest.astype(np.float16)) * grid / v
+    i = int(np.argmax(lost))
+    q = (size[i] * sign).astype(F)
+    keys = np.stack((0.5 * sign, -0.5 * sign)).astype(F)
+    for g in range(0, dim, group):
+        keys[:, g], keys[:, g + 1], keys[:, g + 2] = -1.0, 0.875, 0.0
+        q[g] = q[g + 1] = q[g + 2] = 0.0
+    for g in range(2, dim, group):
+        q[g] = F(size[i] * factor)
+    return q, keys, float(lost[i])
+
+
+def grid_query_bound(q, keys):
+    """s and the bound of tanh(s) that the test below derives."""
+    dim, u = len(q), 2.0 ** -24
+    x, k = np.abs(q.astype(np.float64)) * np.log2(np.e), np.abs(keys[0].astype(np.float64))
+    s = float(q.astype(np.float64) @ keys[0].astype(np.float64))
+    assert s == -float(q.astype(np.float64) @ keys[1].astype(np.float64))
+    g = max(2.0 ** -14 * x.max(), 2.0 ** -19 * x.sum())
+    e = (k * np.maximum(2.0 ** -12 * g, 2.0 ** -22 * x)).sum() + (dim / 4 + 17) * u * (k * x).sum()
+    e += dim / 4 * u * np.maximum(g / 2, 2.0 ** -11 * x).sum()
+    p = 1 / (1 + np.exp(-2 * s))
+    return s, 2 * p * (1 - p) * (2 * e * np.log(2) + 2.0 ** -22 + 4 * u * abs(s)) + 16 * u
+
+
+@pytest.mark.parametrize("dim,group", SHAPES)
+@pytest.mark.parametrize("factor", [8.0, 128.0, 1024.0])
+@pytest.mark.parametrize("heads", [1, 8, 20])
+def test_queries_with_a_large_channel_keep_the_small_ones(nimf_gpu, torch_dev, dim, group, factor, heads):
+    """A decoding query whose groups hold a channel 8 to 1,024 times the others:
+    the others keep their values.
+
+    Two tokens, whose scores are s and -s and whose values are 1 and -1 in every
+    channel: the output is tanh(s).  With u = 2^-24 and x = q scale log2(e):
+      a query's channel is held in two fp16 terms, the first a whole number of
+      steps g = max(2^-14 of the largest, 2^-19 of the sum of all |x|) at most
+      and within g / 2 or 2^-11 of x, the rest in 11 bits: off by
+      max(2^-12 g, 2^-22 |x|) a channel (and by u |x| for the product x);
+      the tensor core cuts each of D / 8 partial sums by 2u of it (of the codes
+      counted from 8 for the first terms, from 0 for the rests); scale, factors
+      and sums in float32 add 16u (kv4_reference.attention; the large channels'
+      keys and the codes' centres are 0 here).  So a base-2 score is off by
+        E = sum |k| max(2^-12 g, 2^-22 |x|) + (D / 4 + 17) u sum |k| |x|
+            + D / 4 u sum max(g / 2, 2^-11 |x|);
+      p is off by 2 E ln 2 + 2^-22 + 4u |s| of p (1 - p), and tanh(s) = 2 p - 1
+      by twice that, with 16u for its sums."""
+    q, keys, _ = grid_query(dim, group, factor, dim + group)
+    pool = R.Pool(1, 1, dim, 16, group)
+    for t in range(2):
+        pool.write(t, True, keys[t:t + 1])
+        pool.write(t, False, np.full((1, dim), 1 - 2 * t, F))
+    s, tol = grid_query_bound(q, keys)
+    qs = np.repeat(q[None, None], heads, 1)
+    got = attend(torch_dev, nimf_gpu, pool, np.array([[0]], np.int32), [2], [1], qs, 1.0)
+    err = np.abs(got[0].astype(np.float64) - np.tanh(s)).max()
+    assert err <= tol, float(err / tol)
