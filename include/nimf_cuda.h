@@ -410,9 +410,10 @@ int nimf_kv4_reserve_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_
                          int32_t* positions, int32_t* granted, void* stream);
 
 /* Puts the blocks of every request with finished[b] != 0 back on the stack (in
- * the order of the requests and their tables) and sets its lens[b] to 0.  More
- * blocks than n_blocks on the stack are dropped, which nimf_sync reports
- * (NIMF_ERR_TIMEOUT-class device error 5). */
+ * the order of the requests and their tables) and sets its lens[b] to 0.  Ids
+ * outside the cache are left out, and so are blocks that would make the stack
+ * longer than n_blocks; nimf_sync reports either (NIMF_ERR_TIMEOUT-class device
+ * errors 4 and 5). */
 int nimf_kv4_release_dev(const nimf_kv4_desc* desc, int64_t n_seqs, int64_t max_blocks,
                          const int32_t* finished, int32_t* lens, const int32_t* block_table,
                          int32_t* free_blocks, int32_t* n_free, void* stream);
@@ -453,8 +454,8 @@ int nimf_kv4_attention_workspace(const nimf_kv4_desc* desc, int64_t n_heads, int
  * softmax and sums are float32; q and the probabilities enter the tensor cores as
  * two fp16 terms each, the codes exactly.  Sequences of few rows take the first
  * term of q from a grid of their row: a channel is held to 2^-22 of itself, one far
- * below the row's largest to 2^-27 of that.  Results do not depend on timing.
- * Buffers 16-byte aligned. */
+ * below the row's largest to 2^-24 of that (2^-27 where few channels are large).
+ * Results do not depend on timing.  Buffers 16-byte aligned. */
 int nimf_kv4_attention_dev(const nimf_kv4_desc* desc, const void* cache, const float* q,
                            int64_t rows, int64_t n_heads, int64_t n_seqs, const int32_t* cu_rows,
                            const int32_t* lens, const int32_t* block_table, int64_t max_blocks,

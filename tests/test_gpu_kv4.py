@@ -870,3 +870,37 @@ def test_queries_with_a_large_channel_keep_the_small_ones(nimf_gpu, torch_dev, d
     got = attend(torch_dev, nimf_gpu, pool, np.array([[0]], np.int32), [2], [1], qs, 1.0)
     err = np.abs(got[0].astype(np.float64) - np.tanh(s)).max()
     assert err <= tol, float(err / tol)
+
+
+# ------------------------------------------------------------------ release of damaged tables
+@pytest.mark.parametrize("n,width,every", [(1, 3, 2), (5, 40, 7), (1500, 7, 3), (2, 3000, 1000), (3, 2100, 1)])
+def test_release_keeps_missing_blocks_off_the_stack(nimf_gpu, torch_dev, n, width, every):
+    """Tables with ids outside the cache: only blocks of the cache go back, in
+    their order, and nimf_sync reports the others; what is reserved next has
+    slots for all its rows."""
+    torch = torch_dev
+    rng = np.random.default_rng(n + width)
+    blocks, bs = n * width, 16
+    lens = np.full(n, width * bs, np.int32)
+    lens[n // 2] -= 5
+    done = np.ones(n, np.int32)
+    done[1::3] = 0
+    table = rng.permutation(blocks).astype(np.int32).reshape(n, width)
+    bad = np.arange(n * width).reshape(n, width) % every == every - 1
+    table[bad] = rng.choice(np.array([-1, -(2 ** 31), blocks, 2 ** 31 - 1]), bad.sum())
+    want = np.concatenate([table[b][~bad[b]] for b in range(n) if done[b]] + [np.zeros(0, np.int32)])
+    d = [up(torch, v) for v in (done, lens, table, np.full(blocks + 2048, -9, np.int32), np.array([0], np.int32))]
+    kv4 = nimf_gpu.KV4Cache(n_blocks=blocks, n_kv_heads=1, head_dim=64, block_size=bs, group=32)
+    kv4.release(n, width, *[t.data_ptr() for t in d], stream=1)
+    torch.cuda.synchronize()
+    with pytest.raises(nimf_gpu.CatchableError, match="code 4"):
+        nimf_gpu.check(nimf_gpu.lib().nimf_sync())
+    nimf_gpu.check(nimf_gpu.lib().nimf_sync())
+    free = d[3].cpu().numpy()
+    assert d[4].item() == len(want) and np.array_equal(free[:len(want)], want) and (free[blocks:] == -9).all()
+    assert np.array_equal(d[1].cpu().numpy(), np.where(done, 0, lens))
+    if len(want):
+        new = np.array([bs * min(len(want), 3)], np.int32)
+        got = run_reserve(torch, nimf_gpu, kv4, 1, 3, new, np.zeros(1, np.int32), np.full((1, 3), -1, np.int32), free[:blocks], len(want),
+                          int(new[0]), False)
+        assert got["granted"].tolist() == [1] and (got["slots"] >= 0).all() and (got["slots"] < blocks * bs).all()
