@@ -904,3 +904,22 @@ def test_release_keeps_missing_blocks_off_the_stack(nimf_gpu, torch_dev, n, widt
         got = run_reserve(torch, nimf_gpu, kv4, 1, 3, new, np.zeros(1, np.int32), np.full((1, 3), -1, np.int32), free[:blocks], len(want),
                           int(new[0]), False)
         assert got["granted"].tolist() == [1] and (got["slots"] >= 0).all() and (got["slots"] < blocks * bs).all()
+
+
+def test_release_writes_nothing_behind_the_stack(nimf_gpu, torch_dev):
+    """More blocks than the pool has: the words behind the stack stay."""
+    torch = torch_dev
+    for n, width, n_free in ((1, 3, 2), (3, 5000, 14000)):
+        kv4 = nimf_gpu.KV4Cache(n_blocks=max(4, n * width // 16 * 16), n_kv_heads=1, head_dim=64, block_size=16, group=32)
+        blocks = kv4.desc.n_blocks
+        lens, table = np.full(n, width * 16, np.int32), (np.arange(n * width, dtype=np.int32) % blocks).reshape(n, width)
+        free = np.full(blocks + 8192, 77, np.int32)
+        free[:n_free] = np.arange(n_free)
+        d = [up(torch, v) for v in (np.ones(n, np.int32), lens, table, free, np.array([n_free], np.int32))]
+        kv4.release(n, width, *[t.data_ptr() for t in d], stream=1)
+        torch.cuda.synchronize()
+        assert nimf_gpu.lib().nimf_sync() == -5
+        nimf_gpu.check(nimf_gpu.lib().nimf_sync())
+        got = d[3].cpu().numpy()
+        assert (got[blocks:] == 77).all() and d[4].item() == blocks
+        assert np.array_equal(got[:blocks], np.concatenate((np.arange(n_free), table.ravel()))[:blocks])
