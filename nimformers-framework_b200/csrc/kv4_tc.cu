@@ -322,7 +322,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (elect_one()) umma_commit(all_done);
       __syncwarp();
-      (void)warp_wait(all_done, 0);             // nothing in flight when TMEM is given back
+      // nothing is in flight when TMEM is given back, after an expired wait neither
+      for (uint32_t i = 0; i < kMaxSpin && !mbar_try_wait(all_done, 0); ++i) {}
+      __syncwarp();
     } else {
       // The three warps with nothing else to do look for blocks outside the cache,
       // beside the loads of q, so that softmax asks which tokens are missing only where
