@@ -329,16 +329,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // The three warps with nothing else to do look for blocks outside the cache,
       // beside the loads of q, so that softmax asks which tokens are missing only where
       // some are: asking in every tile took 1.5 % of a long prompt's time, this 0.4 %
-      // (2 % of a step with one row tile an SM).
+      // (1.4 % of a step whose row tiles have an SM each; 4 % with four entries of a
+      // lane in flight: more code, fetched cold).
       const int32_t* row_of_table = a.table + (int64_t)b * a.width;
       const uint32_t end = (uint32_t)min(seg_len, (t_first + nt) * N), per = (uint32_t)a.bs;
       bool missing = false;
-      for (uint32_t page = (uint32_t)(t_first * N) / per + (tid - 13 * 32); page * per < end; page += 4 * 96) {
-        int blk[4];
+      for (uint32_t page = (uint32_t)(t_first * N) / per + (tid - 13 * 32); page * per < end; page += 2 * 96) {
+        int blk[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) blk[i] = (page + i * 96) * per < end ? row_of_table[page + i * 96] : 0;
+        for (int i = 0; i < 2; ++i) blk[i] = (page + i * 96) * per < end ? row_of_table[page + i * 96] : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) missing |= blk[i] < 0 || blk[i] >= a.n_blocks;
+        for (int i = 0; i < 2; ++i) missing |= (uint32_t)blk[i] >= (uint32_t)a.n_blocks;
       }
       if (missing) s_missing = 1;
       __syncwarp();
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_arrive(q_full);
     named_barrier(2, 256 + 96);
     // all rows see the tiles up to here, and no block of theirs is missing
-    const int all_there = s_missing ? 0 : all_see;
+    const int all_there = s_missing ? INT32_MIN : all_see;
     // This lane: rows row0 and row0 + 8, of every 8 columns the pair 2 c, 2 c + 1.
     constexpr int NP = N / 8, OP = D / 8;
     const int row0 = quad * 32 + half * 16 + (lane >> 2);
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             x[j][i] = pk(base + 8 * j < limit[i] ? lo_of(x[j][i]) : -INFINITY,
                          base + 8 * j + 1 < limit[i] ? hi_of(x[j][i]) : -INFINITY);
         // (the weights of these need nothing more: scale and minimum are 0)
-        if (__builtin_expect(all_there == 0, 0)) {
+        if (__builtin_expect(all_there == INT32_MIN, 0)) {
 #pragma unroll
           for (int j = 0; j < NP; ++j)
             if (__float_as_uint(prm[4 * j].x) == 0x80000000u) x[j][0] = x[j][1] = pk(-INFINITY, -INFINITY);
