@@ -57,7 +57,9 @@ int stream_of(void* stream, cudaStream_t* st);
 int allow_smem(const void* kern, int bytes);
 
 // Launch with programmatic dependent launch allowed; every kernel launched
-// this way waits (griddep_wait) before it touches memory.
+// this way waits (griddep_wait) before it touches memory.  One does not:
+// attn_kernel<.., BESIDE = true>, which only tc_kernel precedes, relies on that
+// kernel having waited before it lets dependents start.
 template <typename... KArgs, typename... Args>
 int launch(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
            unsigned cluster, Args... args) {

@@ -185,8 +185,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     s_stop = s_missing = 0;
     mbar_fence_init();
   }
+  // In this order, and before any CTA returns: attn_kernel<.., BESIDE = true> starts
+  // when all CTAs are past here, and takes what came before this kernel for complete.
   griddep_wait();
-  griddep_launch_dependents();                  // attn_kernel: what came before is complete
+  griddep_launch_dependents();
   if (warp == 0) {
     // the items' number gives their parts, so the item of a CTA is known after it
     int b = 0, tile = 0, total = 0;
