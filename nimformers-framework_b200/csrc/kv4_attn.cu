@@ -62,7 +62,6 @@ struct SegInfo {
   int32_t kvh, tile;
   int32_t parts;    // join: CTAs that hold a part, counted from the one before
   int32_t second;   // join: the first of them holds it as its last segment
-  int32_t pad;
 };
 
 // What a CTA's end needs to know of its part of the line: how CTAs' parts are
@@ -707,7 +706,6 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
     while (last + 1 < l.ctas && cut(last + 1, l.each, l.more) < si.u1) ++last;
     si.parts = (int32_t)(last - (cta - 1) + 1);
     si.second = si.u0 > before;
-    si.pad = 0;
     if (si.u0 == l.begin || si.u0 < before) si.u0 = -1;
     info[cta] = si;
   }
@@ -865,10 +863,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a, int
   store_v<V>(a.out + ((si.row0 + tok) * a.h + hq) * D + lane * V, all.o, all.l == 0.f ? 0.f : 1.f / all.l);
 }
 
-int grid_of(int d, int ng, int nb) {
-  Context* c = ctx();
-  return (c ? c->num_sms : 148) * ctas_per_sm(d, ng, nb);
-}
+int grid_of(int d, int ng, int nb) { return ctx()->num_sms * ctas_per_sm(d, ng, nb); }
 
 size_t few_ws_bytes(int d) { return (ws_bytes(grid_of(d, 4, 1), d) + 255) / 256 * 256; }
 size_t all_ws_bytes(int d) { return few_ws_bytes(d) + (tc_serves(d) ? tc_ws_bytes(d) : 0); }

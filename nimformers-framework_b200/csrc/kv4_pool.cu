@@ -293,24 +293,7 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
-// VPL consecutive floats of a row.
-template <int VPL>
-__device__ __forceinline__ void load_row(const float* p, float (&x)[VPL]) {
-  if constexpr (VPL == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x;
-    x[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < VPL / 4; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = v.x;
-      x[4 * i + 1] = v.y;
-      x[4 * i + 2] = v.z;
-      x[4 * i + 3] = v.w;
-    }
-  }
-}
+// VPL consecutive floats into a row.
 template <int VPL>
 __device__ __forceinline__ void store_row(float* p, const float (&x)[VPL]) {
   if constexpr (VPL == 2) {
@@ -422,7 +405,7 @@ __global__ void __launch_bounds__(256)
     float x[HB][VPL];
 #pragma unroll
     for (int i = 0; i < HB; ++i)
-      if (HB == 1 || h0 + i < heads) load_row<VPL>(src + i * D, x[i]);
+      if (HB == 1 || h0 + i < heads) load_v<VPL>(src + i * D, x[i]);
     bool turn = true;
     if (cos_t) {
       const int64_t pos = positions[t];
@@ -430,8 +413,8 @@ __global__ void __launch_bounds__(256)
       if (!turn && lane == 0 && err) atomicExch(err, 4);
       if (turn && (is_q || is_k)) {
         float c[VPL], s[VPL];
-        load_row<VPL>(cos_t + pos * (D / 2) + (lane & 15) * VPL, c);
-        load_row<VPL>(sin_t + pos * (D / 2) + (lane & 15) * VPL, s);
+        load_v<VPL>(cos_t + pos * (D / 2) + (lane & 15) * VPL, c);
+        load_v<VPL>(sin_t + pos * (D / 2) + (lane & 15) * VPL, s);
 #pragma unroll
         for (int i = 0; i < HB; ++i) rotate<VPL>(x[i], c, s, lane);
       }
@@ -532,8 +515,7 @@ __global__ void __launch_bounds__(256)
 }
 
 unsigned warp_grid(int64_t items) {
-  Context* c = ctx();
-  const int64_t most = (int64_t)(c ? c->num_sms : 148) * 8;
+  const int64_t most = (int64_t)ctx()->num_sms * 8;
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, (items + 7) / 8));
 }
 

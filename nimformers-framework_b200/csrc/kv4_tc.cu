@@ -785,11 +785,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
-int sms() {
-  Context* c = ctx();
-  return c ? c->num_sms : 148;
-}
-
 template <int D, int NG>
 int run(const Args& a, unsigned char* ws, cudaStream_t st) {
   using L = TcLayout<D, NG>;
@@ -802,7 +797,7 @@ int run(const Args& a, unsigned char* ws, cudaStream_t st) {
 }  // namespace
 
 bool tc_serves(int d) { return d <= 128; }
-size_t tc_ws_bytes(int d) { return sms() * tc_part_floats(d) * 4; }
+size_t tc_ws_bytes(int d) { return ctx()->num_sms * tc_part_floats(d) * 4; }
 int64_t tc_items(const Args& a) {
   const int64_t rows = a.rows * a.r;
   return (rows / kTcRows + std::min<int64_t>(a.n_seqs, rows / (a.big + 1))) * a.hkv;

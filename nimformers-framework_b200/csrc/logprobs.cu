@@ -48,7 +48,6 @@ struct LpArgs {
   int32_t* rank;
   int32_t* top_ids;
   float* top_lp;
-  int* err;
   int64_t vocab;
   int slice, top;
 };
@@ -487,7 +486,7 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
     return set_error(NIMF_ERR_ARG, "logprobs: NULL buffer");
   NIMF_TRY(kv4::stream_of(stream, &st));
   // A CTA a row; several where the rows do not fill the SMs, up to two CTAs an SM,
-  // as long as a thread keeps four float4s.
+  // as long as a thread keeps two float4s.
   unsigned ctas = 1;
   while (ctas < (unsigned)kLpMaxCluster && rows * ctas <= ctx()->num_sms && vocab / ctas > 4 * kLpThreads * kLpAhead)
     ctas *= 2;
@@ -499,7 +498,6 @@ extern "C" int nimf_logprobs_dev(const float* logits, int64_t rows, int64_t voca
   a.rank = rank;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  a.err = ctx()->dev_err;
   a.vocab = vocab;
   a.slice = (int)(((vocab + ctas - 1) / ctas + 3) & ~(int64_t)3);
   a.top = (int)n_top;
