@@ -28,10 +28,13 @@
 // more than float32's sums do).  w's integers, of 11 bits, count from the largest w
 // of the 32 tokens of a unit, 2^-23 of which is nothing to their sum.
 //
+// Times are those of captured calls over two sets of buffers in turn.
 // Long contexts are bounded by HBM and by the ALU that masks the nibbles: 4
-// requests of 65,537 to 131,000 tokens and 8 KV heads of 128 take 91 us, 5.2 TB/s.
+// requests of 65,537 to 131,000 tokens and 8 KV heads of 128 take 91 us, 5.2 TB/s
+// (102 us, 4.6 TB/s, where every call has buffers of its own).
 // Short calls are latency, from the plan to the join: 64 ragged requests up to
-// 4,096 tokens 22 us, one of 519 tokens with 32 KV heads 9.7 us.
+// 4,096 tokens 22.4 us (16 heads of 256 over 4: 29), one of 519 tokens with 32 KV
+// heads 9.9 us.
 #include <algorithm>
 #include <cfloat>
 
@@ -901,8 +904,11 @@ int run_attn(const Args& a, int64_t max_new, cudaStream_t st) {
 }
 
 // Rows a KV head from which a sequence is worth the tensor-core kernel's tiles
-// of 128: such a tile costs about what 16 rows cost here (1.1 against 1.2 us
-// for 128 tokens of a 128-channel head).
+// of 128.  With one group a head such a tile costs about what 16 rows cost here: 64
+// ragged requests up to 4,096 tokens, 8 KV heads of 128, 20 rows of each a head
+// take 121 us there and 132 here.  Finer groups shrink its tiles of tokens, which
+// this rule leaves out: with groups of 64 the kernels meet at about 36 rows (20 rows
+// 170 and 157 us), with groups of 32 at about 44 (312 and 225).
 constexpr int kBigRows = 16;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

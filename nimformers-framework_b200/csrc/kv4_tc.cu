@@ -23,8 +23,9 @@
 // four times as many of them, which alone took longer than the products.
 //
 // Bounded by that chain of a softmax warp, 3 us a tile of 128 tokens; the tensor
-// cores are 39 % busy: 2,048 rows of 6,144 tokens with 32 heads of 128 take 426 us
-// (403 TFLOP/s with every product counted once), with groups of 64 725 us.
+// cores are 39 % busy: 2,048 rows of 6,144 tokens with 32 heads of 128 take 429 us
+// (400 TFLOP/s with every product counted once), with groups of 64 706 us, of 32
+// 1,353 us (captured calls over two sets of buffers).
 #include <algorithm>
 #include <type_traits>
 

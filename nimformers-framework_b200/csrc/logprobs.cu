@@ -15,8 +15,9 @@
 // candidates, for which the threads that reach the bound read their shares again
 // (out of L2).  Bounded by HBM; a slice kept in shared memory instead cost 64 KB
 // a CTA, loads and passes took turns, and 4,096 rows of 32,000 took 230 us; they
-// take 92 us now (5.7 TB/s), 64 rows of 128,001 with 20 alternatives 12.5 us, one
-// row of 32,000 6.2 us, both of these latency.
+// take 92 us now (5.7 TB/s; 102 us with buffers of its own for every call), 64 rows
+// of 128,001 with 20 alternatives 12.5 us, one row of 32,000 6.2 us, both of these
+// latency (times of captured calls).
 #include <cfloat>
 
 #include "kv4.cuh"
