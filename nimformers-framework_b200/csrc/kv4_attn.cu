@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(warps_of(D, NG, NB) * 32, ctas_per_sm(D, NG, N
       asum += __shfl_xor_sync(0xffffffffu, asum, 1);
       asum += __shfl_xor_sync(0xffffffffu, asum, 2);
       // the largest magnitude goes below 2^15, the sum of all below 2^20
-      const int e = max(14, min(240, max(exp_field(amax), exp_field(asum) - 5)));
+      const int e = max(14, min(244, max(exp_field(amax), exp_field(asum) - 5)));
       const float up = pow2_field(268 - e);
       float sum[NG], grid[NG];              // of q, and of this column's fp16 values
 #pragma unroll

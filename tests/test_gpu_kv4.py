@@ -872,6 +872,32 @@ def test_queries_with_a_large_channel_keep_the_small_ones(nimf_gpu, torch_dev, d
     assert err <= tol, float(err / tol)
 
 
+@pytest.mark.parametrize("dim,group", SHAPES)
+@pytest.mark.parametrize("size", [1e30, 1e35])
+def test_queries_near_the_largest_floats(nimf_gpu, torch_dev, dim, group, size):
+    """Scores so far apart that one token has all the weight: the output is its
+    value, whose sum is off as in kv4_reference.attention without an error of p
+    (p is 1), for queries up to 2^118 or so."""
+    rng = np.random.default_rng(dim + group)
+    blocks, tab = layout(rng, [50], 16)
+    pool = R.Pool(blocks, 1, dim, 16, group, rng)
+    fill(pool, rng)
+    q = (rng.uniform(-2, 2, (1, 3, dim)) * size).astype(F)
+    got = attend(torch_dev, nimf_gpu, pool, tab, [50], [1], q, 1.0)
+    full = []
+    for key in (True, False):
+        code, sc, low = pool.tokens(tab[0], 50, key)
+        sc, low = (a.astype(np.float64).repeat(group, -1)[:, 0] for a in (sc, low))
+        full.append((code[:, 0] * sc + low, np.abs(code[:, 0] - 8.0) * sc + np.abs(low + 8 * sc)))
+    (k, _), (v, va) = full
+    for h in range(3):
+        s = k @ q[0, h].astype(np.float64)
+        i = int(np.argmax(s))
+        assert s[i] - np.partition(s, -2)[-2] > 1e-4 * np.abs(s).max()
+        tol = va[i] * (2.0 ** -22 + 10 * 2.0 ** -24 + 8 * 2.0 ** -24 * (50 / 32 + 8) + 2.0 ** -23)
+        assert (np.abs(got[0, h] - v[i]) <= tol).all()
+
+
 # ------------------------------------------------------------------ release of damaged tables
 @pytest.mark.parametrize("n,width,every", [(1, 3, 2), (5, 40, 7), (1500, 7, 3), (2, 3000, 1000), (3, 2100, 1)])
 def test_release_keeps_missing_blocks_off_the_stack(nimf_gpu, torch_dev, n, width, every):
